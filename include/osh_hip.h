@@ -45,6 +45,12 @@ typedef void *osh_event;  /* hipEvent_t */
  * GraphFusion.FuseActivationIntoProducer moves into a producer
  * (src/OnnxSharp/Core/GraphFusion.cs:1713-1718). */
 enum { OSH_ACT_NONE = 0, OSH_ACT_RELU = 1, OSH_ACT_SILU = 2, OSH_ACT_SIGMOID = 3 };
+/* x (1 + erf(x / sqrt 2)) / 2; osh_quant_matmul only. */
+enum { OSH_ACT_GELU = 4 };
+
+/* Element types of the language-model operators (e4m3: 8-bit floats without
+ * infinities, largest value 448, as torch.float8_e4m3fn). */
+enum { OSH_T_F32 = 0, OSH_T_F16 = 1, OSH_T_BF16 = 2, OSH_T_I8 = 3, OSH_T_E4M3 = 4 };
 
 /* ONNX auto_pad (src/OnnxSharp/Ops/DnnOps.cs:69-89). */
 enum { OSH_PAD_NOTSET = 0, OSH_PAD_SAME_UPPER = 1, OSH_PAD_SAME_LOWER = 2, OSH_PAD_VALID = 3 };
@@ -578,6 +584,73 @@ OSH_API osh_status osh_softmax_f32(int64_t rows, int cols, float scale, const fl
  * overlap qkv. */
 OSH_API osh_status osh_attention_f32(int heads, int key_dim, int head_dim, int n, float scale, const float *d_qkv,
                                      int64_t head_stride, float *d_y, osh_stream s);
+
+/* ------------------------------------------------ language-model operators */
+/* The operators of a served decoder block.  The reference has none of them: its
+ * attention and normalization run as FP32 node sequences.  None allocates or
+ * synchronizes, so all can be captured into a graph. */
+
+/* RMS norm of rows [rows][cols] (type dtype: f32, f16, bf16; pitches in elements),
+ * with the residual's addition, into 8-bit rows with scales (q_type: i8, e4m3):
+ *   h = round(x + res), or x when d_res is NULL (d_h is then not touched);
+ *   y = h / sqrt(mean(h^2) + eps) * gamma;
+ *   scale[row] = max|y| / top (top = 127, 448);  q = round(y / scale), half to even.
+ * h may be x or res themselves; no other overlap of an output.  A row of zeros
+ * gets scale 0 and zeros; a NaN or an infinity in a row makes its scale NaN.
+ * cols <= 32768; any alignment of whole elements. */
+OSH_API osh_status osh_rms_norm_quant(int64_t rows, int cols, int dtype, const void *d_x, int64_t ldx,
+                                      const void *d_res, int64_t ldr, const void *d_gamma, float eps, void *d_h,
+                                      int64_t ldh, int q_type, void *d_q, int64_t ldq, float *d_scale,
+                                      osh_stream s);
+
+/* Product of 8-bit rows with its epilogue, y [m][n] of type dtype (f32, f16, bf16):
+ *   y[i][j] = act(sum_k a[i][k] w[j][k] * sa[i] * sw[j] + bias[j]) + res[i][j]
+ * a [m][k] and w [n][k] both i8 (int32 sums, k <= 131071) or both e4m3 (FP32 sums),
+ * k contiguous, any pitch and alignment; sa, sw, bias FP32; bias and res (of type
+ * dtype) may be NULL; act: none, relu, silu or gelu.  res may be y itself (same
+ * pitch); no other overlap of y. */
+OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void *d_a, int64_t lda, const float *d_sa,
+                                    const void *d_w, int64_t ldw, const float *d_sw, const float *d_bias, int act,
+                                    int dtype, const void *d_res, int64_t ldr, void *d_y, int64_t ldy, osh_stream s);
+
+/* Causal attention with a sliding window and first tokens that stay visible
+ * (sinks), over a paged cache.  Sequence b brings d_cu[b+1] - d_cu[b] new tokens
+ * (rows d_cu[b].. of q, k_new, v_new and o) and holds d_kl[b] tokens with them.
+ * Its token at position p lies at slot p % page of page d_table[b][p / page].
+ * The call writes the new keys and values to their pages and computes, for the
+ * query at position p,
+ *   o = softmax over the visible j of (q . k_j * scale) times v_j,
+ *   visible: j <= p and (j > p - window or j < sinks).
+ * Query head h reads key head h / (q_heads / kv_heads).  Sums, softmax and its
+ * statistics are FP32; the weights are rounded to dtype for the product with v.
+ * Pages and slots that no query of the call sees are not read (stale entries of
+ * d_table before the window may hold anything).  A new token's slot must belong
+ * to its sequence alone.
+ * max_q and max_kv are the host's bounds of the lengths.  A sequence whose lengths
+ * contradict each other, the bounds or the table, and a query that sees a page id
+ * outside [0, pages), get NaN; nothing out of range is read or written.
+ * Strides are in elements, the head_dim values of a head contiguous, any alignment
+ * of whole elements.  head_dim % 8 == 0 and <= 256, dtype f16 or bf16. */
+typedef struct osh_window_attn {
+    int dtype, batch, q_heads, kv_heads, head_dim;
+    int window, sinks;            /* window >= 1, sinks >= 0 */
+    int max_q, max_kv;
+    int pages, page, table_width; /* pages of page slots; table_width entries a sequence */
+    float scale;                  /* 0 = 1 / sqrt(head_dim) */
+    int reserved;                 /* 0 */
+    int64_t tokens;               /* rows of q, k_new, v_new, o */
+    const void *d_q, *d_k_new, *d_v_new;
+    void *d_o;
+    void *d_k_pages, *d_v_pages;
+    const int32_t *d_table, *d_cu, *d_kl;
+    int64_t q_stride[2], k_new_stride[2], v_new_stride[2], o_stride[2]; /* token, head */
+    int64_t k_stride[3], v_stride[3];                                   /* page, slot, head */
+    int64_t table_stride;
+} osh_window_attn;
+/* Scratch of osh_window_attention (0 where one launch does it all); depends on the
+ * sizes only.  d_scratch may be NULL when it is 0. */
+OSH_API osh_status osh_window_attention_scratch_bytes(const osh_window_attn *p, size_t *bytes);
+OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratch, osh_stream s);
 
 /* ----------------------------------------------------------- HIP graphs */
 /* A segment's launches recorded once and replayed per Forward, the role of

@@ -1,0 +1,286 @@
+// osh_quant_matmul.hip -- product of 8-bit rows with its epilogue:
+//
+//   y[i][j] = act(sa[i] sw[j] sum_k a[i][k] w[j][k] + bias[j]) + res[i][j]
+//
+// with a [m][k] and w [n][k], k contiguous in both.  The weights are the MFMA's
+// A operand and the activations its B operand, so a lane ends with four
+// neighbouring outputs of one row.
+//
+// A k-block is 128 bytes of a row, eight chunks of 16.  Lane (l % 16, g = l / 16)
+// holds chunks g and g + 4 of its row: int8 multiplies them with two
+// v_mfma_i32_16x16x64_i8, e4m3 with one v_mfma_f32_16x16x128_f8f6f4.  Which k
+// a byte stands for is the same for both operands, so the sum does not care that
+// the hardware numbers a lane's bytes otherwise.
+#include <algorithm>
+
+#include "osh_lm.h"
+
+using namespace osh;
+
+namespace osh {
+
+struct QmmArgs {
+    int m, n, k, act;
+    long long lda, ldw, ldr, ldy;
+    const unsigned char *a, *w;
+    const float *sa, *sw, *bias;
+    const void *res;
+    void *y;
+};
+
+constexpr int KB = 128;  // bytes of a k-block
+
+template <int Q> struct QAcc { using type = f32x4; };
+template <> struct QAcc<OSH_T_I8> { using type = i32x4; };
+
+struct Frag {
+    i32x4 lo, hi;  // chunks g and g + 4 of a row's k-block
+};
+
+template <int Q>
+__device__ __forceinline__ typename QAcc<Q>::type mma(const Frag &w, const Frag &a, typename QAcc<Q>::type c) {
+    if constexpr (Q == OSH_T_I8) {
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.lo, a.lo, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(w.hi, a.hi, c, 0, 0, 0);
+    } else {
+        const i32x8 w8 = __builtin_shufflevector(w.lo, w.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        const i32x8 a8 = __builtin_shufflevector(a.lo, a.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a8, c, 0, 0, 0, 0, 0, 0);
+    }
+}
+
+// 16 bytes of a row from byte k0, zero from byte k on.
+__device__ __forceinline__ i32x4 load_chunk(const unsigned char *row, int k0, int k) {
+    i32x4 v = {0, 0, 0, 0};
+    if (k0 + 16 <= k) {
+        __builtin_memcpy(&v, row + k0, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 15; i++)
+            if (k0 + i < k) v[i >> 2] |= (int)row[k0 + i] << (8 * (i & 3));
+    }
+    return v;
+}
+
+__device__ __forceinline__ float apply_act(int act, float v) {
+    switch (act) {
+    case OSH_ACT_RELU: return v > 0.0f || v != v ? v : 0.0f;
+    case OSH_ACT_SILU: return v / (1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+    case OSH_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    default: return v;
+    }
+}
+
+// One output from its sum; scale, bias, activation and residual in FP32, one
+// rounding to T.
+template <typename T>
+__device__ __forceinline__ T finish(const QmmArgs &p, float sum, int row, int col, float sa) {
+    float v = sum * sa * p.sw[col];
+    if (p.bias) v += p.bias[col];
+    v = apply_act(p.act, v);
+    if (p.res) v += (float)static_cast<const T *>(p.res)[row * p.ldr + col];
+    return (T)v;
+}
+
+// Tile of BM rows by BN outputs, WM x WN waves; k-blocks pass through two LDS
+// buffers.  Chunk c of tile row r lies at slot c ^ (r / 2 % 8) of the row's 128
+// bytes: the 16 lanes of an operand read then meet all 64 banks once.
+template <int Q, typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
+    constexpr int THREADS = 64 * WM * WN;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int CH = (BM + BN) * 8 / THREADS;  // chunks a thread stages
+    using Acc = typename QAcc<Q>::type;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jl = lane & 15, g = lane >> 4;
+    const int tiles_m = cdiv(p.m, BM);
+    const int id = xcd_band(blockIdx.x, gridDim.x);
+    const int m0 = id % tiles_m * BM, n0 = id / tiles_m * BN;
+    const int wm = wave % WM, wn = wave / WM;
+
+    const unsigned char *src[CH];
+    int dst[CH];
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+        const int c = tid + THREADS * i, r = c >> 3;
+        src[i] = r < BM ? p.a + (long long)min(m0 + r, p.m - 1) * p.lda
+                        : p.w + (long long)min(n0 + r - BM, p.n - 1) * p.ldw;
+        dst[i] = r * KB + (((c & 7) ^ (r >> 1 & 7)) << 4);
+    }
+    i32x4 st[CH];
+    auto load = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) st[i] = load_chunk(src[i], kb * KB + (tid & 7) * 16, p.k);
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) *reinterpret_cast<i32x4 *>(lds + buf * (BM + BN) * KB + dst[i]) = st[i];
+    };
+    auto frag = [&](int buf, int r) {
+        const unsigned char *row = lds + buf * (BM + BN) * KB + r * KB;
+        Frag f;
+        f.lo = *reinterpret_cast<const i32x4 *>(row + ((g ^ (r >> 1 & 7)) << 4));
+        f.hi = *reinterpret_cast<const i32x4 *>(row + (((g + 4) ^ (r >> 1 & 7)) << 4));
+        return f;
+    };
+
+    Acc acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = Acc{0, 0, 0, 0};
+
+    const int nkb = cdiv(p.k, KB);
+    load(0);
+    store(0);
+    __syncthreads();
+    for (int kb = 0; kb < nkb; kb++) {
+        if (kb + 1 < nkb) load(kb + 1);
+        Frag fa[FM];
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[i] = frag(kb & 1, wm * (BM / WM) + 16 * i + jl);
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+            const Frag fw = frag(kb & 1, BM + wn * (BN / WN) + 16 * j + jl);
+#pragma unroll
+            for (int i = 0; i < FM; i++) acc[i][j] = mma<Q>(fw, fa[i], acc[i][j]);
+        }
+        if (kb + 1 < nkb) store((kb + 1) & 1);
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const int row = m0 + wm * (BM / WM) + 16 * i + jl;
+        if (row >= p.m) continue;
+        const float sa = p.sa[row];
+        T *y = static_cast<T *>(p.y) + row * p.ldy;
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+            const int col = n0 + wn * (BN / WN) + 16 * j + 4 * g;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (col + r < p.n) y[col + r] = finish<T>(p, (float)acc[i][j][r], row, col + r, sa);
+        }
+    }
+}
+
+// Few rows: a workgroup takes 16 outputs of all rows (up to 16 MB), its waves
+// every WAVES-th k-block; the weights go from memory to registers, each byte once.
+// The waves' sums meet in LDS, in the order of the waves.
+template <int Q, typename T, int MB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void qmm_rows_kernel(QmmArgs p) {
+    using Acc = typename QAcc<Q>::type;
+    __shared__ Acc part[WAVES][MB][64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jl = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const unsigned char *w = p.w + (long long)min(n0 + jl, p.n - 1) * p.ldw;
+    const unsigned char *a[MB];
+    Acc acc[MB];
+#pragma unroll
+    for (int i = 0; i < MB; i++) {
+        a[i] = p.a + (long long)min(16 * i + jl, p.m - 1) * p.lda;
+        acc[i] = Acc{0, 0, 0, 0};
+    }
+    const int nkb = cdiv(p.k, KB);
+    for (int kb = wave; kb < nkb; kb += WAVES) {
+        const int k0 = kb * KB + 16 * g;
+        Frag fw{load_chunk(w, k0, p.k), load_chunk(w, k0 + 64, p.k)};
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            const Frag fa{load_chunk(a[i], k0, p.k), load_chunk(a[i], k0 + 64, p.k)};
+            acc[i] = mma<Q>(fw, fa, acc[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MB; i++) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int e = tid; e < MB * 256; e += 64 * WAVES) {
+        const int i = e >> 8, r = e & 3, g4 = e >> 2 & 3, row = 16 * i + (e >> 4 & 15), col = n0 + 4 * g4 + r;
+        auto sum = part[0][i][(e >> 4 & 15) + 16 * g4][r];
+#pragma unroll
+        for (int v = 1; v < WAVES; v++) sum += part[v][i][(e >> 4 & 15) + 16 * g4][r];
+        if (row < p.m && col < p.n)
+            static_cast<T *>(p.y)[row * p.ldy + col] = finish<T>(p, (float)sum, row, col, p.sa[row]);
+    }
+}
+
+template <int Q, typename T>
+static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
+#define OSH_QMM_TILE(BM, BN, WM, WN)                                                                  \
+    OSH_LAUNCH((qmm_tile_kernel<Q, T, BM, BN, WM, WN>), dim3((unsigned)(cdiv(p.m, BM) * cdiv(p.n, BN))), \
+               dim3(64 * WM * WN), 2 * (BM + BN) * KB, st, p)
+    if (p.m <= 16)
+        OSH_LAUNCH((qmm_rows_kernel<Q, T, 1, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
+    else if (p.m <= 32)
+        OSH_LAUNCH((qmm_rows_kernel<Q, T, 2, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
+    else if ((long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
+        OSH_QMM_TILE(128, 128, 2, 2);
+    else
+        OSH_QMM_TILE(64, 64, 2, 2);
+#undef OSH_QMM_TILE
+    OSH_LAUNCH_CHECK("qmm kernel");
+    return OSH_OK;
+}
+
+template <int Q>
+static osh_status qmm_launch_t(const QmmArgs &p, int dtype, hipStream_t st) {
+    if (dtype == OSH_T_F32) return qmm_launch<Q, float>(p, st);
+    if (dtype == OSH_T_F16) return qmm_launch<Q, _Float16>(p, st);
+    return qmm_launch<Q, __bf16>(p, st);
+}
+
+}  // namespace osh
+
+extern "C" {
+
+OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void *d_a, int64_t lda, const float *d_sa,
+                                    const void *d_w, int64_t ldw, const float *d_sw, const float *d_bias, int act,
+                                    int dtype, const void *d_res, int64_t ldr, void *d_y, int64_t ldy, osh_stream s) {
+    if (m < 0 || n < 0 || k < 0) return fail(OSH_E_INVALID, "QuantMatMul: negative sizes");
+    if (q_type != OSH_T_I8 && q_type != OSH_T_E4M3) return fail(OSH_E_INVALID, "QuantMatMul: operands are i8 or e4m3");
+    if (dtype != OSH_T_F32 && dtype != OSH_T_F16 && dtype != OSH_T_BF16)
+        return fail(OSH_E_INVALID, "QuantMatMul: outputs are f32, f16 or bf16");
+    if (act != OSH_ACT_NONE && act != OSH_ACT_RELU && act != OSH_ACT_SILU && act != OSH_ACT_GELU)
+        return fail(OSH_E_INVALID, "QuantMatMul: unknown activation %d", act);
+    if (m == 0 || n == 0) return OSH_OK;
+    if (k == 0) return fail(OSH_E_INVALID, "QuantMatMul: k is 0");
+    // 131071 products of -128 and -128 stay below 2^31
+    if (q_type == OSH_T_I8 && k > 131071) return fail(OSH_E_UNSUPPORTED, "QuantMatMul: k = %d above 131071", k);
+    if (k > (1 << 30)) return fail(OSH_E_UNSUPPORTED, "QuantMatMul: k = %d too long", k);
+    if (!d_a || !d_sa || !d_w || !d_sw || !d_y) return fail(OSH_E_INVALID, "QuantMatMul: NULL pointer");
+    if (lda < k || ldw < k || ldy < n || (d_res && ldr < n))
+        return fail(OSH_E_INVALID, "QuantMatMul: a row pitch below the columns");
+    if ((long long)cdiv(m, 64) * cdiv(n, 64) >= (1LL << 23))
+        return fail(OSH_E_UNSUPPORTED, "QuantMatMul: %d x %d outputs", m, n);
+    const long long e = elem_bytes(dtype), by = ((m - 1LL) * ldy + n) * e;
+    if (ranges_overlap(d_y, by, d_a, (m - 1LL) * lda + k) || ranges_overlap(d_y, by, d_w, (n - 1LL) * ldw + k) ||
+        ranges_overlap(d_y, by, d_sa, m * 4LL) || ranges_overlap(d_y, by, d_sw, n * 4LL) ||
+        ranges_overlap(d_y, by, d_bias, n * 4LL) ||
+        (ranges_overlap(d_y, by, d_res, ((m - 1LL) * ldr + n) * e) && !(d_y == d_res && ldy == ldr)))
+        return fail(OSH_E_INVALID, "QuantMatMul: y overlaps an operand");
+    QmmArgs p;
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.act = act;
+    p.lda = lda;
+    p.ldw = ldw;
+    p.ldr = ldr;
+    p.ldy = ldy;
+    p.a = static_cast<const unsigned char *>(d_a);
+    p.w = static_cast<const unsigned char *>(d_w);
+    p.sa = d_sa;
+    p.sw = d_sw;
+    p.bias = d_bias;
+    p.res = d_res;
+    p.y = d_y;
+    return q_type == OSH_T_I8 ? qmm_launch_t<OSH_T_I8>(p, dtype, to_stream(s))
+                              : qmm_launch_t<OSH_T_E4M3>(p, dtype, to_stream(s));
+}
+
+}  // extern "C"

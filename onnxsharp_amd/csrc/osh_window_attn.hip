@@ -1,0 +1,373 @@
+// osh_window_attn.hip -- causal attention with a sliding window and sinks over a
+// paged cache (osh_window_attention).
+//
+// The G = q_heads / kv_heads query heads of a key head read the same keys, so a
+// sequence's queries at one key head form a matrix of ql * G rows (row = token * G
+// + head of the group), taken 16 rows a workgroup.  For a row block the visible
+// keys are the sinks below the window and one range; "key number" v counts them:
+// v < se is key v, the others are key v - se + lo.
+//
+// Softmax in one pass: each row keeps its running maximum m, the sum l of
+// 2^(s - m) and the weighted sum of values; a larger maximum rescales both by
+// 2^(m_old - m).  Waves and splits that saw different keys are joined by the same
+// rule.
+#include <algorithm>
+
+#include "osh_lm.h"
+#include "osh_window_addr.h"
+
+using namespace osh;
+
+namespace osh {
+
+struct WinArgs {
+    osh_window_attn p;
+    int group, tiles, splits;
+    float scale_log2;
+    float *part_o, *part_ml;  // of a split: [unit][split][16][head_dim], [unit][split][16][2]
+};
+
+template <typename T> struct Half8;
+template <> struct Half8<_Float16> { using type = f16x8; };
+template <> struct Half8<__bf16> { using type = bf16x8; };
+
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// One workgroup: 16 query rows of one key head, one split of their keys; each
+// wave takes every WAVES-th step of 32 keys of the split.
+//
+// A step's scores are S^T = K Q^T, two MFMAs' rows of 16 keys.  MFMA row rho of
+// block b is key 8 (rho / 4) + 4 b + rho % 4 of the step, so that lane (jl, g) ends
+// with the scores of keys 8 g .. 8 g + 7 at query jl: just the operand of
+// O^T = V^T P^T, without a move between lanes.  A lane loads ND neighbouring values
+// of its 8 keys of V and turns the 8 x ND block around in registers; MFMA i then
+// takes values ND jl + i of all lanes.
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a) {
+    constexpr int NS = DP > 128 ? 2 : 1;       // sets of up to 128 values
+    constexpr int ND = DP >= 128 ? 8 : 4;      // neighbouring values of a lane in a set
+    constexpr int KS = DP / 32;                // MFMA steps over the head's values
+    using H8 = typename Half8<T>::type;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const osh_window_attn &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jl = lane & 15, g = lane >> 4;
+    const int d = p.head_dim, G = a.group;
+
+    int id = blockIdx.x;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int unit = id;
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int h = id % p.kv_heads, b = id / p.kv_heads;
+    const WinSeq sq = win_seq(p, b);
+    const int rows = sq.ql * G, r0 = tile * 16;
+    if (r0 >= rows) return;
+    T *o = static_cast<T *>(p.d_o);
+    const int my_row = r0 + jl, my_tok = min(my_row, rows - 1) / G, my_head = h * G + min(my_row, rows - 1) % G;
+    if (!sq.ok) {
+        if (split == 0)
+            for (int e = tid; e < 16 * d; e += 64 * WAVES) {
+                const int r = r0 + e / d;
+                if (r < rows)
+                    o[(long long)(sq.c0 + r / G) * p.o_stride[0] + (h * G + r % G) * p.o_stride[1] + e % d] =
+                        (T)__builtin_nanf("");
+            }
+        return;
+    }
+    const T *kn = static_cast<const T *>(p.d_k_new), *vn = static_cast<const T *>(p.d_v_new);
+    T *kp = static_cast<T *>(p.d_k_pages), *vp = static_cast<T *>(p.d_v_pages);
+
+    // the tokens whose first row lies in this block go to their pages
+    if (split == 0) {
+        const int t0 = (r0 + G - 1) / G, t1 = min((r0 + 16 + G - 1) / G, sq.ql);
+        const int chunks = d / 8;
+        for (int e = tid; e < (t1 - t0) * chunks; e += 64 * WAVES) {
+            const int t = t0 + e / chunks, c = e % chunks * 8;
+            const long long ko = win_cache_at(p, b, sq.past + t, p.k_stride, h);
+            const long long vo = win_cache_at(p, b, sq.past + t, p.v_stride, h);
+            if (ko < 0) continue;
+            const long long row = sq.c0 + t;
+            __builtin_memcpy(kp + ko + c, kn + row * p.k_new_stride[0] + h * p.k_new_stride[1] + c, 16);
+            __builtin_memcpy(vp + vo + c, vn + row * p.v_new_stride[0] + h * p.v_new_stride[1] + c, 16);
+        }
+    }
+
+    // queries: lane (jl, g) holds values 32 s + 8 g .. + 7 of row jl
+    H8 q[KS];
+    {
+        const T *qr = static_cast<const T *>(p.d_q) + (long long)(sq.c0 + my_tok) * p.q_stride[0] +
+                      my_head * p.q_stride[1];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            q[s] = H8{};
+            if (32 * s + 8 * g < d) __builtin_memcpy(&q[s], qr + 32 * s + 8 * g, 16);
+        }
+    }
+    const int last = min(r0 + 15, rows - 1);
+    const WinKeys keys = win_keys(p, sq, r0 / G, last / G);
+    const int nv = keys.count;
+    const int steps = cdiv(nv, 32), per = cdiv(steps, a.splits);
+    const int s_end = min(steps, (split + 1) * per);
+    const int my_pos = sq.past + my_tok;
+
+    float m = -__builtin_inff(), l = 0.0f;
+    f32x4 acc[NS][ND];
+#pragma unroll
+    for (int n = 0; n < NS; n++)
+#pragma unroll
+        for (int i = 0; i < ND; i++) acc[n][i] = f32x4{0, 0, 0, 0};
+
+    const T **at = reinterpret_cast<const T **>(lds) + wave * 64;  // a step's rows of K, then of V
+    for (int st = split * per + wave; st < s_end; st += WAVES) {
+        {
+            const int v = st * 32 + (lane & 31), j = keys.at(v);
+            const bool is_v = lane >= 32;
+            const T *row = nullptr;
+            if (v < nv) {
+                if (j >= sq.past) {
+                    const long long t = sq.c0 + j - sq.past;
+                    row = is_v ? vn + t * p.v_new_stride[0] + h * p.v_new_stride[1]
+                               : kn + t * p.k_new_stride[0] + h * p.k_new_stride[1];
+                } else {
+                    const long long off = win_cache_at(p, b, j, is_v ? p.v_stride : p.k_stride, h);
+                    if (off >= 0) row = (is_v ? vp : kp) + off;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            at[lane] = row;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        f32x4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int bl = 0; bl < 2; bl++) {
+            const T *row = at[8 * (jl >> 2) + 4 * bl + (jl & 3)];
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                H8 k{};
+                if (row && 32 * s + 8 * g < d) __builtin_memcpy(&k, row + 32 * s + 8 * g, 16);
+                sc[bl] = mma16(k, q[s], sc[bl]);
+            }
+        }
+        unsigned vv[NS][8][ND / 2];
+        float s8[8], top = m;
+#pragma unroll
+        for (int j8 = 0; j8 < 8; j8++) {
+            const T *row = at[32 + 8 * g + j8];
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+#pragma unroll
+                for (int i = 0; i < ND / 2; i++) vv[n][j8][i] = 0;
+                if (row && 128 * n + ND * jl < d) __builtin_memcpy(vv[n][j8], row + 128 * n + ND * jl, 2 * ND);
+            }
+            const int v = st * 32 + 8 * g + j8, j = keys.at(v);
+            const bool seen = v < nv && win_sees(p, my_pos, j);
+            float s = sc[j8 >> 2][j8 & 3] * a.scale_log2;
+            if (!row) s = __builtin_nanf("");
+            s8[j8] = seen ? s : -__builtin_inff();
+            top = __builtin_fmaxf(top, s8[j8]);
+        }
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float fade = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= fade;
+        f32x8 w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            w[i] = __builtin_amdgcn_exp2f(s8[i] - base);
+            l += w[i];
+        }
+        const H8 pw = __builtin_convertvector(w, H8);
+#pragma unroll
+        for (int n = 0; n < NS; n++)
+#pragma unroll
+            for (int i = 0; i < ND; i++) {
+                unsigned vt[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    vt[e] = __builtin_amdgcn_perm(vv[n][2 * e + 1][i / 2], vv[n][2 * e][i / 2],
+                                                  i & 1 ? 0x07060302u : 0x05040100u);
+                H8 vh;
+                __builtin_memcpy(&vh, vt, 16);
+                acc[n][i] *= fade;
+                acc[n][i] = mma16(vh, pw, acc[n][i]);
+            }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // join the waves: [WAVES][16] pairs (m, l), then [WAVES][16][DP] sums
+    __syncthreads();
+    float *ml = reinterpret_cast<float *>(lds), *os = ml + WAVES * 32;
+    if (g == 0) {
+        ml[(wave * 16 + jl) * 2] = m;
+        ml[(wave * 16 + jl) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < NS; n++)
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                os[(wave * 16 + jl) * DP + 128 * n + ND * (4 * g + r) + i] = acc[n][i][r];
+    __syncthreads();
+    for (int e = tid; e < 16 * DP; e += 64 * WAVES) {
+        const int r = e / DP, c = e % DP, row = r0 + r;
+        if (row >= rows || c >= d) continue;
+        float mm = ml[r * 2];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) mm = __builtin_fmaxf(mm, ml[(w * 16 + r) * 2]);
+        const float base = mm == -__builtin_inff() ? 0.0f : mm;
+        float sum = 0.0f, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + r) * 2] - base);
+            ll += f * ml[(w * 16 + r) * 2 + 1];
+            sum += f * os[(w * 16 + r) * DP + c];
+        }
+        if (a.splits == 1) {
+            o[(long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1] + c] = (T)(sum / ll);
+        } else {
+            const long long u = (long long)unit * a.splits + split;
+            a.part_o[(u * 16 + r) * d + c] = sum;
+            if (c == 0) {
+                a.part_ml[(u * 16 + r) * 2] = mm;
+                a.part_ml[(u * 16 + r) * 2 + 1] = ll;
+            }
+        }
+    }
+}
+
+// Joins the splits of a row block: a workgroup a unit, a thread an output value.
+template <typename T>
+__global__ __launch_bounds__(256) void window_attn_join_kernel(WinArgs a) {
+    const osh_window_attn &p = a.p;
+    const int unit = blockIdx.x, d = p.head_dim, G = a.group;
+    int id = unit;
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int h = id % p.kv_heads, b = id / p.kv_heads;
+    const WinSeq sq = win_seq(p, b);
+    if (!sq.ok) return;
+    const int rows = sq.ql * G, r0 = tile * 16;
+    for (int e = threadIdx.x; e < 16 * d; e += 256) {
+        const int r = e / d, c = e % d, row = r0 + r;
+        if (row >= rows) break;
+        const float *ml = a.part_ml + (long long)unit * a.splits * 32 + r * 2;
+        const float *os = a.part_o + (long long)unit * a.splits * 16 * d + e;
+        float mm = -__builtin_inff();
+        for (int s = 0; s < a.splits; s++) mm = __builtin_fmaxf(mm, ml[s * 32]);
+        const float base = mm == -__builtin_inff() ? 0.0f : mm;
+        float sum = 0.0f, ll = 0.0f;
+        for (int s = 0; s < a.splits; s++) {
+            const float f = __builtin_amdgcn_exp2f(ml[s * 32] - base);
+            ll += f * ml[s * 32 + 1];
+            sum += f * os[(long long)s * 16 * d];
+        }
+        static_cast<T *>(p.d_o)[(long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1] +
+                                c] = (T)(sum / ll);
+    }
+}
+
+// Row blocks, splits and scratch of a call.
+static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch) {
+    if (!p) return fail(OSH_E_INVALID, "WindowAttention: NULL parameters");
+    if (p->dtype != OSH_T_F16 && p->dtype != OSH_T_BF16)
+        return fail(OSH_E_INVALID, "WindowAttention: queries, keys and values are f16 or bf16");
+    if (p->batch < 0 || p->q_heads <= 0 || p->kv_heads <= 0 || p->head_dim <= 0 || p->max_q < 0 || p->max_kv < 0 ||
+        p->pages < 0 || p->page <= 0 || p->table_width < 0 || p->tokens < 0)
+        return fail(OSH_E_INVALID, "WindowAttention: bad sizes");
+    if (p->q_heads % p->kv_heads) return fail(OSH_E_INVALID, "WindowAttention: %d query heads over %d key heads",
+                                              p->q_heads, p->kv_heads);
+    if (p->window < 1 || p->sinks < 0) return fail(OSH_E_INVALID, "WindowAttention: window %d, sinks %d", p->window,
+                                                   p->sinks);
+    if (!(p->scale >= 0.0f) || p->scale > 3e38f) return fail(OSH_E_INVALID, "WindowAttention: bad scale");
+    if (p->head_dim % 8 || p->head_dim > 256)
+        return fail(OSH_E_UNSUPPORTED, "WindowAttention: heads of %d values (multiples of 8 up to 256)", p->head_dim);
+    if (p->max_kv > (1 << 30) || p->tokens > (1 << 30) || p->max_q > p->max_kv)
+        return fail(p->max_q > p->max_kv ? OSH_E_INVALID : OSH_E_UNSUPPORTED,
+                    "WindowAttention: lengths up to %d new, %d in all", p->max_q, p->max_kv);
+    a.p = *p;
+    a.group = p->q_heads / p->kv_heads;
+    if ((long long)p->max_q * a.group > (1 << 30))
+        return fail(OSH_E_UNSUPPORTED, "WindowAttention: %d new tokens of %d heads", p->max_q, p->q_heads);
+    a.tiles = cdiv(p->max_q * a.group, 16);
+    a.scale_log2 = (p->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)p->head_dim) : p->scale) * 1.4426950408889634f;
+    const long long units = (long long)p->batch * p->kv_heads * a.tiles;
+    if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "WindowAttention: too many row blocks (%lld)", units);
+    const long long span = std::min<long long>(p->max_kv, (long long)p->window + p->sinks + 15);
+    const long long want = units ? (2LL * device_cus() + units - 1) / units : 1;
+    a.splits = (int)std::max(1LL, std::min(want, span / 256));
+    const long long parts = a.splits > 1 ? units * a.splits : 0;
+    scratch = (size_t)parts * 16 * (p->head_dim + 2) * 4;
+    return OSH_OK;
+}
+
+template <typename T, int DP, int WAVES>
+static osh_status win_launch(const WinArgs &a, unsigned units, hipStream_t st) {
+    constexpr size_t lds = std::max<size_t>(WAVES * 64 * sizeof(void *), WAVES * 16 * (DP + 2) * sizeof(float));
+    OSH_LAUNCH((window_attn_rows_kernel<T, DP, WAVES>), dim3(units * a.splits), dim3(64 * WAVES), lds, st, a);
+    OSH_LAUNCH_CHECK("window_attn_rows_kernel");
+    if (a.splits > 1) {
+        OSH_LAUNCH(window_attn_join_kernel<T>, dim3(units), dim3(256), 0, st, a);
+        OSH_LAUNCH_CHECK("window_attn_join_kernel");
+    }
+    return OSH_OK;
+}
+
+template <typename T>
+static osh_status win_launch_t(const WinArgs &a, unsigned units, hipStream_t st) {
+    if (a.p.head_dim <= 64) return win_launch<T, 64, 4>(a, units, st);
+    if (a.p.head_dim <= 128) return win_launch<T, 128, 4>(a, units, st);
+    return win_launch<T, 256, 4>(a, units, st);
+}
+
+}  // namespace osh
+
+extern "C" {
+
+OSH_API osh_status osh_window_attention_scratch_bytes(const osh_window_attn *p, size_t *bytes) {
+    if (!bytes) return fail(OSH_E_INVALID, "WindowAttention: NULL bytes");
+    WinArgs a;
+    return win_plan(p, a, *bytes);
+}
+
+OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratch, osh_stream s) {
+    WinArgs a;
+    size_t scratch = 0;
+    if (const osh_status st = win_plan(p, a, scratch)) return st;
+    if (p->batch == 0 || p->max_q == 0 || p->tokens == 0) return OSH_OK;
+    if (!p->d_q || !p->d_k_new || !p->d_v_new || !p->d_o || !p->d_k_pages || !p->d_v_pages || !p->d_table ||
+        !p->d_cu || !p->d_kl || (scratch && !d_scratch))
+        return fail(OSH_E_INVALID, "WindowAttention: NULL pointer");
+    const long long d = p->head_dim, n = p->tokens - 1;
+    const int64_t *two[4] = {p->q_stride, p->o_stride, p->k_new_stride, p->v_new_stride};
+    for (int i = 0; i < 4; i++)
+        if (two[i][0] < 0 || two[i][1] < 0) return fail(OSH_E_INVALID, "WindowAttention: negative stride");
+    for (int i = 0; i < 3; i++)
+        if (p->k_stride[i] < 0 || p->v_stride[i] < 0) return fail(OSH_E_INVALID, "WindowAttention: negative stride");
+    if (p->table_stride < (p->batch > 1 ? p->table_width : 0))
+        return fail(OSH_E_INVALID, "WindowAttention: table stride below its width");
+    auto bytes2 = [&](const int64_t *st, int heads) { return (n * st[0] + (heads - 1) * st[1] + d) * 2; };
+    const long long bo = bytes2(p->o_stride, p->q_heads);
+    if (ranges_overlap(p->d_o, bo, p->d_q, bytes2(p->q_stride, p->q_heads)) ||
+        ranges_overlap(p->d_o, bo, p->d_k_new, bytes2(p->k_new_stride, p->kv_heads)) ||
+        ranges_overlap(p->d_o, bo, p->d_v_new, bytes2(p->v_new_stride, p->kv_heads)))
+        return fail(OSH_E_INVALID, "WindowAttention: o overlaps an operand");
+    const long long units = (long long)p->batch * p->kv_heads * a.tiles;
+    a.part_ml = static_cast<float *>(d_scratch);
+    a.part_o = a.part_ml + units * a.splits * 32;
+    return p->dtype == OSH_T_F16 ? win_launch_t<_Float16>(a, (unsigned)units, to_stream(s))
+                                 : win_launch_t<__bf16>(a, (unsigned)units, to_stream(s));
+}
+
+}  // extern "C"

@@ -19,6 +19,8 @@ OSH_E_DEVICE = -3
 OSH_E_NOMEM = -4
 
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3
+ACT_GELU = 4
+T_F32, T_F16, T_BF16, T_I8, T_E4M3 = 0, 1, 2, 3, 4
 PAD_NOTSET, PAD_SAME_UPPER, PAD_SAME_LOWER, PAD_VALID = 0, 1, 2, 3
 AUTO_PAD = {"NOTSET": PAD_NOTSET, "SAME_UPPER": PAD_SAME_UPPER, "SAME_LOWER": PAD_SAME_LOWER, "VALID": PAD_VALID}
 ACTIVATIONS = {None: ACT_NONE, "Relu": ACT_RELU, "Silu": ACT_SILU}
@@ -73,6 +75,17 @@ class PwChain(C.Structure):
 
 class PoolParams(C.Structure):
     _fields_ = [(f, C.c_int) for f in ("n", "c", "h", "w", "kh", "kw", "sh", "sw", "pt", "pl", "oh", "ow")]
+
+
+class WindowAttn(C.Structure):
+    """osh_window_attn: sizes, pointers and strides of one attention call."""
+    _fields_ = ([(f, C.c_int) for f in ("dtype", "batch", "q_heads", "kv_heads", "head_dim", "window", "sinks",
+                                        "max_q", "max_kv", "pages", "page", "table_width")]
+                + [("scale", C.c_float), ("reserved", C.c_int), ("tokens", C.c_int64)]
+                + [(f, C.c_void_p) for f in ("d_q", "d_k_new", "d_v_new", "d_o", "d_k_pages", "d_v_pages", "d_table",
+                                             "d_cu", "d_kl")]
+                + [(f, C.c_int64 * 2) for f in ("q_stride", "k_new_stride", "v_new_stride", "o_stride")]
+                + [(f, C.c_int64 * 3) for f in ("k_stride", "v_stride")] + [("table_stride", C.c_int64)])
 
 
 _vp, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
@@ -135,6 +148,10 @@ _SIGS = {
     "osh_transpose_f32": ([_i, _i, _i, _vp, _i64, _vp, _i64, _vp], _i),
     "osh_softmax_f32": ([_i64, _i, C.c_float, _vp, _vp, _vp], _i),
     "osh_attention_f32": ([_i, _i, _i, _i, C.c_float, _vp, _i64, _vp, _vp], _i),
+    "osh_rms_norm_quant": ([_i64, _i, _i, _vp, _i64, _vp, _i64, _vp, C.c_float, _vp, _i64, _i, _vp, _i64, _vp, _vp], _i),
+    "osh_quant_matmul": ([_i, _i, _i, _i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp], _i),
+    "osh_window_attention_scratch_bytes": ([C.POINTER(WindowAttn), C.POINTER(_sz)], _i),
+    "osh_window_attention": ([C.POINTER(WindowAttn), _vp, _vp], _i),
     "osh_graph_begin": ([_vp], _i),
     "osh_graph_end": ([_vp, C.POINTER(_vp)], _i),
     "osh_graph_launch": ([_vp, _vp], _i),
