@@ -49,6 +49,21 @@ __device__ __forceinline__ typename QAcc<Q>::type mma(const Frag &w, const Frag 
     }
 }
 
+// acc[i][j] += w a[i] over FM row fragments; int8 takes the low halves of all rows
+// first, so that no MFMA waits for the one before.
+template <int Q, int FM, int FN>
+__device__ __forceinline__ void mma_rows(const Frag &w, const Frag (&a)[FM], typename QAcc<Q>::type (&acc)[FM][FN], int j) {
+    if constexpr (Q == OSH_T_I8) {
+#pragma unroll
+        for (int i = 0; i < FM; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.lo, a[i].lo, acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < FM; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.hi, a[i].hi, acc[i][j], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < FM; i++) acc[i][j] = mma<Q>(w, a[i], acc[i][j]);
+    }
+}
+
 // 16 bytes of a row from byte k0, zero from byte k on.
 __device__ __forceinline__ i32x4 load_chunk(const unsigned char *row, int k0, int k) {
     i32x4 v = {0, 0, 0, 0};
@@ -80,6 +95,95 @@ __device__ __forceinline__ T finish(const QmmArgs &p, float sum, int row, int co
     v = apply_act(p.act, v);
     if (p.res) v += (float)static_cast<const T *>(p.res)[row * p.ldr + col];
     return (T)v;
+}
+
+// The epilogue of a wave's FM x FN fragments, rows from row0 and outputs from col0:
+// up to four fragments' rows at a time go to the wave's own LDS, 16 * 4 rows of
+// 16 FN sums, and come back eight neighbouring outputs a lane, so that residual and
+// output move in 16-byte pieces and a lane's eight scales and biases are read once.
+// `lds` holds EpiRows * EpiPitch<FN> floats.
+constexpr int EpiRows = 64;
+template <int FN> constexpr int EpiPitch = 16 * FN + 4;
+
+template <int Q, typename T, int FM, int FN>
+__device__ __forceinline__ void qmm_epilogue(const QmmArgs &p, const typename QAcc<Q>::type (&acc)[FM][FN], float *lds,
+                                             int row0, int col0) {
+    constexpr int LPR = 2 * FN, RPP = 64 / LPR;  // lanes of a row, rows of a pass
+    constexpr int GROUP = FM < EpiRows / 16 ? FM : EpiRows / 16;
+    const int lane = threadIdx.x & 63, jl = lane & 15, g = lane >> 4;
+    const int c = lane % LPR * 8, col = col0 + c, cols = p.n - col;
+    float sw[8], bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        sw[i] = i < cols ? p.sw[col + i] : 0.0f;
+        bias[i] = i < cols && p.bias ? p.bias[col + i] : 0.0f;
+    }
+#pragma unroll
+    for (int i0 = 0; i0 < FM; i0 += GROUP) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < GROUP; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                const auto &v = acc[i0 + i][j];
+                *reinterpret_cast<f32x4 *>(lds + (16 * i + jl) * EpiPitch<FN> + 16 * j + 4 * g) =
+                    f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (int r = lane / LPR; r < 16 * GROUP; r += RPP) {
+            const int row = row0 + 16 * i0 + r;
+            if (row >= p.m || cols <= 0) continue;
+            const float sa = p.sa[row];
+            const T *res = static_cast<const T *>(p.res) + row * p.ldr + col;
+            T *y = static_cast<T *>(p.y) + row * p.ldy + col;
+            f32x8 v, add = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (p.res) {
+                if (cols >= 8) {
+                    add = load8(res);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 7; i++)
+                        if (i < cols) add[i] = (float)res[i];
+                }
+            }
+            const f32x4 *from = reinterpret_cast<const f32x4 *>(lds + r * EpiPitch<FN> + c);
+            const f32x4 v0 = from[0], v1 = from[1];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = (i < 4 ? v0[i & 3] : v1[i & 3]) * sa * sw[i] + bias[i];
+            if (p.act == OSH_ACT_GELU) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = apply_act(OSH_ACT_GELU, v[i]);
+            } else if (p.act == OSH_ACT_SILU) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = apply_act(OSH_ACT_SILU, v[i]);
+            } else if (p.act == OSH_ACT_RELU) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = apply_act(OSH_ACT_RELU, v[i]);
+            }
+            v += add;
+            if (cols >= 8) {
+                store8(y, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 7; i++)
+                    if (i < cols) y[i] = (T)v[i];
+            }
+        }
+    }
+}
+
+// Tile (row, column) number id: columns of 8 row tiles one after another, so that
+// the 32 tiles an XCD holds at a time share few rows and few weights.
+__device__ __forceinline__ int2 qmm_tile_of(int id, int tm, int tn) {
+    const int per = 8 * tn, band = id / per, first = band * 8;
+    const int rows = min(8, tm - first), in = id - band * per;
+    return int2{first + in % rows, in / rows};
+}
+
+// 16 bytes a lane from r at byte off + soff to LDS: lane i's to dst + 16 i.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned char *dst, int off, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, off, soff, 0, 0);
 }
 
 // Tile of BM rows by BN outputs, WM x WN waves; k-blocks pass through two LDS
@@ -151,20 +255,132 @@ __global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
         __syncthreads();
     }
 
+    qmm_epilogue<Q, T, FM, FN>(p, acc, reinterpret_cast<float *>(lds) + wave * EpiRows * EpiPitch<FN>,
+                               m0 + wm * (BM / WM), n0 + wn * (BN / WN));
+}
+
+// Large products: BM x BN tiles of four waves, each (BM / 2) x (BN / 2), fed by
+// direct loads from global memory to LDS, 16 bytes a lane, two k-blocks deep.
+// (Rows at any 16-byte alignment; a k-block that k cuts short goes through
+// registers, zeros from byte k on.)
+//
+// A wave keeps the k-block's FM fragments of its rows in registers and takes the
+// FN fragments of the weights one after another, the next read a step ahead.
+// Before the last step every wave has read the whole block: there the one barrier
+// of a k-block stands, behind it the loads of the block after the next start into
+// the buffer just freed, and the row fragments of the next block replace the
+// present ones as the last MFMAs use them.
+template <int Q, typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void qmm_dma_kernel(QmmArgs p) {
+    constexpr int FM = BM / 32, FN = BN / 32, CH = (BM + BN) / 32, BUF = (BM + BN) * KB;
+    using Acc = typename QAcc<Q>::type;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jl = lane & 15, g = lane >> 4;
+    const int2 tile = qmm_tile_of(xcd_band(blockIdx.x, gridDim.x), cdiv(p.m, BM), cdiv(p.n, BN));
+    const int m0 = tile.x * BM, n0 = tile.y * BN;
+    const int wm = wave & 1, wn = wave >> 1;
+
+    // chunk (tid & 7) of LDS row tid / 8 + 32 i, which holds chunk `c` of the row
+    const int c = ((tid & 7) ^ (tid >> 4 & 7)) * 16;
+    int src[CH];
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-        const int row = m0 + wm * (BM / WM) + 16 * i + jl;
-        if (row >= p.m) continue;
-        const float sa = p.sa[row];
-        T *y = static_cast<T *>(p.y) + row * p.ldy;
+    for (int i = 0; i < CH; i++) {
+        const int r = (tid >> 3) + 32 * i;
+        src[i] = r < BM ? (min(m0 + r, p.m - 1) - m0) * (int)p.lda + c : (min(n0 + r - BM, p.n - 1) - n0) * (int)p.ldw + c;
+    }
+    const unsigned char *a0 = p.a + (long long)m0 * p.lda, *w0 = p.w + (long long)n0 * p.ldw;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)a0, (short)0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void *)w0, (short)0, 0x7fffffff, 0x00020000);
+    const int nkb = cdiv(p.k, KB);
+    auto stage1 = [&](int kb, int i) {  // rows 32 i .. 32 i + 31 of a whole k-block
+        load_to_lds(i < BM / 32 ? ra : rw, lds + (kb & 1) * BUF + (32 * i + wave * 8) * KB, src[i], kb * KB);
+    };
+    auto stage = [&](int kb) {
+        if ((kb + 1) * KB <= p.k) {
 #pragma unroll
-        for (int j = 0; j < FN; j++) {
-            const int col = n0 + wn * (BN / WN) + 16 * j + 4 * g;
+            for (int i = 0; i < CH; i++) stage1(kb, i);
+        } else {
+#pragma unroll 1
+            for (int r = tid >> 3; r < BM + BN; r += 32) {
+                const unsigned char *row = r < BM ? a0 + (long long)(min(m0 + r, p.m - 1) - m0) * p.lda
+                                                  : w0 + (long long)(min(n0 + r - BM, p.n - 1) - n0) * p.ldw;
+                *reinterpret_cast<i32x4 *>(lds + (kb & 1) * BUF + r * KB + (tid & 7) * 16) =
+                    load_chunk(row, kb * KB + c, p.k);
+            }
+        }
+    };
+    const int sw = jl >> 1;  // fragment rows are jl plus multiples of 16
+    const int lo = ((g ^ sw) << 4), hi = (((g + 4) ^ sw) << 4);
+    auto frag = [&](int kb, int r) {
+        const unsigned char *row = lds + (kb & 1) * BUF + (r + jl) * KB;
+        Frag f;
+        f.lo = *reinterpret_cast<const i32x4 *>(row + lo);
+        f.hi = *reinterpret_cast<const i32x4 *>(row + hi);
+        return f;
+    };
+
+    Acc acc[FM][FN];
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (col + r < p.n) y[col + r] = finish<T>(p, (float)acc[i][j][r], row, col + r, sa);
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = Acc{0, 0, 0, 0};
+
+    const int rm = wm * (BM / 2), rn = BM + wn * (BN / 2);
+    stage(0);
+    __syncthreads();
+    if (nkb > 1) stage(1);
+    Frag fa[FM], fw[2];
+#pragma unroll
+    for (int i = 0; i < FM; i++) fa[i] = frag(0, rm + 16 * i);
+    fw[0] = frag(0, rn);
+    static_assert(FN % 2 == 0, "the last fragment is in fw[1]");
+    // all steps of k-block kb but the last one
+    auto front = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < FN - 1; j++) {
+            fw[(j + 1) & 1] = frag(kb, rn + 16 * (j + 1));
+            mma_rows<Q, FM>(fw[j & 1], fa, acc, j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+    };
+    int kb = 0;
+    for (const int end = p.k / KB - 2; kb < end; kb++) {  // blocks kb + 2 that are whole
+        front(kb);
+        fw[0] = frag(kb + 1, rn);
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            acc[i][FN - 1] = mma<Q>(fw[1], fa[i], acc[i][FN - 1]);
+            fa[i] = frag(kb + 1, rm + 16 * i);
+#pragma unroll
+            for (int e = i * CH / FM; e < (i + 1) * CH / FM; e++) stage1(kb + 2, e);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+#pragma unroll 1
+    for (; kb < nkb; kb++) {
+        front(kb);
+        mma_rows<Q, FM>(fw[1], fa, acc, FN - 1);
+        if (kb + 2 < nkb) stage(kb + 2);
+        if (kb + 1 < nkb) {
+            fw[0] = frag(kb + 1, rn);
+#pragma unroll
+            for (int i = 0; i < FM; i++) fa[i] = frag(kb + 1, rm + 16 * i);
+        }
+    }
+
+    __syncthreads();
+    qmm_epilogue<Q, T, FM, FN>(p, acc, reinterpret_cast<float *>(lds) + wave * EpiRows * EpiPitch<FN>, m0 + rm,
+                               n0 + rn - BM);
+}
+
+// LDS of a tile kernel: its two buffers, or the epilogue of its waves.
+template <int BM, int BN, int WM, int WN>
+constexpr int qmm_lds() {
+    constexpr int epi = WM * WN * EpiRows * EpiPitch<BN / WN / 16> * 4;
+    return epi > 2 * (BM + BN) * KB ? epi : 2 * (BM + BN) * KB;
 }
 
 // Few rows: a workgroup takes 16 outputs of all rows (up to 16 MB), its waves
@@ -213,16 +429,26 @@ template <int Q, typename T>
 static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
 #define OSH_QMM_TILE(BM, BN, WM, WN)                                                                  \
     OSH_LAUNCH((qmm_tile_kernel<Q, T, BM, BN, WM, WN>), dim3((unsigned)(cdiv(p.m, BM) * cdiv(p.n, BN))), \
-               dim3(64 * WM * WN), 2 * (BM + BN) * KB, st, p)
+               dim3(64 * WM * WN), (qmm_lds<BM, BN, WM, WN>()), st, p)
+#define OSH_QMM_DMA(BM, BN)                                                                             \
+    OSH_LAUNCH((qmm_dma_kernel<Q, T, BM, BN>), dim3((unsigned)(cdiv(p.m, BM) * cdiv(p.n, BN))), dim3(256), \
+               (qmm_lds<BM, BN, 2, 2>()), st, p)
+    const bool aligned = (((uintptr_t)p.a | (uintptr_t)p.w | p.lda | p.ldw) & 15) == 0 && p.lda < (1 << 22) &&
+                         p.ldw < (1 << 22);
     if (p.m <= 16)
         OSH_LAUNCH((qmm_rows_kernel<Q, T, 1, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
     else if (p.m <= 32)
         OSH_LAUNCH((qmm_rows_kernel<Q, T, 2, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
+    else if (aligned && (long long)cdiv(p.m, 256) * cdiv(p.n, 256) >= device_cus())
+        OSH_QMM_DMA(256, 256);
+    else if (aligned && (long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
+        OSH_QMM_DMA(128, 128);
     else if ((long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
         OSH_QMM_TILE(128, 128, 2, 2);
     else
         OSH_QMM_TILE(64, 64, 2, 2);
 #undef OSH_QMM_TILE
+#undef OSH_QMM_DMA
     OSH_LAUNCH_CHECK("qmm kernel");
     return OSH_OK;
 }
