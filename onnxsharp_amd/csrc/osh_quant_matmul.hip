@@ -11,6 +11,8 @@
 // v_mfma_i32_16x16x64_i8, e4m3 with one v_mfma_f32_16x16x128_f8f6f4.  Which k
 // a byte stands for is the same for both operands, so the sum does not care that
 // the hardware numbers a lane's bytes otherwise.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "osh_lm.h"
@@ -77,11 +79,34 @@ __device__ __forceinline__ i32x4 load_chunk(const unsigned char *row, int k0, in
     return v;
 }
 
+// Activations.  EXACT ones are for FP32 outputs.  For 16-bit outputs SiLU takes the
+// hardware's reciprocal, and GELU, x - x Q(x) for x > 0 and x Q(-x) below with Q(z) =
+// erfc(z / sqrt 2) / 2, a least-maximum fit of erfc(z) e^(z^2) by t P(t), t = 1 / (1 +
+// 0.4 z): within 7e-8 of erfc in exact arithmetic and 4e-7 in FP32, 1 / 600 of the
+// rounding to 16 bits.  erff is 45 instructions a value against 17: 8 us of
+// 1028 x 5120 x 1280.
+template <bool EXACT>
 __device__ __forceinline__ float apply_act(int act, float v) {
     switch (act) {
     case OSH_ACT_RELU: return v > 0.0f || v != v ? v : 0.0f;
-    case OSH_ACT_SILU: return v / (1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
-    case OSH_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    case OSH_ACT_SILU: {
+        const float e = 1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f);
+        return EXACT ? v / e : v * __builtin_amdgcn_rcpf(e);
+    }
+    case OSH_ACT_GELU: {
+        if (EXACT) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+        const float z = __builtin_fabsf(v) * 0.70710678118654752f;
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, z, 1.0f));
+        float q = -0.20526915788650513f;
+        q = __builtin_fmaf(q, t, 0.7297442555427551f);
+        q = __builtin_fmaf(q, t, -0.4045509994029999f);
+        q = __builtin_fmaf(q, t, 0.4955560863018036f);
+        q = __builtin_fmaf(q, t, 0.15084387362003326f);
+        q = __builtin_fmaf(q, t, 0.23367586731910706f);
+        q *= t * __builtin_amdgcn_exp2f(z * z * -1.4426950408889634f);
+        const float h = 0.5f * __builtin_fminf(__builtin_fabsf(v), 64.0f) * q;  // q is 0 from 64 on
+        return v > 0.0f ? v - h : -h;
+    }
     default: return v;
     }
 }
@@ -92,32 +117,64 @@ template <typename T>
 __device__ __forceinline__ T finish(const QmmArgs &p, float sum, int row, int col, float sa) {
     float v = sum * sa * p.sw[col];
     if (p.bias) v += p.bias[col];
-    v = apply_act(p.act, v);
+    v = apply_act<sizeof(T) == 4>(p.act, v);
     if (p.res) v += (float)static_cast<const T *>(p.res)[row * p.ldr + col];
     return (T)v;
 }
 
 // The epilogue of a wave's FM x FN fragments, rows from row0 and outputs from col0:
-// up to four fragments' rows at a time go to the wave's own LDS, 16 * 4 rows of
-// 16 FN sums, and come back eight neighbouring outputs a lane, so that residual and
-// output move in 16-byte pieces and a lane's eight scales and biases are read once.
-// `lds` holds EpiRows * EpiPitch<FN> floats.
+// up to four fragments' rows at a time, scaled by row, go to the wave's own LDS, 16 *
+// 4 rows of 16 FN sums, and come back eight neighbouring outputs a lane, so that
+// residual and output move in 16-byte pieces and a lane's eight scales and biases
+// are read once.  The residuals of four passes are loaded while the four before are
+// computed (one pass at a time waited for memory 32 times a tile: 88 us of 355 for
+// 8192 x 8192 x 4096).  `lds` holds EpiRows * EpiPitch<FN> floats.
 constexpr int EpiRows = 64;
 template <int FN> constexpr int EpiPitch = 16 * FN + 4;
+
+template <int ACT, bool EXACT>
+__device__ __forceinline__ void act8(f32x8 &v) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = apply_act<EXACT>(ACT, v[i]);
+}
 
 template <int Q, typename T, int FM, int FN>
 __device__ __forceinline__ void qmm_epilogue(const QmmArgs &p, const typename QAcc<Q>::type (&acc)[FM][FN], float *lds,
                                              int row0, int col0) {
+    using V = typename Vec8<T>::type;
     constexpr int LPR = 2 * FN, RPP = 64 / LPR;  // lanes of a row, rows of a pass
     constexpr int GROUP = FM < EpiRows / 16 ? FM : EpiRows / 16;
+    constexpr int PASSES = FM * 16 / RPP, GPASS = GROUP * 16 / RPP, BATCH = GPASS < 4 ? GPASS : 4;
+    static_assert(GPASS % BATCH == 0, "a group is whole batches");
     const int lane = threadIdx.x & 63, jl = lane & 15, g = lane >> 4;
     const int c = lane % LPR * 8, col = col0 + c, cols = p.n - col;
-    float sw[8], bias[8];
+    float sa[FM], sw[8], bias[8];
+#pragma unroll
+    for (int i = 0; i < FM; i++) sa[i] = p.sa[min(row0 + 16 * i + jl, p.m - 1)];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         sw[i] = i < cols ? p.sw[col + i] : 0.0f;
         bias[i] = i < cols && p.bias ? p.bias[col + i] : 0.0f;
     }
+    V res[BATCH];
+    auto load_res = [&](int pass) {
+#pragma unroll
+        for (int e = 0; e < BATCH; e++) {
+            const int row = row0 + lane / LPR + (pass + e) * RPP;
+            const T *from = static_cast<const T *>(p.res) + row * p.ldr + col;
+            if (!p.res || row >= p.m) continue;
+            if (cols >= 8) {
+                __builtin_memcpy(&res[e], from, sizeof(V));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 7; i++)
+                    if (i < cols) res[e][i] = from[i];
+            }
+        }
+    };
+#pragma unroll
+    for (int e = 0; e < BATCH; e++) res[e] = V{};
+    load_res(0);
 #pragma unroll
     for (int i0 = 0; i0 < FM; i0 += GROUP) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -127,47 +184,48 @@ __device__ __forceinline__ void qmm_epilogue(const QmmArgs &p, const typename QA
             for (int j = 0; j < FN; j++) {
                 const auto &v = acc[i0 + i][j];
                 *reinterpret_cast<f32x4 *>(lds + (16 * i + jl) * EpiPitch<FN> + 16 * j + 4 * g) =
-                    f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+                    f32x4{(float)v[0] * sa[i0 + i], (float)v[1] * sa[i0 + i], (float)v[2] * sa[i0 + i],
+                          (float)v[3] * sa[i0 + i]};
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
-        for (int r = lane / LPR; r < 16 * GROUP; r += RPP) {
-            const int row = row0 + 16 * i0 + r;
-            if (row >= p.m || cols <= 0) continue;
-            const float sa = p.sa[row];
-            const T *res = static_cast<const T *>(p.res) + row * p.ldr + col;
-            T *y = static_cast<T *>(p.y) + row * p.ldy + col;
-            f32x8 v, add = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (p.res) {
+        for (int q = 0; q < GPASS; q += BATCH) {
+            V add[BATCH];
+            f32x8 v[BATCH];
+#pragma unroll
+            for (int e = 0; e < BATCH; e++) {
+                add[e] = res[e];
+                const f32x4 *from =
+                    reinterpret_cast<const f32x4 *>(lds + (lane / LPR + (q + e) * RPP) * EpiPitch<FN> + c);
+                const f32x4 v0 = from[0], v1 = from[1];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[e][i] = (i < 4 ? v0[i & 3] : v1[i & 3]) * sw[i] + bias[i];
+            }
+            const int pass = i0 * 16 / RPP + q;
+            if (pass + BATCH < PASSES) load_res(pass + BATCH);
+            if (p.act == OSH_ACT_GELU) {
+#pragma unroll
+                for (int e = 0; e < BATCH; e++) act8<OSH_ACT_GELU, sizeof(T) == 4>(v[e]);
+            } else if (p.act == OSH_ACT_SILU) {
+#pragma unroll
+                for (int e = 0; e < BATCH; e++) act8<OSH_ACT_SILU, sizeof(T) == 4>(v[e]);
+            } else if (p.act == OSH_ACT_RELU) {
+#pragma unroll
+                for (int e = 0; e < BATCH; e++) act8<OSH_ACT_RELU, sizeof(T) == 4>(v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < BATCH; e++) {
+                const int row = row0 + lane / LPR + (pass + e) * RPP;
+                if (row >= p.m || cols <= 0) continue;
+                T *y = static_cast<T *>(p.y) + row * p.ldy + col;
+                if (p.res) v[e] += __builtin_convertvector(add[e], f32x8);
                 if (cols >= 8) {
-                    add = load8(res);
+                    store8(y, v[e]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 7; i++)
-                        if (i < cols) add[i] = (float)res[i];
+                        if (i < cols) y[i] = (T)v[e][i];
                 }
-            }
-            const f32x4 *from = reinterpret_cast<const f32x4 *>(lds + r * EpiPitch<FN> + c);
-            const f32x4 v0 = from[0], v1 = from[1];
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = (i < 4 ? v0[i & 3] : v1[i & 3]) * sa * sw[i] + bias[i];
-            if (p.act == OSH_ACT_GELU) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = apply_act(OSH_ACT_GELU, v[i]);
-            } else if (p.act == OSH_ACT_SILU) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = apply_act(OSH_ACT_SILU, v[i]);
-            } else if (p.act == OSH_ACT_RELU) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = apply_act(OSH_ACT_RELU, v[i]);
-            }
-            v += add;
-            if (cols >= 8) {
-                store8(y, v);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 7; i++)
-                    if (i < cols) y[i] = (T)v[i];
             }
         }
     }
@@ -259,7 +317,42 @@ __global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
                                m0 + wm * (BM / WM), n0 + wn * (BN / WN));
 }
 
-// Large products: BM x BN tiles of four waves, each (BM / 2) x (BN / 2), fed by
+// Waits written by hand: the compiler does not tie LDS reads to the direct loads that
+// fill it.  wait_lds_and_barrier leaves loads and stores of memory in flight.
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void wait_all_and_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds_and_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Outputs (or residuals) from element `first` on, and 8 of them at a byte offset.
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t out_rsrc(const void *base, long long first) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(static_cast<const T *>(base) + first), (short)0, 0x7fffffff,
+                                             0x00020000);
+}
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type buffer_load8(__amdgpu_buffer_rsrc_t r, int off, int soff) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 w[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, soff, 0);
+    typename Vec8<T>::type v;
+    __builtin_memcpy(&v, w, sizeof(v));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void buffer_store8(typename Vec8<T>::type v, __amdgpu_buffer_rsrc_t r, int off, int soff) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 w[sizeof(T) / 2];
+    __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_amdgcn_raw_buffer_store_b128(w[i], r, off + 16 * i, soff, 0);
+}
+
+// Large products: BM x BN tiles of 2 x WN waves, each (BM / 2) x (BN / WN), fed by
 // direct loads from global memory to LDS, 16 bytes a lane, two k-blocks deep.
 // (Rows at any 16-byte alignment; a k-block that k cuts short goes through
 // registers, zeros from byte k on.)
@@ -270,110 +363,219 @@ __global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
 // of a k-block stands, behind it the loads of the block after the next start into
 // the buffer just freed, and the row fragments of the next block replace the
 // present ones as the last MFMAs use them.
-template <int Q, typename T, int BM, int BN>
-__global__ __launch_bounds__(256) void qmm_dma_kernel(QmmArgs p) {
-    constexpr int FM = BM / 32, FN = BN / 32, CH = (BM + BN) / 32, BUF = (BM + BN) * KB;
+//
+// A workgroup takes every gridDim-th tile.  The loads of a tile's first two blocks
+// start in the last two steps of the tile before, and the epilogue, from registers
+// to memory, needs no LDS, so it runs over them; its stores drain under the next
+// tile's first block, whose barrier does not wait for them.
+//
+// 256 x 256 of eight waves: 8192 x 8192 x 4096 e4m3 218 us (2.5 PFLOP/s; a large
+// library product reaches 2.65 here), 260 with a residual, whose 134 MB the CUs all
+// want at their tiles' ends.  Bringing it to L2 ahead of the end cost 6 us instead.
+// Four waves of 128 x 128 read a quarter less LDS, but their 256 accumulators left
+// no register free and the spills cost more (275 us).
+template <int Q, typename T, int ACT, int BM, int BN, int WN, bool FAST>
+__global__ __launch_bounds__(128 * WN, 2) void qmm_dma_kernel(QmmArgs p) {
+    constexpr int THREADS = 128 * WN, RPC = THREADS / 8;  // LDS rows of a staging pass
+    constexpr int FM = BM / 32, FN = BN / WN / 16, CH = (BM + BN) / RPC, BUF = (BM + BN) * KB;
     using Acc = typename QAcc<Q>::type;
+    using V = typename Vec8<T>::type;
     extern __shared__ __align__(16) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int jl = lane & 15, g = lane >> 4;
-    const int2 tile = qmm_tile_of(xcd_band(blockIdx.x, gridDim.x), cdiv(p.m, BM), cdiv(p.n, BN));
-    const int m0 = tile.x * BM, n0 = tile.y * BN;
+    const int tm = cdiv(p.m, BM), tn = cdiv(p.n, BN), tiles = tm * tn;
     const int wm = wave & 1, wn = wave >> 1;
-
-    // chunk (tid & 7) of LDS row tid / 8 + 32 i, which holds chunk `c` of the row
-    const int c = ((tid & 7) ^ (tid >> 4 & 7)) * 16;
-    int src[CH];
-#pragma unroll
-    for (int i = 0; i < CH; i++) {
-        const int r = (tid >> 3) + 32 * i;
-        src[i] = r < BM ? (min(m0 + r, p.m - 1) - m0) * (int)p.lda + c : (min(n0 + r - BM, p.n - 1) - n0) * (int)p.ldw + c;
-    }
-    const unsigned char *a0 = p.a + (long long)m0 * p.lda, *w0 = p.w + (long long)n0 * p.ldw;
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)a0, (short)0, 0x7fffffff, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void *)w0, (short)0, 0x7fffffff, 0x00020000);
+    const int rm = wm * (BM / 2), rn = BM + wn * (BN / WN);
     const int nkb = cdiv(p.k, KB);
-    auto stage1 = [&](int kb, int i) {  // rows 32 i .. 32 i + 31 of a whole k-block
-        load_to_lds(i < BM / 32 ? ra : rw, lds + (kb & 1) * BUF + (32 * i + wave * 8) * KB, src[i], kb * KB);
+
+    // Opening a tile, its cut k-block and its epilogue start from a thread
+    // number that the compiler cannot see through: kept across the k loop, what they
+    // compute of it would be spilled, and each reload waits for all loads in flight.
+    auto thread = [&] {
+        int t = tid;
+        asm volatile("" : "+v"(t));
+        return t;
     };
-    auto stage = [&](int kb) {
+    // The tile whose blocks are being loaded.  Chunk (tid & 7) of LDS row tid / 8 + RPC i
+    // holds chunk (tid & 7) ^ (tid / 16 & 7) of its row.  A row past the end lies past
+    // its buffer, whose loads are then not made; only the vector offset decides it.
+    auto chunk = [](int t) { return ((t & 7) ^ (t >> 4 & 7)) * 16; };
+    const int src_a = (tid >> 3) * (int)p.lda + chunk(tid), src_w = (tid >> 3) * (int)p.ldw + chunk(tid);
+    int lm0, ln0;
+    const unsigned char *a0, *w0;
+    __amdgpu_buffer_rsrc_t ra, rw;
+    auto open_tile = [&](int number) {
+        const int2 t = qmm_tile_of(xcd_band(number, tiles), tm, tn);
+        lm0 = t.x * BM, ln0 = t.y * BN;
+        a0 = p.a + (long long)lm0 * p.lda, w0 = p.w + (long long)ln0 * p.ldw;
+        ra = __builtin_amdgcn_make_buffer_rsrc((void *)a0, (short)0, min(p.m - 1 - lm0, BM) * (int)p.lda + p.k, 0x00020000);
+        rw = __builtin_amdgcn_make_buffer_rsrc((void *)w0, (short)0, min(p.n - 1 - ln0, BN) * (int)p.ldw + p.k, 0x00020000);
+    };
+    auto stage1 = [&](int buf, int kb, int i) {  // RPC rows of a whole k-block
+        unsigned char *dst = lds + buf * BUF + (RPC * i + wave * 8) * KB;
+        if (i < BM / RPC) load_to_lds(ra, dst, src_a + RPC * i * (int)p.lda, kb * KB);
+        else load_to_lds(rw, dst, src_w + (RPC * i - BM) * (int)p.ldw, kb * KB);
+    };
+    auto stage = [&](int buf, int kb) {
         if ((kb + 1) * KB <= p.k) {
 #pragma unroll
-            for (int i = 0; i < CH; i++) stage1(kb, i);
+            for (int i = 0; i < CH; i++) stage1(buf, kb, i);
         } else {
+            const int t0 = thread();
 #pragma unroll 1
-            for (int r = tid >> 3; r < BM + BN; r += 32) {
-                const unsigned char *row = r < BM ? a0 + (long long)(min(m0 + r, p.m - 1) - m0) * p.lda
-                                                  : w0 + (long long)(min(n0 + r - BM, p.n - 1) - n0) * p.ldw;
-                *reinterpret_cast<i32x4 *>(lds + (kb & 1) * BUF + r * KB + (tid & 7) * 16) =
-                    load_chunk(row, kb * KB + c, p.k);
+            for (int r = t0 >> 3; r < BM + BN; r += RPC) {
+                const unsigned char *row =
+                    r < BM ? a0 + min(r, p.m - 1 - lm0) * p.lda : w0 + min(r - BM, p.n - 1 - ln0) * p.ldw;
+                *reinterpret_cast<i32x4 *>(lds + buf * BUF + r * KB + (t0 & 7) * 16) =
+                    load_chunk(row, kb * KB + chunk(t0), p.k);
             }
         }
     };
     const int sw = jl >> 1;  // fragment rows are jl plus multiples of 16
     const int lo = ((g ^ sw) << 4), hi = (((g + 4) ^ sw) << 4);
-    auto frag = [&](int kb, int r) {
-        const unsigned char *row = lds + (kb & 1) * BUF + (r + jl) * KB;
+    auto frag = [&](int buf, int r) {
+        const unsigned char *row = lds + buf * BUF + (r + jl) * KB;
         Frag f;
         f.lo = *reinterpret_cast<const i32x4 *>(row + lo);
         f.hi = *reinterpret_cast<const i32x4 *>(row + hi);
         return f;
     };
-
-    Acc acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = Acc{0, 0, 0, 0};
-
-    const int rm = wm * (BM / 2), rn = BM + wn * (BN / 2);
-    stage(0);
-    __syncthreads();
-    if (nkb > 1) stage(1);
-    Frag fa[FM], fw[2];
-#pragma unroll
-    for (int i = 0; i < FM; i++) fa[i] = frag(0, rm + 16 * i);
-    fw[0] = frag(0, rn);
     static_assert(FN % 2 == 0, "the last fragment is in fw[1]");
-    // all steps of k-block kb but the last one
-    auto front = [&](int kb) {
-#pragma unroll
-        for (int j = 0; j < FN - 1; j++) {
-            fw[(j + 1) & 1] = frag(kb, rn + 16 * (j + 1));
-            mma_rows<Q, FM>(fw[j & 1], fa, acc, j);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        __syncthreads();
-    };
-    int kb = 0;
-    for (const int end = p.k / KB - 2; kb < end; kb++) {  // blocks kb + 2 that are whole
-        front(kb);
-        fw[0] = frag(kb + 1, rn);
-#pragma unroll
-        for (int i = 0; i < FM; i++) {
-            acc[i][FN - 1] = mma<Q>(fw[1], fa[i], acc[i][FN - 1]);
-            fa[i] = frag(kb + 1, rm + 16 * i);
-#pragma unroll
-            for (int e = i * CH / FM; e < (i + 1) * CH / FM; e++) stage1(kb + 2, e);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-#pragma unroll 1
-    for (; kb < nkb; kb++) {
-        front(kb);
-        mma_rows<Q, FM>(fw[1], fa, acc, FN - 1);
-        if (kb + 2 < nkb) stage(kb + 2);
-        if (kb + 1 < nkb) {
-            fw[0] = frag(kb + 1, rn);
-#pragma unroll
-            for (int i = 0; i < FM; i++) fa[i] = frag(kb + 1, rm + 16 * i);
-        }
-    }
 
-    __syncthreads();
-    qmm_epilogue<Q, T, FM, FN>(p, acc, reinterpret_cast<float *>(lds) + wave * EpiRows * EpiPitch<FN>, m0 + rm,
-                               n0 + rn - BM);
+    int number = blockIdx.x, buf = 0;  // buf holds the present k-block
+    open_tile(number);
+    stage(0, 0);
+    if (nkb > 1) stage(1, 1);
+    wait_all_and_barrier();
+#pragma unroll 1
+    for (bool first = true;; first = false) {
+        const int m0 = lm0, n0 = ln0, following = number + gridDim.x;
+        const bool more = FAST && following < tiles;
+        Acc acc[FM][FN];
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = Acc{0, 0, 0, 0};
+        Frag fa[FM], fw[2];
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[i] = frag(buf, rm + 16 * i);
+        fw[0] = frag(buf, rn);
+        // all steps of a k-block but the last one, and its barrier
+        auto front = [&](bool wait) {
+#pragma unroll
+            for (int j = 0; j < FN - 1; j++) {
+                fw[(j + 1) & 1] = frag(buf, rn + 16 * (j + 1));
+                mma_rows<Q, FM>(fw[j & 1], fa, acc, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (wait) wait_all_and_barrier();
+            else wait_lds_and_barrier();
+        };
+        int kb = 0;
+        for (const int end = p.k / KB - 2; kb < end; kb++) {  // blocks kb + 2 that are whole
+            front(kb > 0 || first);
+            fw[0] = frag(buf ^ 1, rn);
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                acc[i][FN - 1] = mma<Q>(fw[1], fa[i], acc[i][FN - 1]);
+                fa[i] = frag(buf ^ 1, rm + 16 * i);
+#pragma unroll
+                for (int e = i * CH / FM; e < (i + 1) * CH / FM; e++) stage1(buf, kb + 2, e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            buf ^= 1;
+        }
+#pragma unroll 1
+        for (; kb < nkb; kb++) {
+            front(true);
+            mma_rows<Q, FM>(fw[1], fa, acc, FN - 1);
+            int load = kb + 2;
+            if (load >= nkb && more) {  // the following tile's first blocks
+                if (load == nkb) open_tile(following);
+                load -= nkb;
+            }
+            if (load < nkb) stage(buf, load);
+            buf ^= 1;
+            if (kb + 1 < nkb) {
+                fw[0] = frag(buf, rn);
+#pragma unroll
+                for (int i = 0; i < FM; i++) fa[i] = frag(buf, rm + 16 * i);
+            }
+        }
+        if constexpr (FAST) {
+            // Fragments j and j + 1 at a time: exchanging the odd rows of 16 lanes of one
+            // with the even rows of the other leaves a lane eight neighbouring outputs of
+            // fragment j + (g & 1).  Rows and outputs past the end get an offset past the
+            // buffer: loads return 0, stores are dropped, and with no branch around them
+            // waits can count them.
+            __builtin_amdgcn_sched_barrier(0);
+            const int t0 = thread(), jl = t0 & 15, g = t0 >> 4 & 3;
+            const int ec = n0 + rn - BM + 16 * (g & 1) + 8 * (g >> 1);  // of pair 0
+            const __amdgpu_buffer_rsrc_t ry = out_rsrc<T>(p.y, m0 * p.ldy), rr = out_rsrc<T>(p.res, m0 * p.ldr);
+            auto at = [&](int i, int jp, long long ld) {
+                const int r = rm + jl;
+                return m0 + r + 16 * i < p.m && ec + 32 * jp < p.n ? (r * (int)ld + ec) * (int)sizeof(T) : INT_MIN;
+            };
+            float sa[FM];
+#pragma unroll
+            for (int i = 0; i < FM; i++) sa[i] = p.sa[min(m0 + rm + 16 * i + jl, p.m - 1)];
+            f32x8 esw, ebias = {0, 0, 0, 0, 0, 0, 0, 0};
+            constexpr int UR = 8 / sizeof(T), UNITS = FM / UR;  // row fragments of a unit
+            V eres[UR];
+            auto fetch = [&](int jp, int u) {
+                if (u == 0) {
+                    const int col = min(ec + 32 * jp, p.n - 8);
+                    esw = load8(p.sw + col);
+                    if (p.bias) ebias = load8(p.bias + col);
+                }
+                if (p.res) {
+#pragma unroll
+                    for (int i = 0; i < UR; i++)
+                        eres[i] = buffer_load8<T>(rr, at(UR * u + i, jp, p.ldr),
+                                                  (16 * (UR * u + i) * (int)p.ldr + 32 * jp) * (int)sizeof(T));
+                }
+            };
+            fetch(0, 0);
+#pragma unroll
+            for (int s = 0; s < FN / 2 * UNITS; s++) {
+                const int jp = s / UNITS, u = s % UNITS;
+                V out[UR];
+#pragma unroll
+                for (int i = 0; i < UR; i++) {
+                    f32x8 v;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const auto x = __builtin_amdgcn_permlane16_swap(
+                            __float_as_uint((float)acc[UR * u + i][2 * jp][r]),
+                            __float_as_uint((float)acc[UR * u + i][2 * jp + 1][r]), false, false);
+                        v[r] = __uint_as_float(x[0]), v[r + 4] = __uint_as_float(x[1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = v[e] * sa[UR * u + i] * esw[e] + ebias[e];
+                    act8<ACT, sizeof(T) == 4>(v);
+                    if (p.res) v += __builtin_convertvector(eres[i], f32x8);
+                    out[i] = __builtin_convertvector(v, V);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // the following tile's second block is here before the first store
+                if (s == 0) wait_all();
+                if (s + 1 < FN / 2 * UNITS) fetch((s + 1) / UNITS, (s + 1) % UNITS);
+#pragma unroll
+                for (int i = 0; i < UR; i++)
+                    buffer_store8<T>(out[i], ry, at(UR * u + i, jp, p.ldy),
+                                     (16 * (UR * u + i) * (int)p.ldy + 32 * jp) * (int)sizeof(T));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!more) break;
+            number = following;
+        } else {
+            __syncthreads();
+            qmm_epilogue<Q, T, FM, FN>(p, acc, reinterpret_cast<float *>(lds) + wave * EpiRows * EpiPitch<FN>, m0 + rm,
+                                       n0 + rn - BM);
+            break;
+        }
+    }
 }
 
 // LDS of a tile kernel: its two buffers, or the epilogue of its waves.
@@ -425,30 +627,52 @@ __global__ __launch_bounds__(64 * WAVES) void qmm_rows_kernel(QmmArgs p) {
     }
 }
 
+template <int Q, typename T, int BM, int BN, int WN>
+static void qmm_dma_launch(const QmmArgs &p, bool fast, hipStream_t st) {
+    const int tiles = cdiv(p.m, BM) * cdiv(p.n, BN);
+    if (!fast) {
+        OSH_LAUNCH((qmm_dma_kernel<Q, T, 0, BM, BN, WN, false>), dim3((unsigned)tiles), dim3(128 * WN), (qmm_lds<BM, BN, 2, WN>()),
+                   st, p);
+        return;
+    }
+    const int grid = std::min(tiles, device_cus() * (BM * BN > 128 * 128 ? 1 : 2));
+#define OSH_QMM_ACT(ACT)                                                                                             \
+    case ACT:                                                                                                        \
+        OSH_LAUNCH((qmm_dma_kernel<Q, T, ACT, BM, BN, WN, true>), dim3((unsigned)grid), dim3(128 * WN), 2 * (BM + BN) * KB, st, p); \
+        break
+    switch (p.act) {
+        OSH_QMM_ACT(OSH_ACT_NONE);
+        OSH_QMM_ACT(OSH_ACT_RELU);
+        OSH_QMM_ACT(OSH_ACT_SILU);
+        OSH_QMM_ACT(OSH_ACT_GELU);
+    }
+#undef OSH_QMM_ACT
+}
+
 template <int Q, typename T>
 static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
 #define OSH_QMM_TILE(BM, BN, WM, WN)                                                                  \
     OSH_LAUNCH((qmm_tile_kernel<Q, T, BM, BN, WM, WN>), dim3((unsigned)(cdiv(p.m, BM) * cdiv(p.n, BN))), \
                dim3(64 * WM * WN), (qmm_lds<BM, BN, WM, WN>()), st, p)
-#define OSH_QMM_DMA(BM, BN)                                                                             \
-    OSH_LAUNCH((qmm_dma_kernel<Q, T, BM, BN>), dim3((unsigned)(cdiv(p.m, BM) * cdiv(p.n, BN))), dim3(256), \
-               (qmm_lds<BM, BN, 2, 2>()), st, p)
-    const bool aligned = (((uintptr_t)p.a | (uintptr_t)p.w | p.lda | p.ldw) & 15) == 0 && p.lda < (1 << 22) &&
-                         p.ldw < (1 << 22);
+    // direct loads: whole 16-byte chunks; offsets within a tile in 31 bits
+    const bool aligned = (((uintptr_t)p.a | (uintptr_t)p.w | p.lda | p.ldw) & 15) == 0 && p.k > KB &&
+                         std::max(p.lda, p.ldw) < (1 << 21);
+    const int e = 16 / sizeof(T);
+    const bool fast = aligned && p.n % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.res) & 15) == 0 && p.ldy % e == 0 &&
+                      p.ldr % e == 0 && std::max(p.ldy, p.ldr) < (1 << 20);
     if (p.m <= 16)
         OSH_LAUNCH((qmm_rows_kernel<Q, T, 1, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
     else if (p.m <= 32)
         OSH_LAUNCH((qmm_rows_kernel<Q, T, 2, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
     else if (aligned && (long long)cdiv(p.m, 256) * cdiv(p.n, 256) >= device_cus())
-        OSH_QMM_DMA(256, 256);
+        qmm_dma_launch<Q, T, 256, 256, 4>(p, fast, st);
     else if (aligned && (long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
-        OSH_QMM_DMA(128, 128);
+        qmm_dma_launch<Q, T, 128, 128, 2>(p, fast, st);
     else if ((long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
         OSH_QMM_TILE(128, 128, 2, 2);
     else
         OSH_QMM_TILE(64, 64, 2, 2);
 #undef OSH_QMM_TILE
-#undef OSH_QMM_DMA
     OSH_LAUNCH_CHECK("qmm kernel");
     return OSH_OK;
 }
