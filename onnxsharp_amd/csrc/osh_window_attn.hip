@@ -22,9 +22,10 @@ namespace osh {
 
 struct WinArgs {
     osh_window_attn p;
-    int group, tiles, splits;
+    int group, tile_rows, tiles, splits;
+    int page_shift;  // of a page that is a power of two, else -1
     float scale_log2;
-    float *part_o, *part_ml;  // of a split: [unit][split][16][head_dim], [unit][split][16][2]
+    float *part_o, *part_ml;  // of a split: [unit][split][tile_rows][head_dim], [unit][split][tile_rows][2]
 };
 
 template <typename T> struct Half8;
@@ -36,6 +37,48 @@ __device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
 }
 __device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Rows r0 .. r0 + n of a sequence whose lengths contradict each other.
+template <typename T>
+__device__ __forceinline__ void win_fill_nan(const osh_window_attn &p, const WinSeq &sq, int h, int G, int r0, int n,
+                                             int tid, int threads) {
+    const int d = p.head_dim;
+    for (int e = tid; e < n * d; e += threads) {
+        const int r = r0 + e / d;
+        if (r < sq.ql * G)
+            static_cast<T *>(p.d_o)[(long long)(sq.c0 + r / G) * p.o_stride[0] + (h * G + r % G) * p.o_stride[1] + e % d] =
+                (T)__builtin_nanf("");
+    }
+}
+
+// The tokens whose first row lies in rows r0 .. r0 + n go to their pages.
+template <typename T>
+__device__ __forceinline__ void win_append(const osh_window_attn &p, const WinSeq &sq, int b, int h, int G, int r0, int n,
+                                           int tid, int threads) {
+    const T *kn = static_cast<const T *>(p.d_k_new), *vn = static_cast<const T *>(p.d_v_new);
+    T *kp = static_cast<T *>(p.d_k_pages), *vp = static_cast<T *>(p.d_v_pages);
+    const int t0 = cdiv(r0, G), t1 = min(cdiv(r0 + n, G), sq.ql);
+    const int chunks = p.head_dim / 8;
+    for (int e = tid; e < (t1 - t0) * chunks; e += threads) {
+        const int t = t0 + e / chunks, c = e % chunks * 8;
+        const long long ko = win_cache_at(p, b, sq.past + t, p.k_stride, h);
+        const long long vo = win_cache_at(p, b, sq.past + t, p.v_stride, h);
+        if (ko < 0) continue;
+        const long long row = sq.c0 + t;
+        __builtin_memcpy(kp + ko + c, kn + row * p.k_new_stride[0] + h * p.k_new_stride[1] + c, 16);
+        __builtin_memcpy(vp + vo + c, vn + row * p.v_new_stride[0] + h * p.v_new_stride[1] + c, 16);
+    }
+}
+
+// Slot of a 16-byte chunk in an LDS row of C chunks: chunk ^ swizzle(row).
+template <int C>
+__device__ __forceinline__ int win_k_swizzle(int r) {
+    return C >= 16 ? r & 15 : C == 8 ? r >> 1 & 7 : r >> 2 & 3;
+}
+template <int C>
+__device__ __forceinline__ int win_v_swizzle(int r) {
+    return C >= 16 ? (r & 3) << 2 | (r >> 2 & 3) : C == 8 ? (r >> 1 & 1) << 2 : 0;
 }
 
 // One workgroup: 16 query rows of one key head, one split of their keys; each
@@ -73,32 +116,12 @@ __global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a)
     T *o = static_cast<T *>(p.d_o);
     const int my_row = r0 + jl, my_tok = min(my_row, rows - 1) / G, my_head = h * G + min(my_row, rows - 1) % G;
     if (!sq.ok) {
-        if (split == 0)
-            for (int e = tid; e < 16 * d; e += 64 * WAVES) {
-                const int r = r0 + e / d;
-                if (r < rows)
-                    o[(long long)(sq.c0 + r / G) * p.o_stride[0] + (h * G + r % G) * p.o_stride[1] + e % d] =
-                        (T)__builtin_nanf("");
-            }
+        if (split == 0) win_fill_nan<T>(p, sq, h, G, r0, 16, tid, 64 * WAVES);
         return;
     }
     const T *kn = static_cast<const T *>(p.d_k_new), *vn = static_cast<const T *>(p.d_v_new);
-    T *kp = static_cast<T *>(p.d_k_pages), *vp = static_cast<T *>(p.d_v_pages);
-
-    // the tokens whose first row lies in this block go to their pages
-    if (split == 0) {
-        const int t0 = (r0 + G - 1) / G, t1 = min((r0 + 16 + G - 1) / G, sq.ql);
-        const int chunks = d / 8;
-        for (int e = tid; e < (t1 - t0) * chunks; e += 64 * WAVES) {
-            const int t = t0 + e / chunks, c = e % chunks * 8;
-            const long long ko = win_cache_at(p, b, sq.past + t, p.k_stride, h);
-            const long long vo = win_cache_at(p, b, sq.past + t, p.v_stride, h);
-            if (ko < 0) continue;
-            const long long row = sq.c0 + t;
-            __builtin_memcpy(kp + ko + c, kn + row * p.k_new_stride[0] + h * p.k_new_stride[1] + c, 16);
-            __builtin_memcpy(vp + vo + c, vn + row * p.v_new_stride[0] + h * p.v_new_stride[1] + c, 16);
-        }
-    }
+    const T *kp = static_cast<const T *>(p.d_k_pages), *vp = static_cast<const T *>(p.d_v_pages);
+    if (split == 0) win_append<T>(p, sq, b, h, G, r0, 16, tid, 64 * WAVES);
 
     // queries: lane (jl, g) holds values 32 s + 8 g .. + 7 of row jl
     H8 q[KS];
@@ -247,31 +270,297 @@ __global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a)
     }
 }
 
-// Joins the splits of a row block: a workgroup a unit, a thread an output value.
+// ---------------------------------------------------------------- many rows
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// What stands in for a row that is not read: zeros for a key past the last one and
+// for the value of a page outside the cache, NaN (0x7fff in both types) for its key.
+#define WIN_NAN4 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu
+#define WIN_NAN32 WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4
+__device__ const unsigned win_zero_row[128] = {};
+__device__ const unsigned win_nan_row[128] = {WIN_NAN32, WIN_NAN32, WIN_NAN32, WIN_NAN32};
+#undef WIN_NAN4
+#undef WIN_NAN32
+
+// 16 bytes a lane from `from` to LDS: lane i's to dst + 16 i.
+__device__ __forceinline__ void copy_to_lds(const void *from, unsigned char *dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+// Of the 16 lanes of a group, lane 4 j + q reads values 4 q .. 4 q + 3 of row j; lane i
+// gets value i of rows 0..3.
+__device__ __forceinline__ s16x4 read_transposed(const unsigned char *at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+}
+
+// 32 NW query rows of one key head and a split of their keys: a wave owns 32 rows,
+// and tiles of 64 keys pass through two LDS buffers, loaded directly from the pages.
+// S^T = K Q^T leaves a lane the scores of half the keys at one query, and those of
+// each 16 keys are the operand that O^T = V^T P^T wants when its keys come in the
+// order 4 hl + 0..3, 8 + 4 hl + 0..3 (hl = lane / 32); V's operand is read so, by LDS
+// reads that transpose.
+//
+// C chunks of 16 bytes an LDS row, KS MFMA steps over a head's values, OB blocks of
+// 32 of them in the output.  Chunk c of a key's row lies at slot c ^ swizzle: keys'
+// rows spread a 16-lane read over all banks, values' rows one of 4 rows x 64 bytes.
+//
+// The running maximum moves only when a row's scores pass it by 2^8: weights up to
+// 256 are as exact, and most tiles rescale nothing.
+template <typename T, int C, int KS, int OB, int NW>
+__global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
+    using H8 = typename Half8<T>::type;
+    constexpr int BUF = 64 * C * 16, RPI = 64 / C, IT = 2 * C / NW;  // rows an instruction, instructions a wave
+    static_assert(IT * NW == 2 * C, "loads are dealt evenly");
+    extern __shared__ __align__(16) unsigned char lds[];  // two of [K tile][V tile]
+    const osh_window_attn &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ql32 = lane & 31, hl = lane >> 5;
+    const int d = p.head_dim, G = a.group;
+
+    int id = xcd_band(blockIdx.x, gridDim.x);
+    const int unit = id / a.splits, split = id - unit * a.splits;
+    id = unit;
+    const int tile = a.tiles - 1 - id % a.tiles;  // the rows with most keys first
+    id /= a.tiles;
+    const int h = id % p.kv_heads, b = id / p.kv_heads;
+    const WinSeq sq = win_seq(p, b);
+    const int rows = sq.ql * G, r0 = tile * 32 * NW;
+    if (r0 >= rows) return;
+    T *o = static_cast<T *>(p.d_o);
+    const int row = min(r0 + 32 * wave + ql32, rows - 1), tok = row / G, head = h * G + row % G;
+    if (!sq.ok) {
+        if (split == 0) win_fill_nan<T>(p, sq, h, G, r0, 32 * NW, tid, 64 * NW);
+        return;
+    }
+    const T *kn = static_cast<const T *>(p.d_k_new), *vn = static_cast<const T *>(p.d_v_new);
+    const T *kp = static_cast<const T *>(p.d_k_pages), *vp = static_cast<const T *>(p.d_v_pages);
+    if (split == 0) win_append<T>(p, sq, b, h, G, r0, 32 * NW, tid, 64 * NW);
+
+    H8 q[KS];
+    {
+        const T *qr = static_cast<const T *>(p.d_q) + (long long)(sq.c0 + tok) * p.q_stride[0] + head * p.q_stride[1];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            q[s] = H8{};
+            if (16 * s + 8 * hl < d) __builtin_memcpy(&q[s], qr + 16 * s + 8 * hl, 16);
+        }
+    }
+    const int last = min(r0 + 32 * NW - 1, rows - 1);
+    const WinKeys keys = win_keys(p, sq, r0 / G, last / G);
+    const int nt_all = cdiv(keys.count, 64), per = cdiv(nt_all, a.splits);
+    const int t_end = min(nt_all, (split + 1) * per);
+    // by key number: this row sees v <= v_hi with v >= v_lo or v < v_sink, and the wave's
+    // rows together none outside [0, w_hi], all of [w_lo, w_all] (and of [0, v_sink))
+    const int base = keys.sink_end - keys.lo, pos = sq.past + tok;
+    const int v_sink = max(keys.sink_end, win_min(p.sinks, 1 << 30) + base);
+    const int v_hi = pos + base, v_lo = max(pos - p.window + 1, keys.lo) + base;
+    const int wr = r0 + 32 * wave, tok0 = win_min(wr, rows - 1) / G, tok1 = win_min(wr + 31, rows - 1) / G;
+    const int w_hi = sq.past + tok1 + base, w_all = sq.past + tok0 + base;
+    const int w_lo = max(sq.past + tok1 - p.window + 1, keys.lo) + base;
+    const int w_first = max(sq.past + tok0 - p.window + 1, keys.lo) + base;  // below it only sinks
+
+    // loads: instruction i (K for i < C) covers rows RPI (i % C) + lane / C; a wave has
+    // instructions wave + NW e, whose rows repeat for V after C
+    constexpr int RW = IT / 2 > 0 ? IT / 2 : 1;  // rows of a lane in a tile
+    const int slot = lane % C;
+    auto tile_row = [&](int e) { return (wave + NW * e) % C * RPI + lane / C; };
+    int page_id[RW];
+    auto fetch_pages = [&](int t) {
+#pragma unroll
+        for (int e = 0; e < RW; e++) {
+            const int v = t * 64 + tile_row(e), j = keys.at(v);
+            page_id[e] = 0;
+            if (v < keys.count && j < sq.past)
+                page_id[e] = p.d_table[b * p.table_stride + (a.page_shift >= 0 ? j >> a.page_shift : j / p.page)];
+        }
+    };
+    auto load_tile = [&](int t, int buf) {
+#pragma unroll
+        for (int e = 0; e < RW; e++) {
+            const int r = tile_row(e), v = t * 64 + r, j = keys.at(v);
+            const T *kr, *vr;
+            if (v >= keys.count) {
+                kr = vr = reinterpret_cast<const T *>(win_zero_row);
+            } else if (j >= sq.past) {
+                const long long n = sq.c0 + j - sq.past;
+                kr = kn + n * p.k_new_stride[0] + h * p.k_new_stride[1];
+                vr = vn + n * p.v_new_stride[0] + h * p.v_new_stride[1];
+            } else {
+                const int in = a.page_shift >= 0 ? j & (p.page - 1) : j % p.page;
+                kr = kp + page_id[e] * p.k_stride[0] + in * p.k_stride[1] + h * p.k_stride[2];
+                vr = vp + page_id[e] * p.v_stride[0] + in * p.v_stride[1] + h * p.v_stride[2];
+                if ((unsigned)page_id[e] >= (unsigned)p.pages) {
+                    kr = reinterpret_cast<const T *>(win_nan_row);
+                    vr = reinterpret_cast<const T *>(win_zero_row);
+                }
+            }
+            const int kc = slot ^ win_k_swizzle<C>(r), vc = slot ^ win_v_swizzle<C>(r);
+            unsigned char *dst = lds + buf * 2 * BUF + (wave + NW * e) % C * 1024;
+            const bool is_k = wave + NW * e < C, is_v = IT > 1 || !is_k;
+            if (is_k && 8 * kc < d) copy_to_lds(kr + 8 * kc, dst);
+            if (is_v && 8 * vc < d) copy_to_lds(vr + 8 * vc, dst + BUF);
+        }
+    };
+
+    if (d < 8 * C) {  // the slots of no value stay zero
+        for (int e = tid; e < 4 * BUF / 16; e += 64 * NW) reinterpret_cast<uint4 *>(lds)[e] = uint4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    int t = split * per;
+    if (t < t_end) {
+        fetch_pages(t);
+        load_tile(t, 0);
+        if (t + 1 < t_end) fetch_pages(t + 1);
+    }
+    float m = -__builtin_inff(), l = 0.0f;  // m in units of 2^, after the scale
+    f32x16 acc[OB];
+#pragma unroll
+    for (int i = 0; i < OB; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][r] = 0.0f;
+    int buf = 0;
+    for (; t < t_end; t++, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t + 1 < t_end) {
+            load_tile(t + 1, buf ^ 1);
+            if (t + 2 < t_end) fetch_pages(t + 2);
+        }
+        const int v0 = t * 64;
+        if (v0 > w_hi || (v0 >= v_sink && v0 + 63 < w_first)) continue;  // the wave sees none
+        const unsigned char *kt = lds + buf * 2 * BUF, *vt = kt + BUF;
+        f32x16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[kb][r] = 0.0f;
+            const int r = 32 * kb + ql32;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                H8 k;
+                __builtin_memcpy(&k, kt + r * (C * 16) + (((2 * i + hl) ^ win_k_swizzle<C>(r)) << 4), 16);
+                s[kb] = mma32(k, q[i], s[kb]);
+            }
+        }
+        if (v0 + 63 > w_all || (v0 + 63 >= v_sink && v0 < w_lo)) {  // some row sees only some
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int v = v0 + 32 * kb + 8 * (r >> 2) + 4 * hl + (r & 3);
+                    if (v > v_hi || (v < v_lo && v >= v_sink)) s[kb][r] = -__builtin_inff();
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) top = __builtin_fmaxf(top, s[kb][r]);
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
+            const float old = m;
+            m = __builtin_fmaxf(m, top);
+            const float fade = old == m ? 1.0f : __builtin_amdgcn_exp2f(old - m);
+            l *= fade;
+#pragma unroll
+            for (int i = 0; i < OB; i++) acc[i] *= fade;
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
+        H8 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f32x8 f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], a.scale_log2, -ref));
+                l += f[i];
+            }
+            w[e] = __builtin_convertvector(f, H8);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            // this lane reads row key + lane % 16 / 4, values 16 (lane / 16 % 2) + 4 (lane % 4)
+            const int key = 16 * e + 4 * hl + (lane >> 2 & 3), off = (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+            const unsigned char *r0p = vt + key * (C * 16), *r1p = r0p + 8 * (C * 16);
+#pragma unroll
+            for (int i = 0; i < OB; i++) {
+                const int c = 4 * i + (off >> 4);
+                const s16x4 x0 = read_transposed(r0p + ((c ^ win_v_swizzle<C>(key)) << 4) + (off & 15));
+                const s16x4 x1 = read_transposed(r1p + ((c ^ win_v_swizzle<C>(key + 8)) << 4) + (off & 15));
+                const s16x8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                H8 vh;
+                __builtin_memcpy(&vh, &x, 16);
+                acc[i] = mma32(vh, w[e], acc[i]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    // quads of values 8 e + 4 hl + 0..3: exchanging one quad between the halves of the
+    // wave leaves a lane 8 neighbouring values
+    const bool mine = wr + ql32 < rows;
+    const float inv = a.splits == 1 ? 1.0f / l : 1.0f;
+    const long long u = (long long)unit * a.splits + split;
+    const int tr = 32 * wave + ql32;
+    if (a.splits > 1 && mine && hl == 0) {
+        a.part_ml[(u * 32 * NW + tr) * 2] = m;
+        a.part_ml[(u * 32 * NW + tr) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < OB; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            f32x8 f;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][4 * e + r] * inv),
+                                                                __float_as_uint(acc[i][4 * e + 4 + r] * inv), false,
+                                                                false);
+                f[r] = __uint_as_float(x[0]), f[r + 4] = __uint_as_float(x[1]);
+            }
+            const int c = 32 * i + 8 * (e + hl);
+            if (!mine || c >= d) continue;
+            if (a.splits == 1)
+                store8(o + (long long)(sq.c0 + tok) * p.o_stride[0] + head * p.o_stride[1] + c, f);
+            else
+                store8(a.part_o + (u * 32 * NW + tr) * d + c, f);
+        }
+}
+
+// Joins the splits of a row block: a workgroup 16 rows, a thread an output value.
 template <typename T>
 __global__ __launch_bounds__(256) void window_attn_join_kernel(WinArgs a) {
     const osh_window_attn &p = a.p;
-    const int unit = blockIdx.x, d = p.head_dim, G = a.group;
+    const int parts = a.tile_rows / 16, unit = blockIdx.x / parts, d = p.head_dim, G = a.group;
     int id = unit;
-    const int tile = id % a.tiles;
+    const int tile = a.tile_rows > 16 ? a.tiles - 1 - id % a.tiles : id % a.tiles;
     id /= a.tiles;
     const int h = id % p.kv_heads, b = id / p.kv_heads;
     const WinSeq sq = win_seq(p, b);
     if (!sq.ok) return;
-    const int rows = sq.ql * G, r0 = tile * 16;
+    const int rows = sq.ql * G, r0 = tile * a.tile_rows, sub = blockIdx.x % parts * 16;
     for (int e = threadIdx.x; e < 16 * d; e += 256) {
-        const int r = e / d, c = e % d, row = r0 + r;
+        const int r = sub + e / d, c = e % d, row = r0 + r;
         if (row >= rows) break;
-        const float *ml = a.part_ml + (long long)unit * a.splits * 32 + r * 2;
-        const float *os = a.part_o + (long long)unit * a.splits * 16 * d + e;
+        const float *ml = a.part_ml + ((long long)unit * a.splits * a.tile_rows + r) * 2;
+        const float *os = a.part_o + ((long long)unit * a.splits * a.tile_rows + r) * d + c;
+        const long long next = a.tile_rows;
         float mm = -__builtin_inff();
-        for (int s = 0; s < a.splits; s++) mm = __builtin_fmaxf(mm, ml[s * 32]);
+        for (int s = 0; s < a.splits; s++) mm = __builtin_fmaxf(mm, ml[s * next * 2]);
         const float base = mm == -__builtin_inff() ? 0.0f : mm;
         float sum = 0.0f, ll = 0.0f;
         for (int s = 0; s < a.splits; s++) {
-            const float f = __builtin_amdgcn_exp2f(ml[s * 32] - base);
-            ll += f * ml[s * 32 + 1];
-            sum += f * os[(long long)s * 16 * d];
+            const float f = __builtin_amdgcn_exp2f(ml[s * next * 2] - base);
+            ll += f * ml[s * next * 2 + 1];
+            sum += f * os[s * next * d];
         }
         static_cast<T *>(p.d_o)[(long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1] +
                                 c] = (T)(sum / ll);
@@ -300,16 +589,36 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
     a.group = p->q_heads / p->kv_heads;
     if ((long long)p->max_q * a.group > (1 << 30))
         return fail(OSH_E_UNSUPPORTED, "WindowAttention: %d new tokens of %d heads", p->max_q, p->q_heads);
-    a.tiles = cdiv(p->max_q * a.group, 16);
+    a.page_shift = (p->page & (p->page - 1)) == 0 ? __builtin_ctz(p->page) : -1;
     a.scale_log2 = (p->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)p->head_dim) : p->scale) * 1.4426950408889634f;
-    const long long units = (long long)p->batch * p->kv_heads * a.tiles;
+    const int rows = p->max_q * a.group;
+    const long long heads = (long long)p->batch * p->kv_heads;
+    a.tile_rows = rows >= 64 ? (p->head_dim > 128 ? 128 : 256) : 16;
+    a.tiles = cdiv(rows, a.tile_rows);
+    const long long units = heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "WindowAttention: too many row blocks (%lld)", units);
-    const long long span = std::min<long long>(p->max_kv, (long long)p->window + p->sinks + 15);
-    const long long want = units ? (2LL * device_cus() + units - 1) / units : 1;
+    const long long span = std::min<long long>(p->max_kv, (long long)p->window + p->sinks + a.tile_rows / a.group);
+    const long long want = units ? ((a.tile_rows > 16 ? 1LL : 2LL) * device_cus() + units - 1) / units : 1;
     a.splits = (int)std::max(1LL, std::min(want, span / 256));
     const long long parts = a.splits > 1 ? units * a.splits : 0;
-    scratch = (size_t)parts * 16 * (p->head_dim + 2) * 4;
+    scratch = (size_t)parts * a.tile_rows * (p->head_dim + 2) * 4;
     return OSH_OK;
+}
+
+template <typename T>
+static osh_status win_join(const WinArgs &a, unsigned units, hipStream_t st) {
+    if (a.splits > 1) {
+        OSH_LAUNCH(window_attn_join_kernel<T>, dim3(units * (a.tile_rows / 16)), dim3(256), 0, st, a);
+        OSH_LAUNCH_CHECK("window_attn_join_kernel");
+    }
+    return OSH_OK;
+}
+
+template <typename T, int C, int KS, int OB, int NW>
+static osh_status win_tile_launch(const WinArgs &a, unsigned units, hipStream_t st) {
+    OSH_LAUNCH((window_attn_tile_kernel<T, C, KS, OB, NW>), dim3(units * a.splits), dim3(64 * NW), 4 * 64 * C * 16, st, a);
+    OSH_LAUNCH_CHECK("window_attn_tile_kernel");
+    return win_join<T>(a, units, st);
 }
 
 template <typename T, int DP, int WAVES>
@@ -317,15 +626,18 @@ static osh_status win_launch(const WinArgs &a, unsigned units, hipStream_t st) {
     constexpr size_t lds = std::max<size_t>(WAVES * 64 * sizeof(void *), WAVES * 16 * (DP + 2) * sizeof(float));
     OSH_LAUNCH((window_attn_rows_kernel<T, DP, WAVES>), dim3(units * a.splits), dim3(64 * WAVES), lds, st, a);
     OSH_LAUNCH_CHECK("window_attn_rows_kernel");
-    if (a.splits > 1) {
-        OSH_LAUNCH(window_attn_join_kernel<T>, dim3(units), dim3(256), 0, st, a);
-        OSH_LAUNCH_CHECK("window_attn_join_kernel");
-    }
-    return OSH_OK;
+    return win_join<T>(a, units, st);
 }
 
 template <typename T>
 static osh_status win_launch_t(const WinArgs &a, unsigned units, hipStream_t st) {
+    if (a.tile_rows > 16) {
+        if (a.p.head_dim <= 32) return win_tile_launch<T, 4, 2, 1, 8>(a, units, st);
+        if (a.p.head_dim <= 64) return win_tile_launch<T, 8, 4, 2, 8>(a, units, st);
+        if (a.p.head_dim <= 96) return win_tile_launch<T, 16, 6, 3, 8>(a, units, st);
+        if (a.p.head_dim <= 128) return win_tile_launch<T, 16, 8, 4, 8>(a, units, st);
+        return win_tile_launch<T, 32, 16, 8, 4>(a, units, st);
+    }
     if (a.p.head_dim <= 64) return win_launch<T, 64, 4>(a, units, st);
     if (a.p.head_dim <= 128) return win_launch<T, 128, 4>(a, units, st);
     return win_launch<T, 256, 4>(a, units, st);
@@ -365,7 +677,7 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
         return fail(OSH_E_INVALID, "WindowAttention: o overlaps an operand");
     const long long units = (long long)p->batch * p->kv_heads * a.tiles;
     a.part_ml = static_cast<float *>(d_scratch);
-    a.part_o = a.part_ml + units * a.splits * 32;
+    a.part_o = a.part_ml + units * a.splits * a.tile_rows * 2;
     return p->dtype == OSH_T_F16 ? win_launch_t<_Float16>(a, (unsigned)units, to_stream(s))
                                  : win_launch_t<__bf16>(a, (unsigned)units, to_stream(s));
 }
