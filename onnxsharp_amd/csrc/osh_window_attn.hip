@@ -11,6 +11,8 @@
 // 2^(s - m) and the weighted sum of values; a larger maximum rescales both by
 // 2^(m_old - m).  Waves and splits that saw different keys are joined by the same
 // rule.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "osh_lm.h"
@@ -23,10 +25,13 @@ namespace osh {
 struct WinArgs {
     osh_window_attn p;
     int group, tile_rows, tiles, splits;
+    bool wide;       // few rows: eight waves a row block instead of four and splits
     int page_shift;  // of a page that is a power of two, else -1
     float scale_log2;
     float *part_o, *part_ml;  // of a split: [unit][split][tile_rows][head_dim], [unit][split][tile_rows][2]
 };
+
+constexpr int WIN_MAX_SPLITS = 64;  // a lane a split in the join
 
 template <typename T> struct Half8;
 template <> struct Half8<_Float16> { using type = f16x8; };
@@ -38,6 +43,15 @@ __device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
 __device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+
+// What stands in for a row that is not read: zeros for a key past the last one and
+// for the value of a page outside the cache, NaN (0x7fff in both types) for its key.
+#define WIN_NAN4 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu
+#define WIN_NAN32 WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4
+__device__ const unsigned win_zero_row[128] = {};
+__device__ const unsigned win_nan_row[128] = {WIN_NAN32, WIN_NAN32, WIN_NAN32, WIN_NAN32};
+#undef WIN_NAN4
+#undef WIN_NAN32
 
 // Rows r0 .. r0 + n of a sequence whose lengths contradict each other.
 template <typename T>
@@ -81,6 +95,47 @@ __device__ __forceinline__ int win_v_swizzle(int r) {
     return C >= 16 ? (r & 3) << 2 | (r >> 2 & 3) : C == 8 ? (r >> 1 & 1) << 2 : 0;
 }
 
+// Where a key's rows of K and V are; its page is looked up one step ahead.  Selects
+// in place of branches: the lanes of a wave mix new tokens, pages and keys past the
+// end (branches cost 30 us of the 340 of an 8192-token prompt).  Strides fit 31 bits.
+template <typename T>
+struct WinRows {
+    const T *k, *v;
+};
+template <typename T>
+__device__ __forceinline__ const T *win_row(bool fresh, unsigned i0, unsigned i1, const void *fresh_base,
+                                            const int64_t *fresh_stride, const void *base, const int64_t *stride, int h) {
+    const T *f = static_cast<const T *>(fresh_base) + h * fresh_stride[1];
+    const T *c = static_cast<const T *>(base) + h * stride[2];
+    const unsigned s0 = fresh ? (unsigned)fresh_stride[0] : (unsigned)stride[0];
+    return (fresh ? f : c) + ((unsigned long long)i0 * s0 + (unsigned long long)i1 * (unsigned)stride[1]);
+}
+template <typename T>
+__device__ __forceinline__ WinRows<T> win_rows(const osh_window_attn &p, const WinSeq &sq, const WinKeys &keys, int v,
+                                               int page_id, int page_shift, int h) {
+    const int j = keys.at(v);
+    const bool past_end = v >= keys.count, fresh = j >= sq.past;
+    const bool bad = !fresh && (unsigned)page_id >= (unsigned)p.pages;
+    const unsigned in = page_shift >= 0 ? j & (p.page - 1) : j % p.page;
+    const unsigned i0 = fresh ? sq.c0 + j - sq.past : page_id, i1 = fresh ? 0 : in;
+    WinRows<T> r;
+    r.k = win_row<T>(fresh, i0, i1, p.d_k_new, p.k_new_stride, p.d_k_pages, p.k_stride, h);
+    r.v = win_row<T>(fresh, i0, i1, p.d_v_new, p.v_new_stride, p.d_v_pages, p.v_stride, h);
+    if (past_end || bad) {
+        r.k = reinterpret_cast<const T *>(past_end ? win_zero_row : win_nan_row);
+        r.v = reinterpret_cast<const T *>(win_zero_row);
+    }
+    return r;
+}
+__device__ __forceinline__ int win_page(const osh_window_attn &p, const WinSeq &sq, const WinKeys &keys, int b, int v,
+                                        int page_shift) {
+    if (sq.past == 0) return 0;
+    const int j = win_min(keys.at(v), sq.past - 1);  // a key past the pages takes no page
+    return p.d_table[b * p.table_stride + (page_shift >= 0 ? j >> page_shift : j / p.page)];
+}
+
+// ----------------------------------------------------------------- few rows
+
 // One workgroup: 16 query rows of one key head, one split of their keys; each
 // wave takes every WAVES-th step of 32 keys of the split.
 //
@@ -90,11 +145,17 @@ __device__ __forceinline__ int win_v_swizzle(int r) {
 // O^T = V^T P^T, without a move between lanes.  A lane loads ND neighbouring values
 // of its 8 keys of V and turns the 8 x ND block around in registers; MFMA i then
 // takes values ND jl + i of all lanes.
+//
+// Memory's latency is what a step waits for, so the next step's K and V are loaded
+// before this one is computed (BUFS 2; heads above 128 have no registers for it),
+// their addresses pass through the wave's LDS the step before, and the page ids
+// they need are loaded the step before that.
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a) {
+__global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void window_attn_rows_kernel(WinArgs a) {
     constexpr int NS = DP > 128 ? 2 : 1;       // sets of up to 128 values
     constexpr int ND = DP >= 128 ? 8 : 4;      // neighbouring values of a lane in a set
     constexpr int KS = DP / 32;                // MFMA steps over the head's values
+    constexpr int BUFS = DP > 128 ? 1 : 2;
     using H8 = typename Half8<T>::type;
     extern __shared__ __align__(16) unsigned char lds[];
     const osh_window_attn &p = a.p;
@@ -119,9 +180,6 @@ __global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a)
         if (split == 0) win_fill_nan<T>(p, sq, h, G, r0, 16, tid, 64 * WAVES);
         return;
     }
-    const T *kn = static_cast<const T *>(p.d_k_new), *vn = static_cast<const T *>(p.d_v_new);
-    const T *kp = static_cast<const T *>(p.d_k_pages), *vp = static_cast<const T *>(p.d_v_pages);
-    if (split == 0) win_append<T>(p, sq, b, h, G, r0, 16, tid, 64 * WAVES);
 
     // queries: lane (jl, g) holds values 32 s + 8 g .. + 7 of row jl
     H8 q[KS];
@@ -149,53 +207,52 @@ __global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a)
         for (int i = 0; i < ND; i++) acc[n][i] = f32x4{0, 0, 0, 0};
 
     const T **at = reinterpret_cast<const T **>(lds) + wave * 64;  // a step's rows of K, then of V
-    for (int st = split * per + wave; st < s_end; st += WAVES) {
-        {
-            const int v = st * 32 + (lane & 31), j = keys.at(v);
-            const bool is_v = lane >= 32;
-            const T *row = nullptr;
-            if (v < nv) {
-                if (j >= sq.past) {
-                    const long long t = sq.c0 + j - sq.past;
-                    row = is_v ? vn + t * p.v_new_stride[0] + h * p.v_new_stride[1]
-                               : kn + t * p.k_new_stride[0] + h * p.k_new_stride[1];
-                } else {
-                    const long long off = win_cache_at(p, b, j, is_v ? p.v_stride : p.k_stride, h);
-                    if (off >= 0) row = (is_v ? vp : kp) + off;
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            at[lane] = row;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
-        f32x4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    struct Step {
+        H8 k[2][KS];
+        unsigned v[NS][8][ND / 2];
+    };
+    int page_id = 0;
+    auto fetch = [&](int st) {
+        if (st < s_end) page_id = win_page(p, sq, keys, b, st * 32 + (lane & 31), a.page_shift);
+    };
+    auto place = [&](int st) {
+        if (st >= s_end) return;
+        const WinRows<T> r = win_rows<T>(p, sq, keys, st * 32 + (lane & 31), page_id, a.page_shift, h);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        at[lane] = lane < 32 ? r.k : r.v;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    const T *zero = reinterpret_cast<const T *>(win_zero_row);
+    auto load = [&](int st, Step &x) {
+        if (st >= s_end) return;
 #pragma unroll
         for (int bl = 0; bl < 2; bl++) {
             const T *row = at[8 * (jl >> 2) + 4 * bl + (jl & 3)];
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                H8 k{};
-                if (row && 32 * s + 8 * g < d) __builtin_memcpy(&k, row + 32 * s + 8 * g, 16);
-                sc[bl] = mma16(k, q[s], sc[bl]);
-            }
+            for (int s = 0; s < KS; s++)
+                __builtin_memcpy(&x.k[bl][s], 32 * s + 8 * g < d ? row + 32 * s + 8 * g : zero, 16);
         }
-        unsigned vv[NS][8][ND / 2];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const T *row = at[32 + 8 * g + j];
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+                __builtin_memcpy(x.v[n][j], 128 * n + ND * jl < d ? row + 128 * n + ND * jl : zero, 2 * ND);
+        }
+    };
+    auto compute = [&](int st, const Step &x) {
+        f32x4 sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int bl = 0; bl < 2; bl++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) sc[bl] = mma16(x.k[bl][s], q[s], sc[bl]);
         float s8[8], top = m;
 #pragma unroll
-        for (int j8 = 0; j8 < 8; j8++) {
-            const T *row = at[32 + 8 * g + j8];
-#pragma unroll
-            for (int n = 0; n < NS; n++) {
-#pragma unroll
-                for (int i = 0; i < ND / 2; i++) vv[n][j8][i] = 0;
-                if (row && 128 * n + ND * jl < d) __builtin_memcpy(vv[n][j8], row + 128 * n + ND * jl, 2 * ND);
-            }
-            const int v = st * 32 + 8 * g + j8, j = keys.at(v);
-            const bool seen = v < nv && win_sees(p, my_pos, j);
-            float s = sc[j8 >> 2][j8 & 3] * a.scale_log2;
-            if (!row) s = __builtin_nanf("");
-            s8[j8] = seen ? s : -__builtin_inff();
-            top = __builtin_fmaxf(top, s8[j8]);
+        for (int i = 0; i < 8; i++) {
+            const int v = st * 32 + 8 * g + i;
+            const bool seen = v < nv && win_sees(p, my_pos, keys.at(v));
+            s8[i] = seen ? sc[i >> 2][i & 3] * a.scale_log2 : -__builtin_inff();
+            top = __builtin_fmaxf(top, s8[i]);
         }
         top = __builtin_fmaxf(top, __shfl_xor(top, 16));
         top = __builtin_fmaxf(top, __shfl_xor(top, 32));
@@ -217,14 +274,42 @@ __global__ __launch_bounds__(64 * WAVES) void window_attn_rows_kernel(WinArgs a)
                 unsigned vt[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    vt[e] = __builtin_amdgcn_perm(vv[n][2 * e + 1][i / 2], vv[n][2 * e][i / 2],
+                    vt[e] = __builtin_amdgcn_perm(x.v[n][2 * e + 1][i / 2], x.v[n][2 * e][i / 2],
                                                   i & 1 ? 0x07060302u : 0x05040100u);
                 H8 vh;
                 __builtin_memcpy(&vh, vt, 16);
                 acc[n][i] *= fade;
                 acc[n][i] = mma16(vh, pw, acc[n][i]);
             }
+    };
+    int st = split * per + wave;
+    fetch(st);
+    place(st);
+    fetch(st + WAVES);
+    Step x[BUFS];
+    if constexpr (BUFS == 2) {
+        load(st, x[0]);
+        place(st + WAVES);
+        fetch(st + 2 * WAVES);
+        for (; st < s_end; st += 2 * WAVES) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int now = st + e * WAVES;
+                load(now + WAVES, x[e ^ 1]);
+                place(now + 2 * WAVES);
+                fetch(now + 3 * WAVES);
+                if (now < s_end) compute(now, x[e]);
+            }
+        }
+    } else {
+        for (; st < s_end; st += WAVES) {
+            load(st, x[0]);
+            place(st + WAVES);
+            fetch(st + 2 * WAVES);
+            compute(st, x[0]);
+        }
     }
+    if (split == 0) win_append<T>(p, sq, b, h, G, r0, 16, tid, 64 * WAVES);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
@@ -282,15 +367,6 @@ __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// What stands in for a row that is not read: zeros for a key past the last one and
-// for the value of a page outside the cache, NaN (0x7fff in both types) for its key.
-#define WIN_NAN4 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu
-#define WIN_NAN32 WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4, WIN_NAN4
-__device__ const unsigned win_zero_row[128] = {};
-__device__ const unsigned win_nan_row[128] = {WIN_NAN32, WIN_NAN32, WIN_NAN32, WIN_NAN32};
-#undef WIN_NAN4
-#undef WIN_NAN32
-
 // 16 bytes a lane from `from` to LDS: lane i's to dst + 16 i.
 __device__ __forceinline__ void copy_to_lds(const void *from, unsigned char *dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
@@ -342,8 +418,6 @@ __global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
         if (split == 0) win_fill_nan<T>(p, sq, h, G, r0, 32 * NW, tid, 64 * NW);
         return;
     }
-    const T *kn = static_cast<const T *>(p.d_k_new), *vn = static_cast<const T *>(p.d_v_new);
-    const T *kp = static_cast<const T *>(p.d_k_pages), *vp = static_cast<const T *>(p.d_v_pages);
     if (split == 0) win_append<T>(p, sq, b, h, G, r0, 32 * NW, tid, 64 * NW);
 
     H8 q[KS];
@@ -377,38 +451,18 @@ __global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
     int page_id[RW];
     auto fetch_pages = [&](int t) {
 #pragma unroll
-        for (int e = 0; e < RW; e++) {
-            const int v = t * 64 + tile_row(e), j = keys.at(v);
-            page_id[e] = 0;
-            if (v < keys.count && j < sq.past)
-                page_id[e] = p.d_table[b * p.table_stride + (a.page_shift >= 0 ? j >> a.page_shift : j / p.page)];
-        }
+        for (int e = 0; e < RW; e++) page_id[e] = win_page(p, sq, keys, b, t * 64 + tile_row(e), a.page_shift);
     };
     auto load_tile = [&](int t, int buf) {
 #pragma unroll
         for (int e = 0; e < RW; e++) {
-            const int r = tile_row(e), v = t * 64 + r, j = keys.at(v);
-            const T *kr, *vr;
-            if (v >= keys.count) {
-                kr = vr = reinterpret_cast<const T *>(win_zero_row);
-            } else if (j >= sq.past) {
-                const long long n = sq.c0 + j - sq.past;
-                kr = kn + n * p.k_new_stride[0] + h * p.k_new_stride[1];
-                vr = vn + n * p.v_new_stride[0] + h * p.v_new_stride[1];
-            } else {
-                const int in = a.page_shift >= 0 ? j & (p.page - 1) : j % p.page;
-                kr = kp + page_id[e] * p.k_stride[0] + in * p.k_stride[1] + h * p.k_stride[2];
-                vr = vp + page_id[e] * p.v_stride[0] + in * p.v_stride[1] + h * p.v_stride[2];
-                if ((unsigned)page_id[e] >= (unsigned)p.pages) {
-                    kr = reinterpret_cast<const T *>(win_nan_row);
-                    vr = reinterpret_cast<const T *>(win_zero_row);
-                }
-            }
+            const int r = tile_row(e);
+            const WinRows<T> at = win_rows<T>(p, sq, keys, t * 64 + r, page_id[e], a.page_shift, h);
             const int kc = slot ^ win_k_swizzle<C>(r), vc = slot ^ win_v_swizzle<C>(r);
             unsigned char *dst = lds + buf * 2 * BUF + (wave + NW * e) % C * 1024;
             const bool is_k = wave + NW * e < C, is_v = IT > 1 || !is_k;
-            if (is_k && 8 * kc < d) copy_to_lds(kr + 8 * kc, dst);
-            if (is_v && 8 * vc < d) copy_to_lds(vr + 8 * vc, dst + BUF);
+            if (is_k && 8 * kc < d) copy_to_lds(at.k + 8 * kc, dst);
+            if (is_v && 8 * vc < d) copy_to_lds(at.v + 8 * vc, dst + BUF);
         }
     };
 
@@ -535,35 +589,52 @@ __global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
         }
 }
 
-// Joins the splits of a row block: a workgroup 16 rows, a thread an output value.
+// Joins the splits of four rows, a wave a row: the splits' weights first, a lane a
+// split, then the sums, eight splits' loads in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void window_attn_join_kernel(WinArgs a) {
     const osh_window_attn &p = a.p;
-    const int parts = a.tile_rows / 16, unit = blockIdx.x / parts, d = p.head_dim, G = a.group;
+    const int quads = a.tile_rows / 4, d = p.head_dim, G = a.group;
+    const int unit = blockIdx.x / quads, lane = threadIdx.x & 63;
     int id = unit;
     const int tile = a.tile_rows > 16 ? a.tiles - 1 - id % a.tiles : id % a.tiles;
     id /= a.tiles;
     const int h = id % p.kv_heads, b = id / p.kv_heads;
     const WinSeq sq = win_seq(p, b);
-    if (!sq.ok) return;
-    const int rows = sq.ql * G, r0 = tile * a.tile_rows, sub = blockIdx.x % parts * 16;
-    for (int e = threadIdx.x; e < 16 * d; e += 256) {
-        const int r = sub + e / d, c = e % d, row = r0 + r;
-        if (row >= rows) break;
-        const float *ml = a.part_ml + ((long long)unit * a.splits * a.tile_rows + r) * 2;
-        const float *os = a.part_o + ((long long)unit * a.splits * a.tile_rows + r) * d + c;
-        const long long next = a.tile_rows;
-        float mm = -__builtin_inff();
-        for (int s = 0; s < a.splits; s++) mm = __builtin_fmaxf(mm, ml[s * next * 2]);
-        const float base = mm == -__builtin_inff() ? 0.0f : mm;
-        float sum = 0.0f, ll = 0.0f;
-        for (int s = 0; s < a.splits; s++) {
-            const float f = __builtin_amdgcn_exp2f(ml[s * next * 2] - base);
-            ll += f * ml[s * next * 2 + 1];
-            sum += f * os[s * next * d];
+    const int r = blockIdx.x % quads * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = tile * a.tile_rows + r;
+    if (!sq.ok || row >= sq.ql * G) return;
+    const float *ml = a.part_ml + ((long long)unit * a.splits * a.tile_rows + r) * 2;
+    const float *os = a.part_o + ((long long)unit * a.splits * a.tile_rows + r) * d;
+    const long long next = a.tile_rows;
+    const bool mine = lane < a.splits;  // at most WIN_MAX_SPLITS = 64
+    const float m = mine ? ml[lane * next * 2] : -__builtin_inff(), l = mine ? ml[lane * next * 2 + 1] : 0.0f;
+    float top = m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+    const float w = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.0f : top));
+    float sum = w * l;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    const float scale = w / sum;
+    T *out = static_cast<T *>(p.d_o) + (long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1];
+    for (int c = lane * 2; c < d; c += 128) {
+        float2 f = {0.0f, 0.0f};
+        for (int s = 0; s < a.splits; s += 8) {
+            float2 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                v[e] = *reinterpret_cast<const float2 *>(os + min(s + e, a.splits - 1) * next * d + c);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                // lanes past the head's values left the loop: read the weight by its lane
+                const float we = s + e < a.splits ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scale), s + e)) : 0.0f;
+                f.x = s + e < a.splits ? __builtin_fmaf(we, v[e].x, f.x) : f.x;
+                f.y = s + e < a.splits ? __builtin_fmaf(we, v[e].y, f.y) : f.y;
+            }
         }
-        static_cast<T *>(p.d_o)[(long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1] +
-                                c] = (T)(sum / ll);
+        out[c] = (T)f.x;
+        out[c + 1] = (T)f.y;
     }
 }
 
@@ -599,7 +670,9 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "WindowAttention: too many row blocks (%lld)", units);
     const long long span = std::min<long long>(p->max_kv, (long long)p->window + p->sinks + a.tile_rows / a.group);
     const long long want = units ? ((a.tile_rows > 16 ? 1LL : 2LL) * device_cus() + units - 1) / units : 1;
-    a.splits = (int)std::max(1LL, std::min(want, span / 256));
+    a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
+    a.wide = a.tile_rows == 16 && span <= 1024 && units <= device_cus() && p->head_dim <= 128;
+    if (a.wide) a.splits = 1;
     const long long parts = a.splits > 1 ? units * a.splits : 0;
     scratch = (size_t)parts * a.tile_rows * (p->head_dim + 2) * 4;
     return OSH_OK;
@@ -608,7 +681,7 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
 template <typename T>
 static osh_status win_join(const WinArgs &a, unsigned units, hipStream_t st) {
     if (a.splits > 1) {
-        OSH_LAUNCH(window_attn_join_kernel<T>, dim3(units * (a.tile_rows / 16)), dim3(256), 0, st, a);
+        OSH_LAUNCH(window_attn_join_kernel<T>, dim3(units * (a.tile_rows / 4)), dim3(256), 0, st, a);
         OSH_LAUNCH_CHECK("window_attn_join_kernel");
     }
     return OSH_OK;
@@ -638,8 +711,8 @@ static osh_status win_launch_t(const WinArgs &a, unsigned units, hipStream_t st)
         if (a.p.head_dim <= 128) return win_tile_launch<T, 16, 8, 4, 8>(a, units, st);
         return win_tile_launch<T, 32, 16, 8, 4>(a, units, st);
     }
-    if (a.p.head_dim <= 64) return win_launch<T, 64, 4>(a, units, st);
-    if (a.p.head_dim <= 128) return win_launch<T, 128, 4>(a, units, st);
+    if (a.p.head_dim <= 64) return a.wide ? win_launch<T, 64, 8>(a, units, st) : win_launch<T, 64, 4>(a, units, st);
+    if (a.p.head_dim <= 128) return a.wide ? win_launch<T, 128, 8>(a, units, st) : win_launch<T, 128, 4>(a, units, st);
     return win_launch<T, 256, 4>(a, units, st);
 }
 
@@ -667,6 +740,9 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
         if (two[i][0] < 0 || two[i][1] < 0) return fail(OSH_E_INVALID, "WindowAttention: negative stride");
     for (int i = 0; i < 3; i++)
         if (p->k_stride[i] < 0 || p->v_stride[i] < 0) return fail(OSH_E_INVALID, "WindowAttention: negative stride");
+    for (int i = 0; i < 3; i++)
+        if (std::max({p->k_stride[i], p->v_stride[i], p->k_new_stride[i % 2], p->v_new_stride[i % 2]}) > INT_MAX)
+            return fail(OSH_E_UNSUPPORTED, "WindowAttention: a stride above 2^31 - 1");
     if (p->table_stride < (p->batch > 1 ? p->table_width : 0))
         return fail(OSH_E_INVALID, "WindowAttention: table stride below its width");
     auto bytes2 = [&](const int64_t *st, int heads) { return (n * st[0] + (heads - 1) * st[1] + d) * 2; };
