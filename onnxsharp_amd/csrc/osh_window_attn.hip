@@ -389,10 +389,14 @@ __device__ __forceinline__ s16x4 read_transposed(const unsigned char *at) {
 // 32 of them in the output.  Chunk c of a key's row lies at slot c ^ swizzle: keys'
 // rows spread a 16-lane read over all banks, values' rows one of 4 rows x 64 bytes.
 //
+// Workgroups of 128 rows, two a CU: their phases drift apart, so that one's MFMAs run
+// under the other's exponentials (one of 256 rows: 323 us for 314 at 8192 tokens, 87
+// for 49 at pieces of prompts).
+//
 // The running maximum moves only when a row's scores pass it by 2^8: weights up to
 // 256 are as exact, and most tiles rescale nothing.
 template <typename T, int C, int KS, int OB, int NW>
-__global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
+__global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kernel(WinArgs a) {
     using H8 = typename Half8<T>::type;
     constexpr int BUF = 64 * C * 16, RPI = 64 / C, IT = 2 * C / NW;  // rows an instruction, instructions a wave
     static_assert(IT * NW == 2 * C, "loads are dealt evenly");
@@ -444,25 +448,47 @@ __global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
     const int w_first = max(sq.past + tok0 - p.window + 1, keys.lo) + base;  // below it only sinks
 
     // loads: instruction i (K for i < C) covers rows RPI (i % C) + lane / C; a wave has
-    // instructions wave + NW e, whose rows repeat for V after C
+    // instructions wave + NW e, whose rows repeat for V after C.  The C lanes of a row
+    // would all compute its address: lane e of each RW neighbours computes that of the
+    // e-th instruction's row and hands it to the others.  A tile of new tokens alone
+    // (all of a prompt's) has its rows at one stride.
     constexpr int RW = IT / 2 > 0 ? IT / 2 : 1;  // rows of a lane in a tile
     const int slot = lane % C;
     auto tile_row = [&](int e) { return (wave + NW * e) % C * RPI + lane / C; };
-    int page_id[RW];
+    const int my_tile_row = tile_row(lane % RW);
+    const int fresh0 = cdiv(max(sq.past + base, keys.sink_end), 64);  // first tile of new tokens alone
+    int page_id = 0;
     auto fetch_pages = [&](int t) {
-#pragma unroll
-        for (int e = 0; e < RW; e++) page_id[e] = win_page(p, sq, keys, b, t * 64 + tile_row(e), a.page_shift);
+        if (t < fresh0) page_id = win_page(p, sq, keys, b, t * 64 + my_tile_row, a.page_shift);
     };
     auto load_tile = [&](int t, int buf) {
+        const bool fresh = t >= fresh0 && t * 64 + 64 <= keys.count;
+        const T *fk = nullptr, *fv = nullptr;
+        WinRows<T> mine{nullptr, nullptr};
+        if (fresh) {
+            const long long n = sq.c0 + t * 64 - base - sq.past;
+            fk = static_cast<const T *>(p.d_k_new) + n * p.k_new_stride[0] + h * p.k_new_stride[1];
+            fv = static_cast<const T *>(p.d_v_new) + n * p.v_new_stride[0] + h * p.v_new_stride[1];
+        } else {
+            mine = win_rows<T>(p, sq, keys, t * 64 + my_tile_row, page_id, a.page_shift, h);
+        }
 #pragma unroll
         for (int e = 0; e < RW; e++) {
             const int r = tile_row(e);
-            const WinRows<T> at = win_rows<T>(p, sq, keys, t * 64 + r, page_id[e], a.page_shift, h);
-            const int kc = slot ^ win_k_swizzle<C>(r), vc = slot ^ win_v_swizzle<C>(r);
+            const int kc = 8 * (slot ^ win_k_swizzle<C>(r)), vc = 8 * (slot ^ win_v_swizzle<C>(r));
+            const T *kr, *vr;
+            if (fresh) {
+                kr = fk + (unsigned long long)(unsigned)r * (unsigned)p.k_new_stride[0];
+                vr = fv + (unsigned long long)(unsigned)r * (unsigned)p.v_new_stride[0];
+            } else {
+                const int from = lane - lane % RW + e;
+                kr = reinterpret_cast<const T *>(__shfl(reinterpret_cast<unsigned long long>(mine.k), from));
+                vr = reinterpret_cast<const T *>(__shfl(reinterpret_cast<unsigned long long>(mine.v), from));
+            }
             unsigned char *dst = lds + buf * 2 * BUF + (wave + NW * e) % C * 1024;
             const bool is_k = wave + NW * e < C, is_v = IT > 1 || !is_k;
-            if (is_k && 8 * kc < d) copy_to_lds(at.k + 8 * kc, dst);
-            if (is_v && 8 * vc < d) copy_to_lds(at.v + 8 * vc, dst + BUF);
+            if (is_k && kc < d) copy_to_lds(kr + kc, dst);
+            if (is_v && vc < d) copy_to_lds(vr + vc, dst + BUF);
         }
     };
 
@@ -492,19 +518,45 @@ __global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
         const int v0 = t * 64;
         if (v0 > w_hi || (v0 >= v_sink && v0 + 63 < w_first)) continue;  // the wave sees none
         const unsigned char *kt = lds + buf * 2 * BUF, *vt = kt + BUF;
-        f32x16 s[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[kb][r] = 0.0f;
+        // fragments are read ahead of the MFMAs that take them, the first values' before
+        // the softmax (3% of a prompt; heads above 128 have no registers for it)
+        constexpr bool AHEAD = KS <= 8;
+        constexpr int PF = !AHEAD ? 1 : KS < 4 ? KS : 4;
+        auto key_frag = [&](int kb, int i) {
             const int r = 32 * kb + ql32;
+            H8 k;
+            __builtin_memcpy(&k, kt + r * (C * 16) + (((2 * i + hl) ^ win_k_swizzle<C>(r)) << 4), 16);
+            return k;
+        };
+        // this lane reads row key + lane % 16 / 4, values 16 (lane / 16 % 2) + 4 (lane % 4)
+        auto value_frag = [&](int e, int i) {
+            const int key = 16 * e + 4 * hl + (lane >> 2 & 3), off = (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+            const int c = 4 * i + (off >> 4);
+            const unsigned char *row = vt + key * (C * 16) + (off & 15);
+            const s16x4 x0 = read_transposed(row + ((c ^ win_v_swizzle<C>(key)) << 4));
+            const s16x4 x1 = read_transposed(row + 8 * (C * 16) + ((c ^ win_v_swizzle<C>(key + 8)) << 4));
+            const s16x8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+            H8 v;
+            __builtin_memcpy(&v, &x, 16);
+            return v;
+        };
+        f32x16 s[2];
+        H8 kf[PF], vf[2][OB];
+#pragma unroll
+        for (int i = 0; i < PF; i++) kf[i] = key_frag(0, i);
+        if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int i = 0; i < KS; i++) {
-                H8 k;
-                __builtin_memcpy(&k, kt + r * (C * 16) + (((2 * i + hl) ^ win_k_swizzle<C>(r)) << 4), 16);
-                s[kb] = mma32(k, q[i], s[kb]);
+                const int n = kb * KS + i;
+                s[kb] = mma32(kf[n % PF], q[i], i == 0 ? f32x16{} : s[kb]);
+                if (n + PF < 2 * KS) kf[n % PF] = key_frag((n + PF) / KS, (n + PF) % KS);
             }
-        }
+#pragma unroll
+        for (int i = 0; i < OB; i++)
+            if (AHEAD) vf[0][i] = value_frag(0, i);
+        if (AHEAD) __builtin_amdgcn_sched_barrier(0);
         if (v0 + 63 > w_all || (v0 + 63 >= v_sink && v0 < w_lo)) {  // some row sees only some
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
@@ -542,19 +594,13 @@ __global__ __launch_bounds__(64 * NW) void window_attn_tile_kernel(WinArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            // this lane reads row key + lane % 16 / 4, values 16 (lane / 16 % 2) + 4 (lane % 4)
-            const int key = 16 * e + 4 * hl + (lane >> 2 & 3), off = (lane >> 4 & 1) * 32 + (lane & 3) * 8;
-            const unsigned char *r0p = vt + key * (C * 16), *r1p = r0p + 8 * (C * 16);
 #pragma unroll
             for (int i = 0; i < OB; i++) {
-                const int c = 4 * i + (off >> 4);
-                const s16x4 x0 = read_transposed(r0p + ((c ^ win_v_swizzle<C>(key)) << 4) + (off & 15));
-                const s16x4 x1 = read_transposed(r1p + ((c ^ win_v_swizzle<C>(key + 8)) << 4) + (off & 15));
-                const s16x8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                H8 vh;
-                __builtin_memcpy(&vh, &x, 16);
-                acc[i] = mma32(vh, w[e], acc[i]);
+                if (AHEAD && e < 3) vf[(e + 1) & 1][i] = value_frag(e + 1, i);
             }
+#pragma unroll
+            for (int i = 0; i < OB; i++) acc[i] = mma32(AHEAD ? vf[e & 1][i] : value_frag(e, i), w[e], acc[i]);
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
         }
     }
     l += __shfl_xor(l, 32);
@@ -664,7 +710,7 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
     a.scale_log2 = (p->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)p->head_dim) : p->scale) * 1.4426950408889634f;
     const int rows = p->max_q * a.group;
     const long long heads = (long long)p->batch * p->kv_heads;
-    a.tile_rows = rows >= 64 ? (p->head_dim > 128 ? 128 : 256) : 16;
+    a.tile_rows = rows >= 64 ? 128 : 16;
     a.tiles = cdiv(rows, a.tile_rows);
     const long long units = heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "WindowAttention: too many row blocks (%lld)", units);
@@ -705,10 +751,10 @@ static osh_status win_launch(const WinArgs &a, unsigned units, hipStream_t st) {
 template <typename T>
 static osh_status win_launch_t(const WinArgs &a, unsigned units, hipStream_t st) {
     if (a.tile_rows > 16) {
-        if (a.p.head_dim <= 32) return win_tile_launch<T, 4, 2, 1, 8>(a, units, st);
-        if (a.p.head_dim <= 64) return win_tile_launch<T, 8, 4, 2, 8>(a, units, st);
-        if (a.p.head_dim <= 96) return win_tile_launch<T, 16, 6, 3, 8>(a, units, st);
-        if (a.p.head_dim <= 128) return win_tile_launch<T, 16, 8, 4, 8>(a, units, st);
+        if (a.p.head_dim <= 32) return win_tile_launch<T, 4, 2, 1, 4>(a, units, st);
+        if (a.p.head_dim <= 64) return win_tile_launch<T, 8, 4, 2, 4>(a, units, st);
+        if (a.p.head_dim <= 96) return win_tile_launch<T, 16, 6, 3, 4>(a, units, st);
+        if (a.p.head_dim <= 128) return win_tile_launch<T, 16, 8, 4, 4>(a, units, st);
         return win_tile_launch<T, 32, 16, 8, 4>(a, units, st);
     }
     if (a.p.head_dim <= 64) return a.wide ? win_launch<T, 64, 8>(a, units, st) : win_launch<T, 64, 4>(a, units, st);
