@@ -16,6 +16,7 @@ sizes the backend does not take.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -27,6 +28,8 @@ _Q_TYPES = {"int8": (N.T_I8, torch.int8), "e4m3": (N.T_E4M3, torch.float8_e4m3fn
 _Q_CODES = {torch.int8: N.T_I8, torch.float8_e4m3fn: N.T_E4M3}
 _ACTIVATIONS = {None: N.ACT_NONE, "Relu": N.ACT_RELU, "Silu": N.ACT_SILU, "Gelu": N.ACT_GELU}
 _MAX_WINDOW = 2 ** 31 - 1
+# the fields of osh_window_attn in order (packing them costs a third of assigning them)
+_WINDOW_ATTN = struct.Struct("@12ifiq9P8q6qq")
 
 
 def _invalid(layer, message: str) -> N.OshError:
@@ -53,25 +56,28 @@ def _check_device(layer, *tensors) -> torch.device:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with its last dimension contiguous and no negative or shared rows."""
-    if t.stride(-1) == 1 or t.shape[-1] == 1:
-        if t.stride(0) >= t.shape[-1] or t.shape[0] == 1:
-            return t
+    if t.is_contiguous() or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
+        return t
     return t.contiguous()
 
 
 def _pitch(t: Optional[torch.Tensor]) -> int:
     if t is None:
         return 0
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else max(cols, 1)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
-    """A launch on the current stream of `device`."""
-    if device.index != torch.cuda.current_device():
+    """A launch on the current stream of `device`.
+
+    Asks torch for the raw stream: the Stream object that torch.cuda.current_stream builds
+    costs 4 us of the 12 that a small call takes on the host."""
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            N.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            N.check(getattr(N.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device.index)))
         return
-    N.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    N.check(getattr(N.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 class RmsNormQuantLayer:
@@ -244,13 +250,13 @@ class WindowAttentionLayer:
         cu_seqlens, kv_lens = cu_seqlens.contiguous(), kv_lens.contiguous()
         if out is None:
             out = torch.empty((tokens, q_heads, d), dtype=q.dtype, device=device)
-        p = N.WindowAttn(
+        p = N.WindowAttn.from_buffer_copy(_WINDOW_ATTN.pack(
             _ROW_TYPES[q.dtype], batch, q_heads, kv_heads, d,
             _MAX_WINDOW if self.window is None else min(self.window, _MAX_WINDOW), min(self.sinks, _MAX_WINDOW),
             max_q, max_kv, pages, page, width, 0.0 if self.scale is None else self.scale, 0, tokens,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), kp.data_ptr(), vp.data_ptr(), table.data_ptr(),
-            cu_seqlens.data_ptr(), kv_lens.data_ptr(), q.stride()[:2], k.stride()[:2], v.stride()[:2],
-            out.stride()[:2], kp.stride()[:3], vp.stride()[:3], table.stride(0))
+            cu_seqlens.data_ptr(), kv_lens.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+            *out.stride()[:2], *kp.stride()[:3], *vp.stride()[:3], table.stride(0)))
         size = C.c_size_t()
         N.call("osh_window_attention_scratch_bytes", C.byref(p), C.byref(size))
         scratch = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None

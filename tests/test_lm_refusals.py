@@ -200,6 +200,16 @@ def test_window_attn_struct_has_the_c_layout(tmp_path):
     assert got == [getattr(N.WindowAttn, f).offset for f in fields] + [C.sizeof(N.WindowAttn)]
 
 
+def test_window_attn_packing_is_the_struct():
+    from onnxsharp_amd.lm_layers import _WINDOW_ATTN
+    assert _WINDOW_ATTN.size == C.sizeof(N.WindowAttn)
+    values = list(range(1, 13)) + [0.5, 13] + list(range(14, 39))
+    p, got = N.WindowAttn.from_buffer_copy(_WINDOW_ATTN.pack(*values)), []
+    for f, t in N.WindowAttn._fields_:
+        got += list(getattr(p, f)) if issubclass(t, C.Array) else [getattr(p, f)]
+    assert got == values
+
+
 # ------------------------------------------------- keys and slots of a call
 
 PROGRAM = r"""
