@@ -32,6 +32,10 @@ struct QmmArgs {
 
 constexpr int KB = 128;  // bytes of a k-block
 
+template <int N> struct IntC {
+    static constexpr int value = N;
+};
+
 template <int Q> struct QAcc { using type = f32x4; };
 template <> struct QAcc<OSH_T_I8> { using type = i32x4; };
 
@@ -585,43 +589,83 @@ constexpr int qmm_lds() {
     return epi > 2 * (BM + BN) * KB ? epi : 2 * (BM + BN) * KB;
 }
 
-// Few rows: a workgroup takes 16 outputs of all rows (up to 16 MB), its waves
+// Few rows: a workgroup takes 16 NB outputs of all rows (up to 16 MB), its waves
 // every WAVES-th k-block; the weights go from memory to registers, each byte once.
-// The waves' sums meet in LDS, in the order of the waves.
-template <int Q, typename T, int MB, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void qmm_rows_kernel(QmmArgs p) {
+// What bounds it is how many bytes are in flight: the loads of U k-blocks of a wave
+// start together, without a condition around them (24 x 8192 x 4096 e4m3: 13.6 us a
+// block at a time, 9.9 so, of which the host takes 9).  The waves' sums meet in LDS, in the order of the waves.
+template <int Q, typename T, int MB, int NB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void qmm_rows_kernel(QmmArgs p) {
     using Acc = typename QAcc<Q>::type;
-    __shared__ Acc part[WAVES][MB][64];
+    constexpr int U = MB + NB > 4 ? 2 : 4;
+    __shared__ Acc part[WAVES][MB * NB][64];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int jl = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16;
-    const unsigned char *w = p.w + (long long)min(n0 + jl, p.n - 1) * p.ldw;
-    const unsigned char *a[MB];
-    Acc acc[MB];
+    const int n0 = blockIdx.x * (16 * NB);
+    const unsigned char *w[NB], *a[MB];
+    Acc acc[MB][NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) w[j] = p.w + (long long)min(n0 + 16 * j + jl, p.n - 1) * p.ldw;
 #pragma unroll
     for (int i = 0; i < MB; i++) {
         a[i] = p.a + (long long)min(16 * i + jl, p.m - 1) * p.lda;
-        acc[i] = Acc{0, 0, 0, 0};
-    }
-    const int nkb = cdiv(p.k, KB);
-    for (int kb = wave; kb < nkb; kb += WAVES) {
-        const int k0 = kb * KB + 16 * g;
-        Frag fw{load_chunk(w, k0, p.k), load_chunk(w, k0 + 64, p.k)};
 #pragma unroll
-        for (int i = 0; i < MB; i++) {
-            const Frag fa{load_chunk(a[i], k0, p.k), load_chunk(a[i], k0 + 64, p.k)};
-            acc[i] = mma<Q>(fw, fa, acc[i]);
+        for (int j = 0; j < NB; j++) acc[i][j] = Acc{0, 0, 0, 0};
+    }
+    const int whole = p.k / KB, nkb = cdiv(p.k, KB);
+    auto blocks = [&](int kb, auto count, auto cut) {
+        constexpr int N = decltype(count)::value;
+        Frag fw[N][NB], fa[N][MB];
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const int k0 = (kb + u * WAVES) * KB + 16 * g;
+            auto get = [&](const unsigned char *row) {
+                Frag f;
+                if constexpr (decltype(cut)::value) {
+                    f.lo = load_chunk(row, k0, p.k), f.hi = load_chunk(row, k0 + 64, p.k);
+                } else {
+                    __builtin_memcpy(&f.lo, row + k0, 16);
+                    __builtin_memcpy(&f.hi, row + k0 + 64, 16);
+                }
+                return f;
+            };
+#pragma unroll
+            for (int j = 0; j < NB; j++) fw[u][j] = get(w[j]);
+#pragma unroll
+            for (int i = 0; i < MB; i++) fa[u][i] = get(a[i]);
         }
+        __builtin_amdgcn_sched_barrier(0);  // every load in flight before the first MFMA waits
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int i = 0; i < MB; i++) acc[i][j] = mma<Q>(fw[u][j], fa[u][i], acc[i][j]);
+    };
+    int kb = wave;
+    for (; kb + (U - 1) * WAVES < whole; kb += U * WAVES) blocks(kb, IntC<U>{}, IntC<0>{});
+    if (U > 2 && kb + WAVES < whole) {
+        blocks(kb, IntC<2>{}, IntC<0>{});
+        kb += 2 * WAVES;
     }
+    if (kb < whole) {
+        blocks(kb, IntC<1>{}, IntC<0>{});
+        kb += WAVES;
+    }
+    if (kb < nkb) blocks(kb, IntC<1>{}, IntC<1>{});
 #pragma unroll
-    for (int i = 0; i < MB; i++) part[wave][i][lane] = acc[i];
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++) part[wave][i * NB + j][lane] = acc[i][j];
     __syncthreads();
-    for (int e = tid; e < MB * 256; e += 64 * WAVES) {
-        const int i = e >> 8, r = e & 3, g4 = e >> 2 & 3, row = 16 * i + (e >> 4 & 15), col = n0 + 4 * g4 + r;
-        auto sum = part[0][i][(e >> 4 & 15) + 16 * g4][r];
+    for (int e = tid; e < MB * NB * 256; e += 64 * WAVES) {
+        // neighbouring threads, neighbouring outputs
+        const int c = e % (16 * NB), row = e / (16 * NB), col = n0 + c;
+        const int f = row / 16 * NB + c / 16, from = row % 16 + 16 * (c / 4 % 4), r = c % 4;
+        auto sum = part[0][f][from][r];
 #pragma unroll
-        for (int v = 1; v < WAVES; v++) sum += part[v][i][(e >> 4 & 15) + 16 * g4][r];
+        for (int v = 1; v < WAVES; v++) sum += part[v][f][from][r];
         if (row < p.m && col < p.n)
             static_cast<T *>(p.y)[row * p.ldy + col] = finish<T>(p, (float)sum, row, col, p.sa[row]);
     }
@@ -660,10 +704,17 @@ static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
     const int e = 16 / sizeof(T);
     const bool fast = aligned && p.n % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.res) & 15) == 0 && p.ldy % e == 0 &&
                       p.ldr % e == 0 && std::max(p.ldy, p.ldr) < (1 << 20);
-    if (p.m <= 16)
-        OSH_LAUNCH((qmm_rows_kernel<Q, T, 1, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
-    else if (p.m <= 32)
-        OSH_LAUNCH((qmm_rows_kernel<Q, T, 2, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);
+    const bool pairs = p.n >= 32 * device_cus();  // enough workgroups of 32 outputs
+#define OSH_QMM_ROWS(MB)                                                                                             \
+    do {                                                                                                             \
+        if (pairs)                                                                                                   \
+            OSH_LAUNCH((qmm_rows_kernel<Q, T, MB, 2, 8>), dim3((unsigned)cdiv(p.n, 32)), dim3(512), 0, st, p);       \
+        else                                                                                                         \
+            OSH_LAUNCH((qmm_rows_kernel<Q, T, MB, 1, 8>), dim3((unsigned)cdiv(p.n, 16)), dim3(512), 0, st, p);       \
+    } while (0)
+    if (p.m <= 16) OSH_QMM_ROWS(1);
+    else if (p.m <= 32) OSH_QMM_ROWS(2);
+    else if (p.m <= 64) OSH_QMM_ROWS(4);
     else if (aligned && (long long)cdiv(p.m, 256) * cdiv(p.n, 256) >= device_cus())
         qmm_dma_launch<Q, T, 256, 256, 4>(p, fast, st);
     else if (aligned && (long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
@@ -673,6 +724,7 @@ static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
     else
         OSH_QMM_TILE(64, 64, 2, 2);
 #undef OSH_QMM_TILE
+#undef OSH_QMM_ROWS
     OSH_LAUNCH_CHECK("qmm kernel");
     return OSH_OK;
 }
