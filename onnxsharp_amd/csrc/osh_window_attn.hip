@@ -715,7 +715,10 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
     const long long units = heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "WindowAttention: too many row blocks (%lld)", units);
     const long long span = std::min<long long>(p->max_kv, (long long)p->window + p->sinks + a.tile_rows / a.group);
-    const long long want = units ? ((a.tile_rows > 16 ? 1LL : 2LL) * device_cus() + units - 1) / units : 1;
+    // Two workgroups a CU, all resident at once: three sequences of 65536 with window
+    // 32768 take 87 us as 504 workgroups, 104 as 528 (16 of them in a second round), 90
+    // as 1024; 64 ragged ones of 8192 191 us unsplit, 207 split in two.
+    const long long want = units ? std::max(1LL, 2LL * device_cus() / units) : 1;
     a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
     a.wide = a.tile_rows == 16 && span <= 1024 && units <= device_cus() && p->head_dim <= 128;
     if (a.wide) a.splits = 1;
