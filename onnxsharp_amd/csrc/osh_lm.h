@@ -6,6 +6,10 @@
 
 namespace osh {
 
+template <int N> struct IntC {
+    static constexpr int value = N;
+};
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));

@@ -32,10 +32,6 @@ struct QmmArgs {
 
 constexpr int KB = 128;  // bytes of a k-block
 
-template <int N> struct IntC {
-    static constexpr int value = N;
-};
-
 template <int Q> struct QAcc { using type = f32x4; };
 template <> struct QAcc<OSH_T_I8> { using type = i32x4; };
 

@@ -44,6 +44,22 @@ __device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// l plus the eight values of w, in FP32, two an instruction.
+__device__ __forceinline__ float add8(f16x8 w, float l) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(_Float16)1, (_Float16)1};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(f16x2{w[i], w[i + 1]}, one, l, false);
+    return l;
+}
+__device__ __forceinline__ float add8(bf16x8 w, float l) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{w[i], w[i + 1]}, one, l, false);
+    return l;
+}
+
 // What stands in for a row that is not read: zeros for a key past the last one and
 // for the value of a page outside the cache, NaN (0x7fff in both types) for its key.
 #define WIN_NAN4 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu
@@ -461,11 +477,42 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
     auto fetch_pages = [&](int t) {
         if (t < fresh0) page_id = win_page(p, sq, keys, b, t * 64 + my_tile_row, a.page_shift);
     };
+    // Heads of 65 to 128 keep the byte offsets of a lane's chunks in a tile of new tokens
+    // and sum their rounded weights two an instruction (634 -> 612 us at 8192 tokens
+    // without a window); above there are no registers for the offsets, below neither gains.
+    constexpr bool KEEP = C == 16;
+    unsigned k_off[RW], v_off[RW];
+    bool k_in[RW], v_in[RW];
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int e = 0; e < RW; e++) {
+            const int r = tile_row(e), kc = 8 * (slot ^ win_k_swizzle<C>(r)), vc = 8 * (slot ^ win_v_swizzle<C>(r));
+            k_in[e] = kc < d, v_in[e] = vc < d;
+            k_off[e] = 2 * (r * (unsigned)p.k_new_stride[0] + kc), v_off[e] = 2 * (r * (unsigned)p.v_new_stride[0] + vc);
+        }
+    }
+    const bool short_strides = max(p.k_new_stride[0], p.v_new_stride[0]) < (1 << 24);  // 32-bit offsets hold
     auto load_tile = [&](int t, int buf) {
+        unsigned char *dst = lds + buf * 2 * BUF;
         const bool fresh = t >= fresh0 && t * 64 + 64 <= keys.count;
+        if constexpr (KEEP) {
+            if (fresh && short_strides) {
+                const long long n = sq.c0 + t * 64 - base - sq.past;
+                const char *fk =
+                    static_cast<const char *>(p.d_k_new) + 2 * (n * p.k_new_stride[0] + h * p.k_new_stride[1]);
+                const char *fv =
+                    static_cast<const char *>(p.d_v_new) + 2 * (n * p.v_new_stride[0] + h * p.v_new_stride[1]);
+#pragma unroll
+                for (int e = 0; e < RW; e++) {
+                    if (k_in[e]) copy_to_lds(fk + k_off[e], dst + (wave + NW * e) % C * 1024);
+                    if (v_in[e]) copy_to_lds(fv + v_off[e], dst + BUF + (wave + NW * e) % C * 1024);
+                }
+                return;
+            }
+        }
         const T *fk = nullptr, *fv = nullptr;
         WinRows<T> mine{nullptr, nullptr};
-        if (fresh) {
+        if (!KEEP && fresh) {
             const long long n = sq.c0 + t * 64 - base - sq.past;
             fk = static_cast<const T *>(p.d_k_new) + n * p.k_new_stride[0] + h * p.k_new_stride[1];
             fv = static_cast<const T *>(p.d_v_new) + n * p.v_new_stride[0] + h * p.v_new_stride[1];
@@ -477,7 +524,7 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
             const int r = tile_row(e);
             const int kc = 8 * (slot ^ win_k_swizzle<C>(r)), vc = 8 * (slot ^ win_v_swizzle<C>(r));
             const T *kr, *vr;
-            if (fresh) {
+            if (!KEEP && fresh) {
                 kr = fk + (unsigned long long)(unsigned)r * (unsigned)p.k_new_stride[0];
                 vr = fv + (unsigned long long)(unsigned)r * (unsigned)p.v_new_stride[0];
             } else {
@@ -485,10 +532,9 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
                 kr = reinterpret_cast<const T *>(__shfl(reinterpret_cast<unsigned long long>(mine.k), from));
                 vr = reinterpret_cast<const T *>(__shfl(reinterpret_cast<unsigned long long>(mine.v), from));
             }
-            unsigned char *dst = lds + buf * 2 * BUF + (wave + NW * e) % C * 1024;
             const bool is_k = wave + NW * e < C, is_v = IT > 1 || !is_k;
-            if (is_k && kc < d) copy_to_lds(kr + kc, dst);
-            if (is_v && vc < d) copy_to_lds(vr + vc, dst + BUF);
+            if (is_k && kc < d) copy_to_lds(kr + kc, dst + (wave + NW * e) % C * 1024);
+            if (is_v && vc < d) copy_to_lds(vr + vc, dst + BUF + (wave + NW * e) % C * 1024);
         }
     };
 
@@ -588,9 +634,10 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], a.scale_log2, -ref));
-                l += f[i];
+                if (!KEEP) l += f[i];
             }
             w[e] = __builtin_convertvector(f, H8);
+            if (KEEP) l = add8(w[e], l);
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -710,7 +757,9 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
     a.scale_log2 = (p->scale == 0.0f ? 1.0f / __builtin_sqrtf((float)p->head_dim) : p->scale) * 1.4426950408889634f;
     const int rows = p->max_q * a.group;
     const long long heads = (long long)p->batch * p->kv_heads;
-    a.tile_rows = rows >= 64 ? 128 : 16;
+    // More than one block of 16 rows would read the keys again for each: 32 rows of 8
+    // sequences to 8192 take 35 us as two blocks and 31 in a tile of 128, 60 rows 56 and 32.
+    a.tile_rows = rows > 16 ? 128 : 16;
     a.tiles = cdiv(rows, a.tile_rows);
     const long long units = heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "WindowAttention: too many row blocks (%lld)", units);
