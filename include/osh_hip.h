@@ -624,7 +624,10 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
  * Query head h reads key head h / (q_heads / kv_heads).  Sums, softmax and its
  * statistics are FP32; the weights are rounded to dtype for the product with v.
  * Pages and slots that no query of the call sees are not read (stale entries of
- * d_table before the window may hold anything).  A new token's slot must belong
+ * d_table before the window may hold anything).  A key that is not finite reaches only
+ * the queries that see it; a value that is not finite and that some query of a
+ * sequence sees may make others of the same call NaN (their weight for it is 0, and 0
+ * times it is NaN).  A new token's slot must belong
  * to its sequence alone.
  * max_q and max_kv are the host's bounds of the lengths.  A sequence whose lengths
  * contradict each other, the bounds or the table, and a query that sees a page id

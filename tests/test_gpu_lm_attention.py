@@ -214,6 +214,26 @@ def test_attention_bad_page_is_nan_where_it_is_seen(cuda):
     assert _same(s["kp"], kp) and _same(s["vp"], vp)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,ql,kl", [(64, 3, 40), (128, 90, 130), (256, 60, 90)])
+def test_attention_nonfinite_keys_reach_only_who_sees_them(cuda, d, ql, kl, dtype):
+    # a new token's key and an old key are not finite: the queries that see neither keep
+    # the bits that finite ones give
+    s, window = _make(cuda, 4, 2, d, 16, [(ql, kl)], dtype, d + ql), 24
+    past = kl - ql
+    old, tk = past - 10, ql - 2  # the old one leaves the window of later tokens
+    good = _run(s, window, 2)
+    s["k"][tk, 0, 1] = float("nan")
+    s["kp"][int(s["table"][0, old // 16]), old % 16, 0, 7] = float("nan")
+    out = _run(s, window, 2)
+    pos = past + torch.arange(ql, device=cuda)
+    want = torch.zeros(out.shape, dtype=torch.bool, device=cuda)
+    for j in (past + tk, old):
+        want[(j <= pos) & (j > pos - window), :2] = True
+    assert torch.equal(out.isnan(), want)
+    assert torch.equal(out[~want], good[~want])
+
+
 def test_attention_lengths_that_contradict(cuda):
     s = _make(cuda, 4, 2, 64, 16, [(2, 50), (3, 60), (1, 20)], "bf16", 12)
     good = _run(s, 32, 2)

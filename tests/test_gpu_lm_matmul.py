@@ -81,6 +81,16 @@ def test_matmul_large(cuda, m, n, k, q):
     _check(QuantMatMulLayer("Gelu", torch.bfloat16).forward(**s), s, "Gelu", "bf16")
 
 
+@pytest.mark.parametrize("q", Q)
+@pytest.mark.parametrize("m,n,k,dtype", [(4100, 4104, 272, "bf16"), (4099, 4101, 384, "f16"), (4100, 4112, 256, "f32"),
+                                         (2100, 2056, 144, "f32"), (1500, 3333, 1040, "bf16")])
+def test_matmul_several_tiles_a_workgroup(cuda, m, n, k, dtype, q):
+    # more tiles than a launch holds at once, cut rows, columns and k-blocks
+    for act, bias, res in ((None, False, True), ("Gelu", True, False)):
+        s = _make(cuda, m, n, k, q, dtype, m + n, bias, res)
+        _check(QuantMatMulLayer(act, TYPES[dtype]).forward(**s), s, act, dtype)
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 70, 8192), (40, 200, 2000), (300, 500, 700)])
 def test_matmul_arbitrary_e4m3(cuda, m, n, k):
     s = _make(cuda, m, n, k, "e4m3", "f32", 2, bias=False, res=False)
