@@ -407,7 +407,10 @@ __device__ __forceinline__ s16x4 read_transposed(const unsigned char *at) {
 //
 // Workgroups of 128 rows, two a CU: their phases drift apart, so that one's MFMAs run
 // under the other's exponentials (one of 256 rows: 323 us for 314 at 8192 tokens, 87
-// for 49 at pieces of prompts).
+// for 49 at pieces of prompts).  What bounds it is that a SIMD's two waves still spend
+// 2.4 us on a tile each, of which MFMAs are 0.85 and vector instructions 0.9: 8192 tokens,
+// 32 heads of 128, window 2048: 294 us (820 TFLOP/s), without a window 606 (910).  The next
+// tile's scores interleaved with this one's exponentials in one wave were 5% slower.
 //
 // The running maximum moves only when a row's scores pass it by 2^8: weights up to
 // 256 are as exact, and most tiles rescale nothing.
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
         if (t < fresh0) page_id = win_page(p, sq, keys, b, t * 64 + my_tile_row, a.page_shift);
     };
     // Heads of 65 to 128 keep the byte offsets of a lane's chunks in a tile of new tokens
-    // and sum their rounded weights two an instruction (634 -> 612 us at 8192 tokens
+    // and sum their rounded weights two an instruction (634 -> 606 us at 8192 tokens
     // without a window); above there are no registers for the offsets, below neither gains.
     constexpr bool KEEP = C == 16;
     unsigned k_off[RW], v_off[RW];
@@ -609,7 +612,9 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int v = v0 + 32 * kb + 8 * (r >> 2) + 4 * hl + (r & 3);
-                    if (v > v_hi || (v < v_lo && v >= v_sink)) s[kb][r] = -__builtin_inff();
+                    // selects, not branches: a branch around an element of s moves all of it
+                    const bool hidden = (v > v_hi) | ((v < v_lo) & (v >= v_sink));
+                    s[kb][r] = hidden ? -__builtin_inff() : s[kb][r];
                 }
         }
         float top = s[0][0];
