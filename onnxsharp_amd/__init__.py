@@ -3,8 +3,9 @@
 Conv (+ fused Relu/SiLU), MatMul with a fused column bias and the int8
 DynamicQuantizeMatMul run as hand-written HIP kernels in libosh_hip.so behind
 the C ABI of include/osh_hip.h; `layers` mirrors the reference operators over
-that ABI.
+that ABI, and `lm_layers` adds the operators of a served language model's block
+(`decoder` runs them together).
 """
 from . import native  # noqa: F401
 
-__all__ = ["native", "layers", "synth"]
+__all__ = ["native", "layers", "lm_layers", "decoder", "synth"]
