@@ -343,13 +343,17 @@ __device__ __forceinline__ typename Vec8<T>::type buffer_load8(__amdgpu_buffer_r
     __builtin_memcpy(&v, w, sizeof(v));
     return v;
 }
+// No scalar offset: the compiler keeps a vector instruction that reuses a data register
+// apart from a 16-byte store only where the store has none.  Right behind stores that had
+// one, lanes 12 to 15 of each 16 stored the register's next content now and then (up to
+// 400 of 17 million values of a product).
 template <typename T>
-__device__ __forceinline__ void buffer_store8(typename Vec8<T>::type v, __amdgpu_buffer_rsrc_t r, int off, int soff) {
+__device__ __forceinline__ void buffer_store8(typename Vec8<T>::type v, __amdgpu_buffer_rsrc_t r, int off) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     u32x4 w[sizeof(T) / 2];
     __builtin_memcpy(w, &v, sizeof(v));
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_amdgcn_raw_buffer_store_b128(w[i], r, off + 16 * i, soff, 0);
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) __builtin_amdgcn_raw_buffer_store_b128(w[i], r, off + 16 * i, 0, 0);
 }
 
 // Large products: BM x BN tiles of 2 x WN waves, each (BM / 2) x (BN / WN), fed by
@@ -563,8 +567,8 @@ __global__ __launch_bounds__(128 * WN, 2) void qmm_dma_kernel(QmmArgs p) {
                 if (s + 1 < FN / 2 * UNITS) fetch((s + 1) / UNITS, (s + 1) % UNITS);
 #pragma unroll
                 for (int i = 0; i < UR; i++)
-                    buffer_store8<T>(out[i], ry, at(UR * u + i, jp, p.ldy),
-                                     (16 * (UR * u + i) * (int)p.ldy + 32 * jp) * (int)sizeof(T));
+                    buffer_store8<T>(out[i], ry, at(UR * u + i, jp, p.ldy) +
+                                                     (16 * (UR * u + i) * (int)p.ldy + 32 * jp) * (int)sizeof(T));
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (!more) break;
