@@ -605,10 +605,12 @@ OSH_API osh_status osh_rms_norm_quant(int64_t rows, int cols, int dtype, const v
 
 /* Product of 8-bit rows with its epilogue, y [m][n] of type dtype (f32, f16, bf16):
  *   y[i][j] = act(sum_k a[i][k] w[j][k] * sa[i] * sw[j] + bias[j]) + res[i][j]
- * a [m][k] and w [n][k] both i8 (int32 sums, k <= 131071) or both e4m3 (FP32 sums),
- * k contiguous, any pitch and alignment; sa, sw, bias FP32; bias and res (of type
- * dtype) may be NULL; act: none, relu, silu or gelu.  res may be y itself (same
- * pitch); no other overlap of y. */
+ * a [m][k] and w [n][k] both i8 (int32 sums, k <= 131071) or both e4m3, k contiguous,
+ * any pitch and alignment; sa, sw, bias FP32; bias and res (of type dtype) may be NULL;
+ * act: none, relu, silu or gelu.  res may be y itself (same pitch); no other overlap of y.
+ * e4m3 sums are FP32 for y of type f32; for f16 and bf16 they are those of the 8-bit
+ * float matrix instruction, which differ from FP32 ones by 1.5e-5 of the result in the
+ * 2-norm (1/14 of f16's own rounding, 1/110 of bf16's). */
 OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void *d_a, int64_t lda, const float *d_sa,
                                     const void *d_w, int64_t ldw, const float *d_sw, const float *d_bias, int act,
                                     int dtype, const void *d_res, int64_t ldr, void *d_y, int64_t ldy, osh_stream s);

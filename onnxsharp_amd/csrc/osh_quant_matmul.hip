@@ -11,6 +11,15 @@
 // v_mfma_i32_16x16x64_i8, e4m3 with one v_mfma_f32_16x16x128_f8f6f4.  Which k
 // a byte stands for is the same for both operands, so the sum does not care that
 // the hardware numbers a lane's bytes otherwise.
+//
+// The 8-bit float MFMA (the 32-deep one too) drops what its products have below about
+// 2^-16 of an instruction's largest: 1.5e-5 of the result in the 2-norm, for k from 64
+// to 16384 alike.  16-bit outputs round by 14 (f16) and 110 (bf16) times that and take
+// it.  FP32 outputs take their operands to f16, which holds every e4m3 value (all 256
+// codes checked, NaN among them), and v_mfma_f32_16x16x32_f16, whose sums are within
+// FP32's roundings: 2.6e-8 at k = 512, 1.2e-7 at 8192.  It has half the rate, and the
+// conversions run beside it: 8192 x 8192 x 4096 469 us (1.2 PFLOP/s; with the 8-bit
+// instruction 252), 1028 x 5120 x 1280 25.2 (17.6), 24 x 8192 x 4096 10.8 (10.5).
 #include <limits.h>
 
 #include <algorithm>
@@ -32,16 +41,51 @@ struct QmmArgs {
 
 constexpr int KB = 128;  // bytes of a k-block
 
+// What Q is in the kernels: an element type of the operands, or e4m3 multiplied in f16.
+constexpr int Q_E4M3_AS_F16 = OSH_T_F16;
+
 template <int Q> struct QAcc { using type = f32x4; };
 template <> struct QAcc<OSH_T_I8> { using type = i32x4; };
 
 struct Frag {
     i32x4 lo, hi;  // chunks g and g + 4 of a row's k-block
 };
+struct FragF16 {
+    f16x8 v[4];  // the same, 8 bytes of them each
+};
+
+// A fragment as the MFMAs take it.
+template <int Q> struct QOp { using type = Frag; };
+template <> struct QOp<Q_E4M3_AS_F16> { using type = FragF16; };
+template <int Q>
+__device__ __forceinline__ typename QOp<Q>::type operand(const Frag &f) {
+    if constexpr (Q == Q_E4M3_AS_F16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        FragF16 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int word = (i < 2 ? f.lo : f.hi)[(2 * i & 3) + e / 2];
+                const auto two = e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, true)
+                                       : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, false);
+                const f16x2 v = __builtin_bit_cast(f16x2, two);
+                o.v[i][2 * e] = v[0], o.v[i][2 * e + 1] = v[1];
+            }
+        return o;
+    } else {
+        return f;
+    }
+}
 
 template <int Q>
-__device__ __forceinline__ typename QAcc<Q>::type mma(const Frag &w, const Frag &a, typename QAcc<Q>::type c) {
-    if constexpr (Q == OSH_T_I8) {
+__device__ __forceinline__ typename QAcc<Q>::type mma(const typename QOp<Q>::type &w, const typename QOp<Q>::type &a,
+                                                      typename QAcc<Q>::type c) {
+    if constexpr (Q == Q_E4M3_AS_F16) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], a.v[i], c, 0, 0, 0);
+        return c;
+    } else if constexpr (Q == OSH_T_I8) {
         c = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.lo, a.lo, c, 0, 0, 0);
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(w.hi, a.hi, c, 0, 0, 0);
     } else {
@@ -51,11 +95,18 @@ __device__ __forceinline__ typename QAcc<Q>::type mma(const Frag &w, const Frag 
     }
 }
 
-// acc[i][j] += w a[i] over FM row fragments; int8 takes the low halves of all rows
+// acc[i][j] += w a[i] over FM row fragments; int8 and f16 take a part of all rows
 // first, so that no MFMA waits for the one before.
 template <int Q, int FM, int FN>
-__device__ __forceinline__ void mma_rows(const Frag &w, const Frag (&a)[FM], typename QAcc<Q>::type (&acc)[FM][FN], int j) {
-    if constexpr (Q == OSH_T_I8) {
+__device__ __forceinline__ void mma_rows(const typename QOp<Q>::type &w, const typename QOp<Q>::type (&a)[FM],
+                                         typename QAcc<Q>::type (&acc)[FM][FN], int j) {
+    if constexpr (Q == Q_E4M3_AS_F16) {
+#pragma unroll
+        for (int h = 0; h < 4; h++)
+#pragma unroll
+            for (int i = 0; i < FM; i++)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[h], a[i].v[h], acc[i][j], 0, 0, 0);
+    } else if constexpr (Q == OSH_T_I8) {
 #pragma unroll
         for (int i = 0; i < FM; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.lo, a[i].lo, acc[i][j], 0, 0, 0);
 #pragma unroll
@@ -285,7 +336,7 @@ __global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
         Frag f;
         f.lo = *reinterpret_cast<const i32x4 *>(row + ((g ^ (r >> 1 & 7)) << 4));
         f.hi = *reinterpret_cast<const i32x4 *>(row + (((g + 4) ^ (r >> 1 & 7)) << 4));
-        return f;
+        return operand<Q>(f);
     };
 
     Acc acc[FM][FN];
@@ -300,12 +351,12 @@ __global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
     __syncthreads();
     for (int kb = 0; kb < nkb; kb++) {
         if (kb + 1 < nkb) load(kb + 1);
-        Frag fa[FM];
+        typename QOp<Q>::type fa[FM];
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[i] = frag(kb & 1, wm * (BM / WM) + 16 * i + jl);
 #pragma unroll
         for (int j = 0; j < FN; j++) {
-            const Frag fw = frag(kb & 1, BM + wn * (BN / WN) + 16 * j + jl);
+            const auto fw = frag(kb & 1, BM + wn * (BN / WN) + 16 * j + jl);
 #pragma unroll
             for (int i = 0; i < FM; i++) acc[i][j] = mma<Q>(fw, fa[i], acc[i][j]);
         }
@@ -443,7 +494,7 @@ __global__ __launch_bounds__(128 * WN, 2) void qmm_dma_kernel(QmmArgs p) {
         Frag f;
         f.lo = *reinterpret_cast<const i32x4 *>(row + lo);
         f.hi = *reinterpret_cast<const i32x4 *>(row + hi);
-        return f;
+        return operand<Q>(f);
     };
     static_assert(FN % 2 == 0, "the last fragment is in fw[1]");
 
@@ -461,7 +512,7 @@ __global__ __launch_bounds__(128 * WN, 2) void qmm_dma_kernel(QmmArgs p) {
         for (int i = 0; i < FM; i++)
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = Acc{0, 0, 0, 0};
-        Frag fa[FM], fw[2];
+        typename QOp<Q>::type fa[FM], fw[2];
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[i] = frag(buf, rm + 16 * i);
         fw[0] = frag(buf, rn);
@@ -641,7 +692,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void qmm_rows_kernel(QmmArgs p) {
 #pragma unroll
             for (int j = 0; j < NB; j++)
 #pragma unroll
-                for (int i = 0; i < MB; i++) acc[i][j] = mma<Q>(fw[u][j], fa[u][i], acc[i][j]);
+                for (int i = 0; i < MB; i++) acc[i][j] = mma<Q>(operand<Q>(fw[u][j]), operand<Q>(fa[u][i]), acc[i][j]);
     };
     int kb = wave;
     for (; kb + (U - 1) * WAVES < whole; kb += U * WAVES) blocks(kb, IntC<U>{}, IntC<0>{});
@@ -704,6 +755,10 @@ static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
     const int e = 16 / sizeof(T);
     const bool fast = aligned && p.n % 8 == 0 && (((uintptr_t)p.y | (uintptr_t)p.res) & 15) == 0 && p.ldy % e == 0 &&
                       p.ldr % e == 0 && std::max(p.ldy, p.ldr) < (1 << 20);
+    // f16 fragments are twice as long: those of a 256 x 256 tile and its accumulators take
+    // more registers than a wave has
+    constexpr int LARGE = Q == Q_E4M3_AS_F16 ? 128 : 256;
+    const bool large = aligned && (long long)cdiv(p.m, LARGE) * cdiv(p.n, LARGE) >= device_cus();
     const bool pairs = p.n >= 32 * device_cus();  // enough workgroups of 32 outputs
 #define OSH_QMM_ROWS(MB)                                                                                             \
     do {                                                                                                             \
@@ -715,8 +770,8 @@ static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
     if (p.m <= 16) OSH_QMM_ROWS(1);
     else if (p.m <= 32) OSH_QMM_ROWS(2);
     else if (p.m <= 64) OSH_QMM_ROWS(4);
-    else if (aligned && (long long)cdiv(p.m, 256) * cdiv(p.n, 256) >= device_cus())
-        qmm_dma_launch<Q, T, 256, 256, 4>(p, fast, st);
+    else if (large)
+        qmm_dma_launch<Q, T, LARGE, LARGE, LARGE / 64>(p, fast, st);
     else if (aligned && (long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
         qmm_dma_launch<Q, T, 128, 128, 2>(p, fast, st);
     else if ((long long)cdiv(p.m, 128) * cdiv(p.n, 128) >= device_cus())
@@ -731,7 +786,7 @@ static osh_status qmm_launch(const QmmArgs &p, hipStream_t st) {
 
 template <int Q>
 static osh_status qmm_launch_t(const QmmArgs &p, int dtype, hipStream_t st) {
-    if (dtype == OSH_T_F32) return qmm_launch<Q, float>(p, st);
+    if (dtype == OSH_T_F32) return qmm_launch<Q == OSH_T_E4M3 ? Q_E4M3_AS_F16 : Q, float>(p, st);
     if (dtype == OSH_T_F16) return qmm_launch<Q, _Float16>(p, st);
     return qmm_launch<Q, __bf16>(p, st);
 }

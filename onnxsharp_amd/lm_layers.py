@@ -133,7 +133,9 @@ class QuantMatMulLayer:
     """y = act((a * a_scale) @ (w * w_scale).T + bias) + residual of 8-bit a and w.
 
     activation None, "Relu", "Silu" or "Gelu" (with erf); out_dtype float32, float16 or
-    bfloat16."""
+    bfloat16.  float8_e4m3fn sums are FP32 for float32 outputs (at up to 2.3 times the
+    time of a 16-bit one), those of the 8-bit matrix instruction, 1.5e-5 of the result
+    off, for the others."""
 
     def __init__(self, activation: Optional[str] = None, out_dtype: torch.dtype = torch.bfloat16,
                  name: str = "quant_matmul"):
