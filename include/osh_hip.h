@@ -634,6 +634,8 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
  * max_q and max_kv are the host's bounds of the lengths.  A sequence whose lengths
  * contradict each other, the bounds or the table, and a query that sees a page id
  * outside [0, pages), get NaN; nothing out of range is read or written.
+ * o, the scratch and the pages share no memory with themselves, each other or an input
+ * (views that interleave without a common byte are fine); what shares is refused.
  * Strides are in elements, the head_dim values of a head contiguous, any alignment
  * of whole elements.  head_dim % 8 == 0 and <= 256, dtype f16 or bf16. */
 typedef struct osh_window_attn {

@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "osh_lm.h"
+#include "osh_overlap.h"
 #include "osh_window_addr.h"
 
 using namespace osh;
@@ -841,7 +842,7 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
     if (!p->d_q || !p->d_k_new || !p->d_v_new || !p->d_o || !p->d_k_pages || !p->d_v_pages || !p->d_table ||
         !p->d_cu || !p->d_kl || (scratch && !d_scratch))
         return fail(OSH_E_INVALID, "WindowAttention: NULL pointer");
-    const long long d = p->head_dim, n = p->tokens - 1;
+    const long long d = p->head_dim;
     const int64_t *two[4] = {p->q_stride, p->o_stride, p->k_new_stride, p->v_new_stride};
     for (int i = 0; i < 4; i++)
         if (two[i][0] < 0 || two[i][1] < 0) return fail(OSH_E_INVALID, "WindowAttention: negative stride");
@@ -852,12 +853,30 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
             return fail(OSH_E_UNSUPPORTED, "WindowAttention: a stride above 2^31 - 1");
     if (p->table_stride < (p->batch > 1 ? p->table_width : 0))
         return fail(OSH_E_INVALID, "WindowAttention: table stride below its width");
-    auto bytes2 = [&](const int64_t *st, int heads) { return (n * st[0] + (heads - 1) * st[1] + d) * 2; };
-    const long long bo = bytes2(p->o_stride, p->q_heads);
-    if (ranges_overlap(p->d_o, bo, p->d_q, bytes2(p->q_stride, p->q_heads)) ||
-        ranges_overlap(p->d_o, bo, p->d_k_new, bytes2(p->k_new_stride, p->kv_heads)) ||
-        ranges_overlap(p->d_o, bo, p->d_v_new, bytes2(p->v_new_stride, p->kv_heads)))
-        return fail(OSH_E_INVALID, "WindowAttention: o overlaps an operand");
+    auto rows = [&](const void *t, const int64_t *st, int heads) {
+        return Strided(t, d * 2).by(p->tokens, (Strided::wide)st[0] * 2).by(heads, (Strided::wide)st[1] * 2);
+    };
+    auto cache = [&](const void *t, const int64_t *st) {
+        return Strided(t, d * 2).by(p->pages, st[0] * 2).by(p->page, st[1] * 2).by(p->kv_heads, st[2] * 2);
+    };
+    const Strided o = rows(p->d_o, p->o_stride, p->q_heads), kc = cache(p->d_k_pages, p->k_stride),
+                  vc = cache(p->d_v_pages, p->v_stride), room(d_scratch, scratch);
+    const Strided in[6] = {rows(p->d_q, p->q_stride, p->q_heads), rows(p->d_k_new, p->k_new_stride, p->kv_heads),
+                           rows(p->d_v_new, p->v_new_stride, p->kv_heads),
+                           strided_rows(p->d_table, p->batch, p->table_stride * 4, p->table_width * 4LL),
+                           Strided(p->d_cu, (p->batch + 1LL) * 4), Strided(p->d_kl, p->batch * 4LL)};
+    if (shares_itself(o)) return fail(OSH_E_INVALID, "WindowAttention: rows of o share memory");
+    if (shares_itself(kc) || shares_itself(vc) || share_bytes(kc, vc))
+        return fail(OSH_E_INVALID, "WindowAttention: slots of the cache share memory");
+    if (share_bytes(o, kc) || share_bytes(o, vc)) return fail(OSH_E_INVALID, "WindowAttention: o overlaps the cache");
+    for (const Strided &t : in) {
+        if (share_bytes(o, t)) return fail(OSH_E_INVALID, "WindowAttention: o overlaps an operand");
+        if (share_bytes(kc, t) || share_bytes(vc, t))
+            return fail(OSH_E_INVALID, "WindowAttention: the cache overlaps an operand");
+        if (share_bytes(room, t)) return fail(OSH_E_INVALID, "WindowAttention: the scratch overlaps an operand");
+    }
+    if (share_bytes(room, o) || share_bytes(room, kc) || share_bytes(room, vc))
+        return fail(OSH_E_INVALID, "WindowAttention: the scratch overlaps an operand");
     const long long units = (long long)p->batch * p->kv_heads * a.tiles;
     a.part_ml = static_cast<float *>(d_scratch);
     a.part_o = a.part_ml + units * a.splits * a.tile_rows * 2;

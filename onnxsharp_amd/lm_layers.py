@@ -186,7 +186,7 @@ class PagedKvCache:
     """Pages of keys and values, and which pages each sequence holds.
 
     k_pages and v_pages are [pages, page, kv_heads, head_dim] of float16 or bfloat16 (any
-    strides with contiguous head values); table [batch, width] int32: position p of
+    strides with contiguous head values, no two slots in the same memory); table [batch, width] int32: position p of
     sequence b lies in slot p % page of page table[b, p // page].  Entries that no query
     sees (before the window, past the length) may hold anything."""
 

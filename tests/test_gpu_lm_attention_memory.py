@@ -1,0 +1,45 @@
+"""GPU: WindowAttentionLayer where its operands lie in one another's memory: views that
+interleave give what separate tensors give, views that share bytes are refused."""
+import pytest
+import torch
+
+from onnxsharp_amd import native as N
+from onnxsharp_amd.lm_layers import PagedKvCache, WindowAttentionLayer
+from test_gpu_lm_attention import _make, _run, _same
+
+pytestmark = pytest.mark.gpu
+LENS = [(20, 90), (1, 40)]
+
+
+def test_attention_into_the_buffer_that_holds_q(cuda):
+    s = _make(cuda, 8, 2, 64, 16, LENS, "bf16", 21)
+    want = _run(s, 32, 4)
+    wide = torch.zeros(21, 16, 64, dtype=torch.bfloat16, device=cuda)
+    wide[:, :8] = s["q"]
+    s["q"] = wide[:, :8]
+    out = _run(s, 32, 4, out=wide[:, 8:])
+    assert _same(out, want)
+    heads = torch.zeros(21, 8, 2, 64, dtype=torch.bfloat16, device=cuda)  # every other head
+    heads[:, :, 1] = s["q"]
+    s["q"] = heads[:, :, 1]
+    assert _same(_run(s, 32, 4, out=heads[:, :, 0]), want)
+
+
+def test_attention_refuses_shared_views(cuda):
+    s = _make(cuda, 8, 2, 64, 16, LENS, "bf16", 22)
+    layer = WindowAttentionLayer(32, 4)
+
+    def run(k_pages, v_pages, **kw):
+        layer.forward(s["q"], s["k"], s["v"], PagedKvCache(k_pages, v_pages, s["table"]), s["cu"], s["kl"], 20, 90, **kw)
+
+    kp, vp = s["kp"], s["vp"]
+    with pytest.raises(N.OshError, match="share memory"):
+        run(kp, kp)
+    with pytest.raises(N.OshError, match="share memory"):
+        run(kp, vp[:1].expand(vp.shape))
+    with pytest.raises(N.OshError, match="share memory"):
+        run(torch.cat([kp, vp])[:len(kp)], torch.empty_like(vp), out=s["q"][:1].clone().expand(s["q"].shape))
+    with pytest.raises(N.OshError, match="overlaps the cache"):
+        run(kp, vp, out=vp.view(-1, 8, 64)[:21])
+    with pytest.raises(N.OshError, match="overlaps an operand"):
+        run(kp, vp, out=s["q"])
