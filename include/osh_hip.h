@@ -631,9 +631,13 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
  * sequence sees may make others of the same call NaN (their weight for it is 0, and 0
  * times it is NaN).  A new token's slot must belong
  * to its sequence alone.
- * max_q and max_kv are the host's bounds of the lengths.  A sequence whose lengths
- * contradict each other, the bounds or the table, and a query that sees a page id
- * outside [0, pages), get NaN; nothing out of range is read or written.
+ * max_q and max_kv are the host's bounds of the lengths.  All rows of a sequence whose
+ * lengths contradict each other, the bounds or the table get NaN, and so does a query that
+ * sees a cached key whose page id lies outside [0, pages).  A new token whose own page id
+ * does is computed like any other (its key and value come from k_new and v_new), but not
+ * kept.  Nothing out of range is read or written.  Rows that no sequence holds are not
+ * written; d_cu ascends, so that none is held twice.  With batch, max_q or tokens 0 the call
+ * does nothing.
  * o, the scratch and the pages share no memory with themselves, each other or an input
  * (views that interleave without a common byte are fine); what shares is refused.
  * Strides are in elements, the head_dim values of a head contiguous, any alignment

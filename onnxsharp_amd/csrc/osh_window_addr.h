@@ -19,10 +19,10 @@ OSH_HD int win_min(int a, int b) { return a < b ? a : b; }
 OSH_HD int win_max(int a, int b) { return a > b ? a : b; }
 
 // A sequence's rows and lengths.  ok is false where they contradict each other,
-// the host's bounds or the table; c0 and ql stay within the tensors even then, so
-// that its rows can be filled with NaN.
+// the host's bounds or the table; c0, ql and held, all of its rows, stay within the
+// tensors even then, so that they can be filled with NaN.
 struct WinSeq {
-    int c0, ql, kl, past;
+    int c0, ql, kl, past, held;
     bool ok;
 };
 OSH_HD WinSeq win_seq(const osh_window_attn &p, int b) {
@@ -35,6 +35,7 @@ OSH_HD WinSeq win_seq(const osh_window_attn &p, int b) {
     c0 = c0 < 0 ? 0 : c0 > n ? n : c0;
     c1 = c1 < c0 ? c0 : c1 > n ? n : c1;
     s.c0 = (int)c0;
+    s.held = (int)(c1 - c0);
     s.ql = (int)(c1 - c0 < p.max_q ? c1 - c0 : p.max_q);
     s.past = s.kl - s.ql;
     return s;

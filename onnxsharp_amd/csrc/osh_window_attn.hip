@@ -70,16 +70,16 @@ __device__ const unsigned win_nan_row[128] = {WIN_NAN32, WIN_NAN32, WIN_NAN32, W
 #undef WIN_NAN4
 #undef WIN_NAN32
 
-// Rows r0 .. r0 + n of a sequence whose lengths contradict each other.
+// All rows of a sequence whose lengths contradict each other or the bounds (it may hold
+// more than the call's row blocks cover), at one key head's query heads.
 template <typename T>
-__device__ __forceinline__ void win_fill_nan(const osh_window_attn &p, const WinSeq &sq, int h, int G, int r0, int n,
-                                             int tid, int threads) {
+__device__ __forceinline__ void win_fill_nan(const osh_window_attn &p, const WinSeq &sq, int h, int G, int tid,
+                                             int threads) {
     const int d = p.head_dim;
-    for (int e = tid; e < n * d; e += threads) {
-        const int r = r0 + e / d;
-        if (r < sq.ql * G)
-            static_cast<T *>(p.d_o)[(long long)(sq.c0 + r / G) * p.o_stride[0] + (h * G + r % G) * p.o_stride[1] + e % d] =
-                (T)__builtin_nanf("");
+    for (long long e = tid; e < (long long)sq.held * G * d; e += threads) {
+        const long long r = e / d;
+        static_cast<T *>(p.d_o)[(sq.c0 + r / G) * p.o_stride[0] + (h * G + r % G) * p.o_stride[1] + e % d] =
+            (T)__builtin_nanf("");
     }
 }
 
@@ -191,13 +191,13 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void window_attn_rows
     const int h = id % p.kv_heads, b = id / p.kv_heads;
     const WinSeq sq = win_seq(p, b);
     const int rows = sq.ql * G, r0 = tile * 16;
+    if (!sq.ok) {
+        if (tile == 0 && split == 0) win_fill_nan<T>(p, sq, h, G, tid, 64 * WAVES);
+        return;
+    }
     if (r0 >= rows) return;
     T *o = static_cast<T *>(p.d_o);
     const int my_row = r0 + jl, my_tok = min(my_row, rows - 1) / G, my_head = h * G + min(my_row, rows - 1) % G;
-    if (!sq.ok) {
-        if (split == 0) win_fill_nan<T>(p, sq, h, G, r0, 16, tid, 64 * WAVES);
-        return;
-    }
 
     // queries: lane (jl, g) holds values 32 s + 8 g .. + 7 of row jl
     H8 q[KS];
@@ -436,13 +436,13 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
     const int h = id % p.kv_heads, b = id / p.kv_heads;
     const WinSeq sq = win_seq(p, b);
     const int rows = sq.ql * G, r0 = tile * 32 * NW;
+    if (!sq.ok) {
+        if (tile == 0 && split == 0) win_fill_nan<T>(p, sq, h, G, tid, 64 * NW);
+        return;
+    }
     if (r0 >= rows) return;
     T *o = static_cast<T *>(p.d_o);
     const int row = min(r0 + 32 * wave + ql32, rows - 1), tok = row / G, head = h * G + row % G;
-    if (!sq.ok) {
-        if (split == 0) win_fill_nan<T>(p, sq, h, G, r0, 32 * NW, tid, 64 * NW);
-        return;
-    }
     if (split == 0) win_append<T>(p, sq, b, h, G, r0, 32 * NW, tid, 64 * NW);
 
     H8 q[KS];

@@ -27,7 +27,7 @@ _ROW_TYPES = {torch.float32: N.T_F32, torch.float16: N.T_F16, torch.bfloat16: N.
 _Q_TYPES = {"int8": (N.T_I8, torch.int8), "e4m3": (N.T_E4M3, torch.float8_e4m3fn)}
 _Q_CODES = {torch.int8: N.T_I8, torch.float8_e4m3fn: N.T_E4M3}
 _ACTIVATIONS = {None: N.ACT_NONE, "Relu": N.ACT_RELU, "Silu": N.ACT_SILU, "Gelu": N.ACT_GELU}
-_MAX_WINDOW = 2 ** 31 - 1
+_MAX_INT = 2 ** 31 - 1
 # the fields of osh_window_attn in order (packing them costs a third of assigning them)
 _WINDOW_ATTN = struct.Struct("@12ifiq9P8q6qq")
 
@@ -228,9 +228,10 @@ class WindowAttentionLayer:
         """o [tokens, q_heads, head_dim] for the new tokens' q, and k and v
         [tokens, kv_heads, head_dim], which go to their pages.
 
-        cu_seqlens [batch + 1] int32: sequence b's tokens are rows cu_seqlens[b] to
-        cu_seqlens[b + 1]; kv_lens [batch] int32: its length with them; max_q and max_kv:
-        upper bounds of new and whole lengths, known to the host."""
+        cu_seqlens [batch + 1] int32, ascending: sequence b's tokens are rows cu_seqlens[b]
+        to cu_seqlens[b + 1]; kv_lens [batch] int32: its length with them; max_q and max_kv:
+        upper bounds of new and whole lengths, known to the host.  A sequence whose lengths
+        contradict them gets NaN; rows of no sequence are not written."""
         kp, vp, table = cache.k_pages, cache.v_pages, cache.table
         pages, page, kv_heads, d = kp.shape
         batch, width = table.shape
@@ -243,6 +244,10 @@ class WindowAttentionLayer:
         _check_tensor(self, "v", v, kp.dtype, (tokens, kv_heads, d))
         _check_tensor(self, "cu_seqlens", cu_seqlens, torch.int32, (batch + 1,))
         _check_tensor(self, "kv_lens", kv_lens, torch.int32, (batch,))
+        if tokens and (batch == 0 or max_q < 1):
+            raise _invalid(self, f"{tokens} tokens, but {batch} sequences of at most {max_q} new ones")
+        if not 0 <= max_q <= max_kv <= _MAX_INT:
+            raise _invalid(self, f"max_q {max_q} and max_kv {max_kv}")
         if out is not None:
             _check_tensor(self, "out", out, kp.dtype, q.shape)
             if out.stride(2) != 1:
@@ -254,7 +259,7 @@ class WindowAttentionLayer:
             out = torch.empty((tokens, q_heads, d), dtype=q.dtype, device=device)
         p = N.WindowAttn.from_buffer_copy(_WINDOW_ATTN.pack(
             _ROW_TYPES[q.dtype], batch, q_heads, kv_heads, d,
-            _MAX_WINDOW if self.window is None else min(self.window, _MAX_WINDOW), min(self.sinks, _MAX_WINDOW),
+            _MAX_INT if self.window is None else min(self.window, _MAX_INT), min(self.sinks, _MAX_INT),
             max_q, max_kv, pages, page, width, 0.0 if self.scale is None else self.scale, 0, tokens,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), kp.data_ptr(), vp.data_ptr(), table.data_ptr(),
             cu_seqlens.data_ptr(), kv_lens.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],

@@ -43,3 +43,34 @@ def test_attention_refuses_shared_views(cuda):
         run(kp, vp, out=vp.view(-1, 8, 64)[:21])
     with pytest.raises(N.OshError, match="overlaps an operand"):
         run(kp, vp, out=s["q"])
+
+
+@pytest.mark.parametrize("max_q", [1, 3, 40, 200])
+def test_attention_more_new_tokens_than_the_bound(cuda, max_q):
+    # every row of a sequence above max_q is NaN, the others keep their bits, and nothing of
+    # it goes to the pages
+    lens = [(max_q, 300), (max_q + 157, 400), (1, 20)]
+    s = _make(cuda, 4, 2, 64, 16, lens, "bf16", 23)
+    kp, vp = s["kp"].clone(), s["vp"].clone()
+
+    def run():
+        cache = PagedKvCache(s["kp"], s["vp"], s["table"])
+        return WindowAttentionLayer(32, 2).forward(s["q"], s["k"], s["v"], cache, s["cu"], s["kl"], max_q, 400,
+                                                   out=torch.full_like(s["q"], 7.0))
+
+    out = run()
+    first, last = lens[0][0], lens[0][0] + lens[1][0]
+    assert out[first:last].isnan().all() and out[:first].isfinite().all() and out[last:].isfinite().all()
+    for i in range(lens[1][1]):
+        slot = int(s["table"][1, i // 16]), i % 16
+        assert _same(s["kp"][slot], kp[slot]) and _same(s["vp"][slot], vp[slot])
+    s["kl"][1] = -1  # refused for another reason
+    assert _same(run().nan_to_num(nan=5.0), out.nan_to_num(nan=5.0))
+
+
+def test_attention_rows_of_no_sequence_stay(cuda):
+    s = _make(cuda, 4, 2, 64, 16, [(3, 50), (2, 40), (4, 30)], "f16", 24)
+    s["cu"].copy_(torch.tensor([2, 5, 7, 7]))
+    s["kl"][2] = 26
+    out = _run(s, 32, 2, out=torch.full_like(s["q"], 7.0))
+    assert (out[:2] == 7.0).all() and (out[7:] == 7.0).all() and (out[2:7] != 7.0).any(-1).all()
