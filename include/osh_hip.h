@@ -595,8 +595,11 @@ OSH_API osh_status osh_attention_f32(int heads, int key_dim, int head_dim, int n
  *   h = round(x + res), or x when d_res is NULL (d_h is then not touched);
  *   y = h / sqrt(mean(h^2) + eps) * gamma;
  *   scale[row] = max|y| / top (top = 127, 448);  q = round(y / scale), half to even.
- * h may be x or res themselves; no other overlap of an output.  A row of zeros
- * gets scale 0 and zeros; a NaN or an infinity in a row makes its scale NaN.
+ * h may be x or res themselves; no other overlap of an output.  Rows of any finite size
+ * (their squares may leave FP32's range) and any eps >= 0.  A scale below FP32's normal
+ * numbers is rounded to its subnormal ones, q is y over the scale that is stored, within
+ * [-top, top], and a scale of 0, as of a row of zeros, has zeros.  A NaN or an infinity in a
+ * row makes its scale NaN.
  * cols <= 32768; any alignment of whole elements. */
 OSH_API osh_status osh_rms_norm_quant(int64_t rows, int cols, int dtype, const void *d_x, int64_t ldx,
                                       const void *d_res, int64_t ldr, const void *d_gamma, float eps, void *d_h,

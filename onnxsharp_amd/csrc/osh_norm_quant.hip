@@ -29,13 +29,34 @@ struct NormArgs {
     int q_int8;
 };
 
-// |v| as an integer of the same order, with NaN above infinity: a NaN or an
-// infinity in a row (whose sum, or inf * 0, is NaN) or in gamma reaches the row's
-// scale, and with it every value that the row stands for.
+// |v| as an integer of the same order, with NaN above infinity: a NaN in gamma, and a NaN or
+// an infinity in a row (whose mean is then NaN), reaches the row's scale, and with it every
+// value that the row stands for.
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// 1 / scale; 0 where it would not be finite (a row of zeros gets scale 0 and zeros).
-__device__ __forceinline__ float row_back(float amax, float top) { return amax > 0x1p-117f ? top / amax : 0.0f; }
+// Whether FP32 squares of a row went wrong, mean being their sum / cols: it left FP32's
+// range, or is so small that what they lost below it counts.
+__device__ __forceinline__ bool squares_lost(float mean, float eps) {
+    return !(mean < __builtin_inff()) || !(mean + eps >= 0x1p-100f);
+}
+// Such a row is taken times the power of two that brings the larger of its largest |h| and
+// sqrt(eps) to [1, 2), as far as floats go: y is that of the row times it, with eps times
+// its square.
+__device__ __forceinline__ float row_shift(float hmax, float eps) {
+    const int e = __float_as_uint(__builtin_fmaxf(hmax, __builtin_sqrtf(eps))) >> 23;
+    return __uint_as_float((unsigned)min(max(254 - e, 1), 253) << 23);
+}
+// 1 / sqrt; 0 for a row of zeros without eps.
+__device__ __forceinline__ float row_inv(float mean, float eps) {
+    return mean + eps == 0.0f ? 0.0f : 1.0f / __builtin_sqrtf(mean + eps);
+}
+
+// Where the scale would lie below FP32's normal numbers, y does so too and has few bits: it
+// is then computed 2^60 times as large.  NaN counts as small, and keeps its NaN.
+__device__ __forceinline__ bool row_small(float amax) { return !(amax > 0x1p-117f); }
+constexpr float ROW_UP = 0x1p60f, ROW_DOWN = 0x1p-60f;
+// A small row's 1 / scale for such y, from the scale that is stored; 0 for a scale of 0.
+__device__ __forceinline__ float row_back_up(float scale) { return scale > 0.0f ? 1.0f / (scale * ROW_UP) : 0.0f; }
 
 // WPR waves share a row; a lane holds NV vectors of 8 neighbouring columns,
 // vector v of it at column 8 * (thread + 64 WPR v).  The vector that would cross
@@ -62,7 +83,6 @@ __global__ __launch_bounds__(WPR > 4 ? WPR * 64 : 256) void norm_quant_kernel(No
         T *h = static_cast<T *>(a.h) + row * a.ldh;
         f32x8 f[NV], g[NV];
         int col[NV], skip[NV];
-        float sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int c = 8 * (t + TPR * v);
@@ -80,51 +100,78 @@ __global__ __launch_bounds__(WPR > 4 ? WPR * 64 : 256) void norm_quant_kernel(No
                 }
             }
         }
+        // taken in turn: the barrier of each frees the other's LDS
+        auto mean_square = [&] {
+            float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; v++)
+            for (int v = 0; v < NV; v++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) sum = __builtin_fmaf(i >= skip[v] ? f[v][i] : 0.0f, f[v][i], sum);
+                for (int i = 0; i < 8; i++) sum = __builtin_fmaf(i >= skip[v] ? f[v][i] : 0.0f, f[v][i], sum);
 #pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-        if constexpr (WPR > 1) {
-            if ((t & 63) == 0) s_sum[slot][wave] = sum;
-            __syncthreads();
-            sum = 0.0f;
+            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+            if constexpr (WPR > 1) {
+                if ((t & 63) == 0) s_sum[slot][wave] = sum;
+                __syncthreads();
+                sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WPR; w++) sum += s_sum[slot][w];
+                for (int w = 0; w < WPR; w++) sum += s_sum[slot][w];
+            }
+            return sum / (float)cols;
+        };
+        auto largest = [&](auto value) {
+            unsigned top_bits = 0;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const f32x8 y = value(v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top_bits = max(top_bits, abs_bits(y[i]));
+            }
+#pragma unroll
+            for (int o = 32; o; o >>= 1) top_bits = max(top_bits, (unsigned)__shfl_xor((int)top_bits, o));
+            if constexpr (WPR > 1) {
+                if ((t & 63) == 0) s_max[slot][wave] = top_bits;
+                __syncthreads();
+                top_bits = 0;
+#pragma unroll
+                for (int w = 0; w < WPR; w++) top_bits = max(top_bits, s_max[slot][w]);
+            }
+            return __uint_as_float(top_bits);
+        };
+        float mean = mean_square(), eps = a.eps;
+        if (a.r) {
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+                if (skip[v] < 8) store8(h + col[v], f[v]);
         }
-        const float inv = 1.0f / __builtin_sqrtf(sum / (float)cols + a.eps);
-        unsigned top_bits = 0;
+        if (squares_lost(mean, eps)) {  // the same for all waves of a row
+            const float hmax = largest([&](int v) { return f[v]; }), shift = row_shift(hmax, eps);
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
-            if (a.r && skip[v] < 8) store8(h + col[v], f[v]);
-            f[v] = f[v] * inv * g[v];
-#pragma unroll
-            for (int i = 0; i < 8; i++) top_bits = max(top_bits, abs_bits(f[v][i]));
+            for (int v = 0; v < NV; v++) f[v] *= shift;
+            mean = mean_square();
+            if (!(hmax < __builtin_inff())) mean = __builtin_nanf("");
+            eps = eps * shift * shift;
         }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) top_bits = max(top_bits, (unsigned)__shfl_xor((int)top_bits, o));
-        if constexpr (WPR > 1) {
-            if ((t & 63) == 0) s_max[slot][wave] = top_bits;
-            __syncthreads();
-            top_bits = 0;
-#pragma unroll
-            for (int w = 0; w < WPR; w++) top_bits = max(top_bits, s_max[slot][w]);
+        float inv = row_inv(mean, eps);
+        auto y = [&](int v) { return f[v] * inv * g[v]; };
+        float amax = largest(y), scale = amax / a.top, back = a.top / amax;
+        if (row_small(amax)) {  // the same for all waves of a row
+            inv *= ROW_UP;
+            if constexpr (WPR > 1) __syncthreads();
+            amax = largest(y), scale = amax / a.top * ROW_DOWN, back = row_back_up(scale);
         }
-        const float amax = __uint_as_float(top_bits);
-        const float back = row_back(amax, a.top);
-        if (live && t == 0) a.scale[row] = amax / a.top;
+        if (live && t == 0) a.scale[row] = scale;
         unsigned char *q = a.q + row * a.ldq;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             if (skip[v] == 8) continue;
+            const f32x8 yv = y(v);
             unsigned w[2];
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 float s[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    s[i] = __builtin_fminf(__builtin_fmaxf(f[v][4 * p + i] * back, -a.top), a.top);
+                    s[i] = __builtin_fminf(__builtin_fmaxf(yv[4 * p + i] * back, -a.top), a.top);
                 if (a.q_int8) {
                     w[p] = 0;
 #pragma unroll
@@ -148,8 +195,7 @@ __global__ __launch_bounds__(256) void norm_quant_narrow_kernel(NormArgs a) {
         const T *x = static_cast<const T *>(a.x) + row * a.ldx;
         const T *r = static_cast<const T *>(a.r) + row * a.ldr;
         T *h = static_cast<T *>(a.h) + row * a.ldh;
-        float f[8], sum = 0.0f;
-        unsigned top_bits = 0;
+        float f[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             f[i] = 0.0f;
@@ -160,21 +206,39 @@ __global__ __launch_bounds__(256) void norm_quant_narrow_kernel(NormArgs a) {
                 h[i] = s;
                 f[i] = (float)s;
             }
-            sum = __builtin_fmaf(f[i], f[i], sum);
         }
-        const float inv = 1.0f / __builtin_sqrtf(sum / (float)a.cols + a.eps);
+        auto mean_square = [&] {
+            float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (i < a.cols) f[i] = f[i] * inv * (float)gamma[i];
-            top_bits = max(top_bits, abs_bits(f[i]));
+            for (int i = 0; i < 8; i++) sum = __builtin_fmaf(f[i], f[i], sum);
+            return sum / (float)a.cols;
+        };
+        auto largest = [&](float by, const T *g) {  // of f by g
+            unsigned top_bits = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < a.cols) top_bits = max(top_bits, abs_bits(f[i] * by * (g ? (float)g[i] : 1.0f)));
+            return __uint_as_float(top_bits);
+        };
+        float mean = mean_square(), eps = a.eps;
+        if (squares_lost(mean, eps)) {
+            const float hmax = largest(1.0f, nullptr), shift = row_shift(hmax, eps);
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] *= shift;
+            mean = mean_square();
+            if (!(hmax < __builtin_inff())) mean = __builtin_nanf("");
+            eps = eps * shift * shift;
         }
-        const float amax = __uint_as_float(top_bits);
-        const float back = row_back(amax, a.top);
-        a.scale[row] = amax / a.top;
+        float inv = row_inv(mean, eps), amax = largest(inv, gamma), scale = amax / a.top, back = a.top / amax;
+        if (row_small(amax)) {
+            inv *= ROW_UP;
+            amax = largest(inv, gamma), scale = amax / a.top * ROW_DOWN, back = row_back_up(scale);
+        }
+        a.scale[row] = scale;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (i >= a.cols) continue;
-            const float s = __builtin_fminf(__builtin_fmaxf(f[i] * back, -a.top), a.top);
+            const float s = __builtin_fminf(__builtin_fmaxf(f[i] * inv * (float)gamma[i] * back, -a.top), a.top);
             a.q[row * a.ldq + i] = a.q_int8 ? (unsigned char)(signed char)(int)__builtin_rintf(s)
                                             : (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(s, s, 0, false);
         }
