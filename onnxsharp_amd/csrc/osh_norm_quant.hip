@@ -11,6 +11,7 @@
 // e4m3 with the residual 80.5 us (5.8 TB/s; a copy reaches 4.95); one row 3.5 us, launch
 // and latency.
 #include <algorithm>
+#include <cmath>
 
 #include "osh_lm.h"
 
@@ -26,7 +27,7 @@ struct NormArgs {
     unsigned char *q;
     float *scale;
     float eps, top;
-    int q_int8;
+    int eps_exp, q_int8;
 };
 
 // |v| as an integer of the same order, with NaN above infinity: a NaN in gamma, and a NaN or
@@ -34,28 +35,32 @@ struct NormArgs {
 // value that the row stands for.
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// Whether FP32 squares of a row went wrong, mean being their sum / cols: it left FP32's
-// range, or is so small that what they lost below it counts.
-__device__ __forceinline__ bool squares_lost(float mean, float eps) {
-    return !(mean < __builtin_inff()) || !(mean + eps >= 0x1p-100f);
+// A row is done again in steps that hold for every finite one where its squares left FP32's
+// range (mean of squares infinite: inv and amax are then 0; or below 2^-100 with eps) or its
+// scale is not above FP32's normal numbers (amax <= 2^-117): one scalar test of a row, NaN
+// among what it catches.  Tests at each step cost 10% of 65536 x 1024 (113 us for 103).
+__device__ __forceinline__ bool row_is_rare(float inv, float amax) {
+    const unsigned i = __builtin_amdgcn_readfirstlane(__float_as_uint(inv));
+    const unsigned m = __builtin_amdgcn_readfirstlane(__float_as_uint(amax));
+    return i > 0x58800000u /* 2^50 */ || m <= 0x05000000u /* 2^-117 */ || m > 0x7f800000u;
 }
-// Such a row is taken times the power of two that brings the larger of its largest |h| and
-// sqrt(eps) to [1, 2), as far as floats go: y is that of the row times it, with eps times
-// its square.
-__device__ __forceinline__ float row_shift(float hmax, float eps) {
-    const int e = __float_as_uint(__builtin_fmaxf(hmax, __builtin_sqrtf(eps))) >> 23;
+// The steps.  The row is taken times the power of two that brings the larger of its largest
+// |h| and sqrt(eps) (of biased exponent eps_exp) to [1, 2), as far as floats go: y is that of
+// the row times it, with eps times its square.
+__device__ __forceinline__ float row_shift(float hmax, int eps_exp) {
+    const int e = max((int)(__float_as_uint(hmax) >> 23), eps_exp);
     return __uint_as_float((unsigned)min(max(254 - e, 1), 253) << 23);
 }
-// 1 / sqrt; 0 for a row of zeros without eps.
-__device__ __forceinline__ float row_inv(float mean, float eps) {
+// 1 / sqrt; 0 for a row of zeros without eps, NaN for a row that is not finite.
+__device__ __forceinline__ float row_inv(float hmax, float mean, float eps) {
+    if (!(hmax < __builtin_inff())) return __builtin_nanf("");
     return mean + eps == 0.0f ? 0.0f : 1.0f / __builtin_sqrtf(mean + eps);
 }
-
-// Where the scale would lie below FP32's normal numbers, y does so too and has few bits: it
-// is then computed 2^60 times as large.  NaN counts as small, and keeps its NaN.
-__device__ __forceinline__ bool row_small(float amax) { return !(amax > 0x1p-117f); }
+// Where the scale lies below FP32's normal numbers, y does so too and has few bits: it is
+// then taken 2^60 times as large, and `back` is 1 / (2^60 times the scale that is stored), or
+// 0 for a scale of 0.
 constexpr float ROW_UP = 0x1p60f, ROW_DOWN = 0x1p-60f;
-// A small row's 1 / scale for such y, from the scale that is stored; 0 for a scale of 0.
+__device__ __forceinline__ bool row_small(float amax) { return !(amax > 0x1p-117f); }
 __device__ __forceinline__ float row_back_up(float scale) { return scale > 0.0f ? 1.0f / (scale * ROW_UP) : 0.0f; }
 
 // WPR waves share a row; a lane holds NV vectors of 8 neighbouring columns,
@@ -101,12 +106,14 @@ __global__ __launch_bounds__(WPR > 4 ? WPR * 64 : 256) void norm_quant_kernel(No
             }
         }
         // taken in turn: the barrier of each frees the other's LDS
-        auto mean_square = [&] {
+        auto mean_square = [&](auto value) {
             float sum = 0.0f;
 #pragma unroll
-            for (int v = 0; v < NV; v++)
+            for (int v = 0; v < NV; v++) {
+                const f32x8 y = value(v);
 #pragma unroll
-                for (int i = 0; i < 8; i++) sum = __builtin_fmaf(i >= skip[v] ? f[v][i] : 0.0f, f[v][i], sum);
+                for (int i = 0; i < 8; i++) sum = __builtin_fmaf(i >= skip[v] ? y[i] : 0.0f, y[i], sum);
+            }
 #pragma unroll
             for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
             if constexpr (WPR > 1) {
@@ -137,41 +144,50 @@ __global__ __launch_bounds__(WPR > 4 ? WPR * 64 : 256) void norm_quant_kernel(No
             }
             return __uint_as_float(top_bits);
         };
-        float mean = mean_square(), eps = a.eps;
-        if (a.r) {
+        auto row_f = [&](int v) { return f[v]; };
+        float inv = 1.0f / __builtin_sqrtf(mean_square(row_f) + a.eps);
 #pragma unroll
-            for (int v = 0; v < NV; v++)
-                if (skip[v] < 8) store8(h + col[v], f[v]);
+        for (int v = 0; v < NV; v++) {
+            if (a.r && skip[v] < 8) store8(h + col[v], f[v]);
+            f[v] = f[v] * inv * g[v];
         }
-        if (squares_lost(mean, eps)) {  // the same for all waves of a row
-            const float hmax = largest([&](int v) { return f[v]; }), shift = row_shift(hmax, eps);
-#pragma unroll
-            for (int v = 0; v < NV; v++) f[v] *= shift;
-            mean = mean_square();
-            if (!(hmax < __builtin_inff())) mean = __builtin_nanf("");
-            eps = eps * shift * shift;
-        }
-        float inv = row_inv(mean, eps);
-        auto y = [&](int v) { return f[v] * inv * g[v]; };
-        float amax = largest(y), scale = amax / a.top, back = a.top / amax;
-        if (row_small(amax)) {  // the same for all waves of a row
-            inv *= ROW_UP;
+        float amax = largest(row_f);
+        float scale = amax / a.top, back = a.top / amax;
+        if (row_is_rare(inv, amax)) {  // the same for all waves of a row
             if constexpr (WPR > 1) __syncthreads();
-            amax = largest(y), scale = amax / a.top * ROW_DOWN, back = row_back_up(scale);
+            // what this lane stored, or x as it was; no address of it computed ahead of the
+            // row's loads
+            const T *hr = a.r ? h : x, *gr = gamma;
+            asm volatile("" : "+v"(hr), "+v"(gr));
+            constexpr f32x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int v = 0; v < NV; v++) f[v] = skip[v] < 8 ? load8(hr + col[v]) : zero;
+            const float hmax = largest(row_f), by = row_shift(hmax, a.eps_exp);
+#pragma unroll
+            for (int v = 0; v < NV; v++) f[v] *= by;
+            inv = row_inv(hmax, mean_square(row_f), a.eps * by * by);
+            auto y = [&](int v) { return skip[v] < 8 ? f[v] * inv * load8(gr + col[v]) : zero; };
+            amax = largest(y), scale = amax / a.top, back = a.top / amax;
+            if (row_small(amax)) {
+                inv *= ROW_UP;
+                if constexpr (WPR > 1) __syncthreads();
+                amax = largest(y), scale = amax / a.top * ROW_DOWN, back = row_back_up(scale);
+            }
+#pragma unroll
+            for (int v = 0; v < NV; v++) f[v] = y(v);
         }
         if (live && t == 0) a.scale[row] = scale;
         unsigned char *q = a.q + row * a.ldq;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             if (skip[v] == 8) continue;
-            const f32x8 yv = y(v);
             unsigned w[2];
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 float s[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    s[i] = __builtin_fminf(__builtin_fmaxf(yv[4 * p + i] * back, -a.top), a.top);
+                    s[i] = __builtin_fminf(__builtin_fmaxf(f[v][4 * p + i] * back, -a.top), a.top);
                 if (a.q_int8) {
                     w[p] = 0;
 #pragma unroll
@@ -220,16 +236,12 @@ __global__ __launch_bounds__(256) void norm_quant_narrow_kernel(NormArgs a) {
                 if (i < a.cols) top_bits = max(top_bits, abs_bits(f[i] * by * (g ? (float)g[i] : 1.0f)));
             return __uint_as_float(top_bits);
         };
-        float mean = mean_square(), eps = a.eps;
-        if (squares_lost(mean, eps)) {
-            const float hmax = largest(1.0f, nullptr), shift = row_shift(hmax, eps);
+        // the steps that hold for every row, for all
+        const float hmax = largest(1.0f, nullptr), shift = row_shift(hmax, a.eps_exp);
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] *= shift;
-            mean = mean_square();
-            if (!(hmax < __builtin_inff())) mean = __builtin_nanf("");
-            eps = eps * shift * shift;
-        }
-        float inv = row_inv(mean, eps), amax = largest(inv, gamma), scale = amax / a.top, back = a.top / amax;
+        for (int i = 0; i < 8; i++) f[i] *= shift;
+        float inv = row_inv(hmax, mean_square(), a.eps * shift * shift);
+        float amax = largest(inv, gamma), scale = amax / a.top, back = a.top / amax;
         if (row_small(amax)) {
             inv *= ROW_UP;
             amax = largest(inv, gamma), scale = amax / a.top * ROW_DOWN, back = row_back_up(scale);
@@ -328,6 +340,7 @@ OSH_API osh_status osh_rms_norm_quant(int64_t rows, int cols, int dtype, const v
     a.q = static_cast<unsigned char *>(d_q);
     a.scale = d_scale;
     a.eps = eps;
+    a.eps_exp = eps > 0.0f ? std::min(std::ilogb(std::sqrt(eps)), 127) + 127 : 0;
     a.q_int8 = q_type == OSH_T_I8;
     a.top = a.q_int8 ? 127.0f : 448.0f;
     if (dtype == OSH_T_F32) return norm_quant_launch<float>(a, to_stream(s));
