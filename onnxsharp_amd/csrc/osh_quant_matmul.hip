@@ -130,12 +130,14 @@ __device__ __forceinline__ i32x4 load_chunk(const unsigned char *row, int k0, in
     return v;
 }
 
-// Activations.  EXACT ones are for FP32 outputs.  For 16-bit outputs SiLU takes the
-// hardware's reciprocal, and GELU, x - x Q(x) for x > 0 and x Q(-x) below with Q(z) =
+// Activations.  EXACT ones are for FP32 outputs: GELU is x erfc(-x / sqrt 2) / 2, since
+// 1 + erf cancels below zero (4% off at -5, 0 from -5.6 on).  For 16-bit outputs SiLU takes
+// the hardware's reciprocal, and GELU, x - x Q(x) for x > 0 and x Q(-x) below with Q(z) =
 // erfc(z / sqrt 2) / 2, a least-maximum fit of erfc(z) e^(z^2) by t P(t), t = 1 / (1 +
-// 0.4 z): within 7e-8 of erfc in exact arithmetic and 4e-7 in FP32, 1 / 600 of the
-// rounding to 16 bits.  erff is 45 instructions a value against 17: 8 us of
-// 1028 x 5120 x 1280.
+// 0.4 z): within 7e-8 of erfc in exact arithmetic, and GELU within 8e-8 in FP32.  Of its own
+// size it is 5e-7 off for x > -1, 2e-6 at -3, 3e-5 at -5 (1/16 of f16's half step where f16
+// has normal numbers, from -4 up), 5e-4 at -8 and 2e-3 at -12 (1/8 and 1/2 of bf16's).
+// erff is 45 instructions a value against 17: 8 us of 1028 x 5120 x 1280.
 template <bool EXACT>
 __device__ __forceinline__ float apply_act(int act, float v) {
     switch (act) {
@@ -145,7 +147,10 @@ __device__ __forceinline__ float apply_act(int act, float v) {
         return EXACT ? v / e : v * __builtin_amdgcn_rcpf(e);
     }
     case OSH_ACT_GELU: {
-        if (EXACT) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+        if (EXACT) {
+            const float c = v < -64.0f ? -64.0f : v;  // -0 from there on, at -infinity too
+            return 0.5f * c * erfcf(c * -0.70710678118654752f);
+        }
         const float z = __builtin_fabsf(v) * 0.70710678118654752f;
         const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, z, 1.0f));
         float q = -0.20526915788650513f;
