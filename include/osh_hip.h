@@ -650,7 +650,7 @@ typedef struct osh_window_attn {
     int window, sinks;            /* window >= 1, sinks >= 0 */
     int max_q, max_kv;
     int pages, page, table_width; /* pages of page slots; table_width entries a sequence */
-    float scale;                  /* 0 = 1 / sqrt(head_dim) */
+    float scale;                  /* 0 = 1 / sqrt(head_dim); at most 2e38 */
     int reserved;                 /* 0 */
     int64_t tokens;               /* rows of q, k_new, v_new, o */
     const void *d_q, *d_k_new, *d_v_new;

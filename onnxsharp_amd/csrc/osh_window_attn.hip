@@ -751,7 +751,8 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
                                               p->q_heads, p->kv_heads);
     if (p->window < 1 || p->sinks < 0) return fail(OSH_E_INVALID, "WindowAttention: window %d, sinks %d", p->window,
                                                    p->sinks);
-    if (!(p->scale >= 0.0f) || p->scale > 3e38f) return fail(OSH_E_INVALID, "WindowAttention: bad scale");
+    if (!(p->scale >= 0.0f) || p->scale > 2e38f)  // times log2(e) it stays finite
+        return fail(OSH_E_INVALID, "WindowAttention: bad scale");
     if (p->head_dim % 8 || p->head_dim > 256)
         return fail(OSH_E_UNSUPPORTED, "WindowAttention: heads of %d values (multiples of 8 up to 256)", p->head_dim);
     if (p->max_kv > (1 << 30) || p->tokens > (1 << 30) || p->max_q > p->max_kv)

@@ -218,7 +218,8 @@ class WindowAttentionLayer:
                  name: str = "window_attention"):
         if window is not None and window < 1 or sinks < 0:
             raise ValueError(f"WindowAttentionLayer '{name}': window {window}, sinks {sinks}")
-        if scale is not None and not 0.0 < scale < float("inf"):
+        # as a float: 0 stands for 1 / sqrt(head_dim), and times log2(e) it stays finite
+        if scale is not None and not 2.0 ** -126 <= scale <= 2e38:
             raise ValueError(f"WindowAttentionLayer '{name}': scale {scale}")
         self.window, self.sinks, self.scale, self.name = window, sinks, scale, name
 

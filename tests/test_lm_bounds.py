@@ -1,5 +1,6 @@
 """Bounds and scales that the language-model layers refuse before anything touches a
 device, and the rows that a sequence of contradicting lengths holds."""
+import ctypes as C
 import os
 import shutil
 import subprocess
@@ -31,6 +32,22 @@ def test_attention_bounds():
             call(2, max_q, max_kv)
     with pytest.raises(ValueError, match="device tensors"):
         call(2, 3, 5)
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e-46, 3e38, 1e39, -0.5])
+def test_attention_scales_that_are_no_float(scale):
+    # 1e-50 would be 0, which stands for 1 / sqrt(head_dim)
+    with pytest.raises(ValueError, match="scale"):
+        WindowAttentionLayer(scale=scale)
+    assert WindowAttentionLayer(scale=1e-30).scale == 1e-30
+
+
+def test_attention_entry_refuses_a_scale_without_room():
+    p = N.WindowAttn(dtype=N.T_BF16, batch=1, q_heads=1, kv_heads=1, head_dim=64, window=1, max_q=1, max_kv=1, pages=1,
+                     page=1, table_width=1, tokens=1, scale=2.9e38)
+    n = C.c_size_t()
+    assert N.lib().osh_window_attention_scratch_bytes(C.byref(p), C.byref(n)) == N.OSH_E_INVALID
+    assert "scale" in N.last_error()
 
 
 PROGRAM = r"""
