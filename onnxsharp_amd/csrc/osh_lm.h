@@ -46,10 +46,4 @@ inline int elem_bytes(int t) {
     }
 }
 
-// Whether a_bytes from a and b_bytes from b share a byte (NULL shares none).
-inline bool ranges_overlap(const void *a, long long a_bytes, const void *b, long long b_bytes) {
-    const char *a0 = static_cast<const char *>(a), *b0 = static_cast<const char *>(b);
-    return a && b && a0 < b0 + b_bytes && b0 < a0 + a_bytes;
-}
-
 }  // namespace osh

@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include "osh_lm.h"
+#include "osh_overlap.h"
 
 using namespace osh;
 
@@ -309,23 +310,19 @@ OSH_API osh_status osh_rms_norm_quant(int64_t rows, int cols, int dtype, const v
     if (!d_x || !d_gamma || !d_q || !d_scale || (d_res && !d_h)) return fail(OSH_E_INVALID, "RmsNormQuant: NULL pointer");
     if (ldx < cols || ldq < cols || (d_res && (ldr < cols || ldh < cols)))
         return fail(OSH_E_INVALID, "RmsNormQuant: a row pitch below the columns");
-    const long long e = elem_bytes(dtype), last = rows - 1;
-    const long long bx = (last * ldx + cols) * e, br = (last * ldr + cols) * e, bh = (last * ldh + cols) * e;
-    const long long bq = last * ldq + cols;
-    if (d_res) {
-        if (ranges_overlap(d_h, bh, d_x, bx) && !(d_h == d_x && ldh == ldx))
-            return fail(OSH_E_INVALID, "RmsNormQuant: h overlaps x without being x");
-        if (ranges_overlap(d_h, bh, d_res, br) && !(d_h == d_res && ldh == ldr))
-            return fail(OSH_E_INVALID, "RmsNormQuant: h overlaps the residual without being it");
-        if (ranges_overlap(d_q, bq, d_res, br) || ranges_overlap(d_q, bq, d_h, bh) ||
-            ranges_overlap(d_h, bh, d_gamma, cols * e) || ranges_overlap(d_h, bh, d_scale, rows * 4) ||
-            ranges_overlap(d_scale, rows * 4, d_res, br))
-            return fail(OSH_E_INVALID, "RmsNormQuant: an output overlaps another operand");
-    }
-    if (ranges_overlap(d_q, bq, d_x, bx) || ranges_overlap(d_q, bq, d_gamma, cols * e) ||
-        ranges_overlap(d_q, bq, d_scale, rows * 4) || ranges_overlap(d_scale, rows * 4, d_x, bx) ||
-        ranges_overlap(d_scale, rows * 4, d_gamma, cols * e))
+    const long long e = elem_bytes(dtype);
+    const Strided x = strided_rows(d_x, rows, ldx * e, cols * e), r = strided_rows(d_res, rows, ldr * e, cols * e),
+                  h = strided_rows(d_res ? d_h : nullptr, rows, ldh * e, cols * e), g(d_gamma, cols * e),
+                  q = strided_rows(d_q, rows, ldq, cols), scale(d_scale, rows * 4);
+    if (share_bytes(h, x) && !(d_h == d_x && ldh == ldx))
+        return fail(OSH_E_INVALID, "RmsNormQuant: h overlaps x without being x");
+    if (share_bytes(h, r) && !(d_h == d_res && ldh == ldr))
+        return fail(OSH_E_INVALID, "RmsNormQuant: h overlaps the residual without being it");
+    if (share_bytes(h, g) || share_bytes(h, q) || share_bytes(h, scale) || share_bytes(q, scale))
         return fail(OSH_E_INVALID, "RmsNormQuant: an output overlaps another operand");
+    for (const Strided &t : {x, r, g})
+        if (share_bytes(q, t) || share_bytes(scale, t))
+            return fail(OSH_E_INVALID, "RmsNormQuant: an output overlaps another operand");
     NormArgs a;
     a.rows = rows;
     a.cols = cols;

@@ -25,6 +25,7 @@
 #include <algorithm>
 
 #include "osh_lm.h"
+#include "osh_overlap.h"
 
 using namespace osh;
 
@@ -819,11 +820,11 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
         return fail(OSH_E_INVALID, "QuantMatMul: a row pitch below the columns");
     if ((long long)cdiv(m, 64) * cdiv(n, 64) >= (1LL << 23))
         return fail(OSH_E_UNSUPPORTED, "QuantMatMul: %d x %d outputs", m, n);
-    const long long e = elem_bytes(dtype), by = ((m - 1LL) * ldy + n) * e;
-    if (ranges_overlap(d_y, by, d_a, (m - 1LL) * lda + k) || ranges_overlap(d_y, by, d_w, (n - 1LL) * ldw + k) ||
-        ranges_overlap(d_y, by, d_sa, m * 4LL) || ranges_overlap(d_y, by, d_sw, n * 4LL) ||
-        ranges_overlap(d_y, by, d_bias, n * 4LL) ||
-        (ranges_overlap(d_y, by, d_res, ((m - 1LL) * ldr + n) * e) && !(d_y == d_res && ldy == ldr)))
+    const long long e = elem_bytes(dtype);
+    const Strided y = strided_rows(d_y, m, ldy * e, n * e), res = strided_rows(d_res, m, ldr * e, n * e);
+    if (share_bytes(y, strided_rows(d_a, m, lda, k)) || share_bytes(y, strided_rows(d_w, n, ldw, k)) ||
+        share_bytes(y, Strided(d_sa, m * 4LL)) || share_bytes(y, Strided(d_sw, n * 4LL)) ||
+        share_bytes(y, Strided(d_bias, n * 4LL)) || (share_bytes(y, res) && !(d_y == d_res && ldy == ldr)))
         return fail(OSH_E_INVALID, "QuantMatMul: y overlaps an operand");
     QmmArgs p;
     p.m = m;

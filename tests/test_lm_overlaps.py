@@ -130,3 +130,33 @@ def _attn(**kw):
 def test_attention_refuses_shared_memory(kw, msg):
     assert _attn(**kw) == N.OSH_E_INVALID
     assert msg in N.last_error()
+
+
+def _p(i, off=0):
+    return C.c_void_p((i << 40) + off)
+
+
+def _norm(rows=4, cols=16, x=_p(1), ldx=16, res=_p(2), ldr=16, g=_p(3), h=_p(4), ldh=16, q=_p(5), ldq=16, scale=_p(6)):
+    return N.lib().osh_rms_norm_quant(rows, cols, N.T_BF16, x, ldx, res, ldr, g, 1e-5, h, ldh, N.T_I8, q, ldq, scale, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(h=_p(1), ldx=40, ldh=41), dict(h=_p(1, 30), ldx=40, ldh=40), dict(h=_p(1, 50), ldx=40, ldh=40),
+    dict(h=_p(3, 30)), dict(q=_p(4, 127)), dict(q=_p(2), ldr=20, ldq=40), dict(scale=_p(1, 124)), dict(scale=_p(5, 60)),
+    dict(scale=_p(3, -12)), dict(res=None, h=None, q=_p(1, 1)), dict(res=None, h=None, scale=_p(5)),
+])
+def test_norm_refuses_shared_memory(kw):
+    assert _norm(**kw) == N.OSH_E_INVALID and "overlaps" in N.last_error()
+
+
+def _mm(m=4, n=8, k=16, a=_p(1), lda=16, w=_p(3), ldw=16, bias=_p(5), res=_p(6), ldr=8, y=_p(7), ldy=8):
+    return N.lib().osh_quant_matmul(m, n, k, N.T_I8, a, lda, _p(2), w, ldw, _p(4), bias, N.ACT_NONE, N.T_F16, res, ldr, y,
+                                    ldy, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(y=_p(1), ldy=8), dict(y=_p(3, 127)), dict(y=_p(2, 15)), dict(y=_p(4, -60)), dict(y=_p(5, 31)),
+    dict(y=_p(6, 14), ldr=16, ldy=16), dict(y=_p(6, 18), ldr=16, ldy=16), dict(y=_p(6), ldr=16, ldy=17),
+])
+def test_matmul_refuses_shared_memory(kw):
+    assert _mm(**kw) == N.OSH_E_INVALID and "overlaps" in N.last_error()
