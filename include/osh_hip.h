@@ -627,13 +627,14 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
  *   o = softmax over the visible j of (q . k_j * scale) times v_j,
  *   visible: j <= p and (j > p - window or j < sinks).
  * Query head h reads key head h / (q_heads / kv_heads).  Sums, softmax and its
- * statistics are FP32; the weights are rounded to dtype for the product with v.
+ * statistics are FP32; the weights are rounded to dtype for the product with v.  Their sum
+ * is that of the rounded weights where max_q times the heads of a group passes 16 and
+ * head_dim is 65 to 128, of the FP32 ones elsewhere.
  * Pages and slots that no query of the call sees are not read (stale entries of
  * d_table before the window may hold anything).  A key that is not finite reaches only
- * the queries that see it; a value that is not finite and that some query of a
- * sequence sees may make others of the same call NaN (their weight for it is 0, and 0
- * times it is NaN).  A new token's slot must belong
- * to its sequence alone.
+ * the queries that see it; a value that is not finite and that some query of a sequence
+ * sees may make other queries of that sequence in the call NaN (their weight for it is 0,
+ * and 0 times it is NaN).  A new token's slot must belong to its sequence alone.
  * max_q and max_kv are the host's bounds of the lengths.  All rows of a sequence whose
  * lengths contradict each other, the bounds or the table get NaN, and so does a query that
  * sees a cached key whose page id lies outside [0, pages).  A new token whose own page id
@@ -644,7 +645,9 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
  * o, the scratch and the pages share no memory with themselves, each other or an input
  * (views that interleave without a common byte are fine); what shares is refused.
  * Strides are in elements, the head_dim values of a head contiguous, any alignment
- * of whole elements.  head_dim % 8 == 0 and <= 256, dtype f16 or bf16. */
+ * of whole elements.  head_dim % 8 == 0 and <= 256, dtype f16 or bf16; max_kv and tokens
+ * <= 2^30, strides of new and cached keys and values < 2^31, and fewer than 2^22 row blocks:
+ * batch * kv_heads, times max_q * (q_heads / kv_heads) / 128 where that passes 1. */
 typedef struct osh_window_attn {
     int dtype, batch, q_heads, kv_heads, head_dim;
     int window, sinks;            /* window >= 1, sinks >= 0 */

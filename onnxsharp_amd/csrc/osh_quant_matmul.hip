@@ -18,8 +18,8 @@
 // it.  FP32 outputs take their operands to f16, which holds every e4m3 value (all 256
 // codes checked, NaN among them), and v_mfma_f32_16x16x32_f16, whose sums are within
 // FP32's roundings: 2.6e-8 at k = 512, 1.2e-7 at 8192.  It has half the rate, and the
-// conversions run beside it: 8192 x 8192 x 4096 469 us (1.2 PFLOP/s; with the 8-bit
-// instruction 252), 1028 x 5120 x 1280 25.2 (17.6), 24 x 8192 x 4096 10.8 (10.5).
+// conversions run beside it: 8192 x 8192 x 4096 451 us (1.2 PFLOP/s; with the 8-bit
+// instruction 252), 1028 x 5120 x 1280 23.3 (17.6), 24 x 8192 x 4096 10.1 (10.1).
 #include <limits.h>
 
 #include <algorithm>
@@ -301,8 +301,9 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned c
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, off, soff, 0, 0);
 }
 
-// Tile of BM rows by BN outputs, WM x WN waves; k-blocks pass through two LDS
-// buffers.  Chunk c of tile row r lies at slot c ^ (r / 2 % 8) of the row's 128
+// Tile of BM rows by BN outputs, WM x WN waves; k-blocks pass through registers into two
+// LDS buffers: operands at any address, and products with fewer tiles than CUs (8192 x 8191
+// x 4097 e4m3 486 us, 215 at whole 16-byte chunks; 128 x 4096 x 4096 20.6).  Chunk c of tile row r lies at slot c ^ (r / 2 % 8) of the row's 128
 // bytes: the 16 lanes of an operand read then meet all 64 banks once.
 template <int Q, typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void qmm_tile_kernel(QmmArgs p) {
@@ -430,8 +431,8 @@ __device__ __forceinline__ void buffer_store8(typename Vec8<T>::type v, __amdgpu
 // to memory, needs no LDS, so it runs over them; its stores drain under the next
 // tile's first block, whose barrier does not wait for them.
 //
-// 256 x 256 of eight waves: 8192 x 8192 x 4096 e4m3 218 us (2.5 PFLOP/s; a large
-// library product reaches 2.65 here), 260 with a residual, whose 134 MB the CUs all
+// 256 x 256 of eight waves: 8192 x 8192 x 4096 e4m3 215 us (2.56 PFLOP/s; a large
+// library product reaches 2.65 here), 288 with a residual, whose 134 MB the CUs all
 // want at their tiles' ends.  Bringing it to L2 ahead of the end cost 6 us instead.
 // Four waves of 128 x 128 read a quarter less LDS, but their 256 accumulators left
 // no register free and the spills cost more (275 us).
@@ -650,7 +651,8 @@ constexpr int qmm_lds() {
 // every WAVES-th k-block; the weights go from memory to registers, each byte once.
 // What bounds it is how many bytes are in flight: the loads of U k-blocks of a wave
 // start together, without a condition around them (24 x 8192 x 4096 e4m3: 13.6 us a
-// block at a time, 9.9 so, of which the host takes 9).  The waves' sums meet in LDS, in the order of the waves.
+// block at a time, 9.8 so, all of it on the device: the host's part of a call, 9, runs
+// beside it).  The waves' sums meet in LDS, in the order of the waves.
 template <int Q, typename T, int MB, int NB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void qmm_rows_kernel(QmmArgs p) {
     using Acc = typename QAcc<Q>::type;

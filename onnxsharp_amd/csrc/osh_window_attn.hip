@@ -3,14 +3,18 @@
 //
 // The G = q_heads / kv_heads query heads of a key head read the same keys, so a
 // sequence's queries at one key head form a matrix of ql * G rows (row = token * G
-// + head of the group), taken 16 rows a workgroup.  For a row block the visible
-// keys are the sinks below the window and one range; "key number" v counts them:
+// + head of the group), taken 16 rows a workgroup where that is all of them, 128 where
+// there are more.  For a row block the visible keys are the sinks below the window and one range; "key number" v counts them:
 // v < se is key v, the others are key v - se + lo.
 //
 // Softmax in one pass: each row keeps its running maximum m, the sum l of
 // 2^(s - m) and the weighted sum of values; a larger maximum rescales both by
 // 2^(m_old - m).  Waves and splits that saw different keys are joined by the same
-// rule.
+// rule.  All of it is FP32 but the weights, which the MFMAs take in the type of V: half a
+// step each, which adds a quarter to 40% to an output's own rounding.  l sums the FP32
+// weights; row blocks of 128 at heads of 65 to 128 sum the rounded ones, which V is weighted
+// with, two an instruction.  The two sums are half a step apart at most, all weights rounded
+// one way.
 #include <limits.h>
 
 #include <algorithm>
@@ -166,8 +170,9 @@ __device__ __forceinline__ int win_page(const osh_window_attn &p, const WinSeq &
 // Memory's latency is what a step waits for, so the next step's K and V are loaded
 // before this one is computed (BUFS 2; heads above 128 have no registers for it),
 // their addresses pass through the wave's LDS the step before, and the page ids
-// they need are loaded the step before that.  HBM bounds it: 64 sequences to 8192,
-// window 4096, take 191 us (5.1 TB/s; a copy reaches 4.95), 234 with one step at a time.
+// they need are loaded the step before that.  The loads in flight bound it: 64 sequences
+// to 8192, window 4096, take 191 us (5.1 TB/s, each byte read once; reads alone reach 7.15),
+// 234 with one step at a time.
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void window_attn_rows_kernel(WinArgs a) {
     constexpr int NS = DP > 128 ? 2 : 1;       // sets of up to 128 values
@@ -408,11 +413,12 @@ __device__ __forceinline__ s16x4 read_transposed(const unsigned char *at) {
 // rows spread a 16-lane read over all banks, values' rows one of 4 rows x 64 bytes.
 //
 // Workgroups of 128 rows, two a CU: their phases drift apart, so that one's MFMAs run
-// under the other's exponentials (one of 256 rows: 323 us for 314 at 8192 tokens, 87
-// for 49 at pieces of prompts).  What bounds it is that a SIMD's two waves still spend
-// 2.4 us on a tile each, of which MFMAs are 0.85 and vector instructions 0.9: 8192 tokens,
-// 32 heads of 128, window 2048: 294 us (820 TFLOP/s), without a window 606 (910).  The next
-// tile's scores interleaved with this one's exponentials in one wave were 5% slower.
+// under the other's exponentials (one of 256 rows took 3% more at 8192 tokens and 78% more
+// at pieces of prompts).  What bounds it is that a SIMD's two waves still spend 2.4 us on a
+// tile each, of which MFMAs are 0.85 and vector instructions 0.9: 8192 tokens, 32 heads of
+// 128, window 2048: 293 us (820 TFLOP/s), without a window 591 (930); 8 heads of 256, window
+// 2048: 248 (490).  The next tile's scores interleaved with this one's exponentials in one
+// wave were 5% slower.
 //
 // The running maximum moves only when a row's scores pass it by 2^8: weights up to
 // 256 are as exact, and most tiles rescale nothing.
@@ -483,8 +489,8 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
         if (t < fresh0) page_id = win_page(p, sq, keys, b, t * 64 + my_tile_row, a.page_shift);
     };
     // Heads of 65 to 128 keep the byte offsets of a lane's chunks in a tile of new tokens
-    // and sum their rounded weights two an instruction (634 -> 606 us at 8192 tokens
-    // without a window); above there are no registers for the offsets, below neither gains.
+    // and sum their rounded weights two an instruction (4% of 8192 tokens without a window);
+    // above there are no registers for the offsets, below neither gains.
     constexpr bool KEEP = C == 16;
     unsigned k_off[RW], v_off[RW];
     bool k_in[RW], v_in[RW];
@@ -778,8 +784,13 @@ static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch
     // as 1024; 64 ragged ones of 8192 191 us unsplit, 207 split in two.
     const long long want = units ? std::max(1LL, 2LL * device_cus() / units) : 1;
     a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
-    // One launch of eight waves for short spans, else splits and a join: over 516 keys 10.2
-    // us against 12.6, over 400 12.3 against 13.7, over 1000 18.7 against 16.0.
+    // One launch of eight waves for short spans, else four waves, splits and a join.  Device
+    // times, eight waves against four, over 64, 200, 400, 640, 800 and 1000 keys: one sequence
+    // of 12 heads of 64 on 4: 6.3 (5.9), 7.0 (7.8), 8.6 (10.9), 10.2 (12.6), 11.8 (12.5), 13.0
+    // (13.0) us; 4 of 32 heads of 128 on 8: 7.9 (7.3), 8.9 (9.7), 11.7 (14.0), 13.6 (15.2), 15.7
+    // (15.3), 18.2 (15.6); 32 of them, a workgroup a CU: 8.2 (7.5), 9.7 (10.1), 16.9 (18.0),
+    // 20.3 (26.1), 23.5 (29.6), 26.6 (32.2).  Few workgroups lose past 640 keys, many do not;
+    // below 100 keys four waves are 0.7 us ahead.
     a.wide = a.tile_rows == 16 && span <= 640 && units <= device_cus() && p->head_dim <= 128;
     if (a.wide) a.splits = 1;
     const long long parts = a.splits > 1 ? units * a.splits : 0;

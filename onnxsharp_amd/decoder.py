@@ -1,5 +1,5 @@
-"""One block of a decoder-only language model from the layers of lm_layers: prompts,
-pieces of prompts and single tokens of many sequences in one call.
+"""An example: a decoder block from the layers of lm_layers, over prompts, pieces of prompts
+and single tokens of many sequences in one call.
 
     x -> RMS norm, 8 bits -> q, k, v -> window attention over the pages -> RMS norm, 8
     bits -> output product -> add, RMS norm, 8 bits -> up, SiLU -> RMS norm, 8 bits ->
@@ -8,7 +8,7 @@ pieces of prompts and single tokens of many sequences in one call.
 Six products' worth of operands move in 8 bits; the residual stream stays in 16.  The
 attention's and the feed-forward's inner outputs are normalized before they are rounded
 to 8 bits, so one operator makes every 8-bit row.  The block knows positions through the
-causal window alone.
+causal window alone; it is no released model's architecture.
 
 `python -m onnxsharp_amd.decoder` runs a prompt and a few tokens on the GPU.
 """
