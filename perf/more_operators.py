@@ -1,0 +1,419 @@
+"""Performance cases of the operators of a decoder block that is served in 4 bits: products
+with 4-bit weights and group scales, attention over a paged cache whose keys and values are
+held in 4 bits, and the norms after and before a block with its gate and residual scale.
+
+`run` computes them in their plain form from torch's elementary operations, or through the
+framework's layers where `own` is true.  The listed cases stand for ranges that `draw`
+samples.
+
+Inputs: activations N(0, 1) with a few large channels where they are a residual stream;
+weights quantized from normals, with or without zero points; queries, keys and values
+N(0, 1), the cached ones quantized; pages handed out in no order.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+_DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+_EPS = 1e-5
+
+_MM_OPS = 2.0 * 8192 * 4096 * 8192
+_NORM_VALUES = 16384 * 4096
+_ATTN_SCORES = 32.0 * 4096 * 16384      # scores the plain form holds at once
+_ATTN_CACHE = 64.0 * 8192 * 8 * 128     # values of K in the cache
+
+
+def listed():
+    return [
+        # one token between two blocks of an answer being written: latency
+        dict(name="norm_token", kind="norm", rows=1, cols=4096, dtype="bf16", post=True, gate="cols", act="None"),
+        # a ragged sequence at an odd width, a gate computed for every token
+        dict(name="norm_ragged", kind="norm", rows=1028, cols=1283, dtype="f16", post=True, gate="rows",
+             act="Sigmoid"),
+        # a batch of prompts: memory-bound
+        dict(name="norm_large", kind="norm", rows=16384, cols=4096, dtype="bf16", post=True, gate="cols", act="None"),
+        # one token through a small projection in single precision: latency
+        dict(name="mm_token", kind="mm", m=1, k=768, n=768, group=32, zeros=True, dtype="f32", act="None", bias=True,
+             res=False),
+        # one token through a large feed-forward layer: reads the weights
+        dict(name="mm_token_large", kind="mm", m=1, k=8192, n=16384, group=128, zeros=False, dtype="bf16", act="Silu",
+             bias=False, res=False),
+        # a step of 24 sequences back into the residual stream
+        dict(name="mm_step", kind="mm", m=24, k=8192, n=4096, group=64, zeros=True, dtype="f16", act="None", bias=True,
+             res=True),
+        # a ragged sequence, a width that ends inside a group
+        dict(name="mm_ragged", kind="mm", m=517, k=1283, n=2051, group=32, zeros=True, dtype="f32", act="Gelu",
+             bias=True, res=False),
+        # a batch of prompts: the throughput end
+        dict(name="mm_large", kind="mm", m=8192, k=4096, n=8192, group=128, zeros=False, dtype="bf16", act="None",
+             bias=False, res=True),
+        # one token of one sequence: latency
+        dict(name="attn_token", kind="attn", b=1, hq=12, hkv=4, d=64, group=32, q_max=1, kv_max=600, window=512,
+             sinks=4, page=16, dtype="f16", ragged=False),
+        # a step of 64 sequences of different lengths: reads the cache
+        dict(name="attn_decode", kind="attn", b=64, hq=32, hkv=8, d=128, group=128, q_max=1, kv_max=8192, window=8192,
+             sinks=0, page=64, dtype="bf16", ragged=True),
+        # few sequences with long histories: a sequence has to fill the card; groups of 32
+        dict(name="attn_long", kind="attn", b=2, hq=32, hkv=8, d=128, group=32, q_max=1, kv_max=131072, window=131072,
+             sinks=0, page=64, dtype="bf16", ragged=False),
+        # a piece of a long prompt behind its history
+        dict(name="attn_piece", kind="attn", b=1, hq=32, hkv=8, d=128, group=64, q_max=4096, kv_max=16384, window=8192,
+             sinks=4, page=64, dtype="bf16", ragged=False),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "mm", "mm", "attn", "attn"])
+    while True:
+        if kind == "norm":
+            c = dict(kind="norm", rows=_log_int(rng, 1, 16384), cols=_log_int(rng, 64, 16384),
+                     dtype=rng.choice(["f32", "f16", "bf16", "bf16"]), post=rng.random() < 0.6,
+                     gate=rng.choice(["none", "cols", "rows"]), act=rng.choice(["None", "Sigmoid"]))
+            if c["gate"] == "none":
+                c["act"] = "None"
+            if rng.random() < 0.6:  # the round widths of real models
+                c["cols"] = (c["cols"] + 63) // 64 * 64
+            cost = (2 if c["dtype"] == "f32" else 1) * (1.25 if c["gate"] == "rows" else 1)
+            if c["rows"] * c["cols"] * cost <= _NORM_VALUES:
+                return c
+        elif kind == "mm":
+            c = dict(kind="mm", m=_log_int(rng, 1, 8192), k=_log_int(rng, 64, 8192), n=_log_int(rng, 64, 8192),
+                     group=rng.choice([32, 64, 128]), zeros=rng.random() < 0.5,
+                     dtype=rng.choice(["f32", "f16", "bf16", "bf16"]), act=rng.choice(["None", "Relu", "Silu", "Gelu"]),
+                     bias=rng.random() < 0.5, res=rng.random() < 0.5)
+            if rng.random() < 0.7:
+                c["k"], c["n"] = (c["k"] + 127) // 128 * 128, (c["n"] + 63) // 64 * 64
+            if 2.0 * c["m"] * c["k"] * c["n"] * (4 if c["dtype"] == "f32" else 1) <= _MM_OPS:
+                return c
+        else:
+            hkv = rng.choice([1, 2, 4, 8])
+            q_max = rng.choice([1, 1, rng.randint(2, 8), _log_int(rng, 9, 4096)])
+            d = rng.choice([32, 64, 96, 128, 128, 256])
+            c = dict(kind="attn", b=_log_int(rng, 1, 64), hq=hkv * rng.choice([1, 2, 3, 4, 8]), hkv=hkv, d=d,
+                     group=rng.choice([g for g in (32, 64, 128) if d % g == 0]), q_max=q_max,
+                     kv_max=q_max + _log_int(rng, 1, 32768) - 1, window=_log_int(rng, 16, 32768),
+                     sinks=rng.choice([0, 1, 4, 4, 16, 130]), page=rng.choice([16, 32, 64, 128]),
+                     dtype=rng.choice(["f16", "bf16"]), ragged=rng.random() < 0.6)
+            if (1.0 * c["b"] * c["hq"] * c["q_max"] * c["kv_max"] <= _ATTN_SCORES / 4
+                    and 1.0 * c["b"] * c["kv_max"] * c["hkv"] * c["d"] <= _ATTN_CACHE / 4):
+                return c
+
+
+# ------------------------------------------------------------------- inputs
+
+def _two_a_byte(c):
+    """Codes 0..15 [..., k] two a byte, the even one in the low half."""
+    c = c.to(torch.uint8)
+    if c.shape[-1] % 2:
+        c = torch.nn.functional.pad(c, (0, 1))
+    return c[..., 0::2] | c[..., 1::2] << 4
+
+
+def _one_a_byte(p):
+    return torch.stack((p & 15, p >> 4), -1).flatten(-2)
+
+
+def _quantize_weight(w, group, zeros, t):
+    """w [n, k] in codes of 4 bits, a scale (and a zero point) a group of a row."""
+    n, k = w.shape
+    groups = (k + group - 1) // group
+    full = torch.nn.functional.pad(w, (0, groups * group - k)).reshape(n, groups, group)
+    if zeros:
+        lo, hi = full.amin(2).clamp(max=0), full.amax(2).clamp(min=0)
+        scale = ((hi - lo) / 15).to(t)
+        zero = (-lo / scale.float()).round().clamp(0, 15)
+    else:
+        scale = (full.abs().amax(2) / 7).to(t)
+        zero = torch.full_like(full[..., 0], 8)
+    codes = (full / scale.float()[..., None] + zero[..., None]).round().clamp(0, 15).reshape(n, -1)[:, :k]
+    return _two_a_byte(codes), scale, _two_a_byte(zero) if zeros else None
+
+
+def _quantize_kv(v, group):
+    """v [..., d] of a cache's type: codes two a byte [..., d / 2] and (scale, lo) of each
+    group [..., d / group, 2] in v's type."""
+    f = v.float().unflatten(-1, (-1, group))
+    lo = f.amin(-1, keepdim=True)
+    scale = ((f.amax(-1, keepdim=True) - lo) / 15).to(v.dtype).float()
+    codes = torch.where(scale > 0, torch.round((f - lo) / scale), torch.zeros_like(f)).clamp(0, 15)
+    return _two_a_byte(codes.flatten(-2)), torch.cat((scale, lo), -1).to(v.dtype)
+
+
+def _kv_values(codes, scales, group):
+    """What codes and (scale, lo) stand for, in FP32."""
+    c = _one_a_byte(codes).float().unflatten(-1, (-1, group))
+    s = scales.float()
+    return (s[..., 1:] + s[..., :1] * c).flatten(-2)
+
+
+def _lens(case, seed):
+    """The sequences' new and whole lengths, as the host of a server knows them: the
+    case's own lengths, with the histories dealt out by the seed."""
+    b, q_max, past = case["b"], case["q_max"], case["kv_max"] - case["q_max"]
+    if not case["ragged"]:
+        return [q_max] * b, [q_max + past] * b
+    g = torch.Generator().manual_seed(b * 1000003 + q_max * 1009 + past)
+    ql = torch.randint((q_max + 3) // 4, q_max + 1, (b,), generator=g)
+    old = torch.randint(past // 4, past + 1, (b,), generator=g)
+    ql[0], old[-1] = q_max, past
+    old = old[torch.randperm(b, generator=g.manual_seed(seed))]
+    return ql.tolist(), (ql + old).tolist()
+
+
+def prepare(case, seed):
+    seed = int(seed) % (1 << 62)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    normal = lambda *shape: torch.randn(shape, generator=g, device="cuda")  # noqa: E731
+    s = dict(case)
+    t = _DT[case["dtype"]]
+    if case["kind"] == "norm":
+        rows, cols = case["rows"], case["cols"]
+        loud = 1.0 + 20.0 * (torch.rand(cols, generator=g, device="cuda") < 0.01).float()
+        s["x"] = (normal(rows, cols) * loud).to(t)
+        s["branch"] = normal(rows, cols).to(t)
+        s["gamma"] = (1.0 + 0.2 * normal(cols)).to(t)
+        s["post_gamma"] = (1.0 + 0.2 * normal(cols)).to(t) if case["post"] else None
+        s["gates"] = {"none": None, "cols": (cols,), "rows": (rows, cols)}[case["gate"]]
+        s["gates"] = None if s["gates"] is None else (0.5 + 0.2 * normal(*s["gates"])).to(t)
+        s["a"], s["b"] = 1.0, 0.7071
+    elif case["kind"] == "mm":
+        m, n, k = case["m"], case["n"], case["k"]
+        s["x"] = normal(m, k).to(t)
+        s["codes"], s["scale"], s["zero"] = _quantize_weight(normal(n, k) / math.sqrt(k), case["group"], case["zeros"], t)
+        s["b"] = 0.1 * normal(n) if case["bias"] else None
+        s["r"] = normal(m, n).to(t) if case["res"] else None
+        if own:  # laid out once, when the model is loaded
+            from onnxsharp_amd.lm_layers import Int4Weight
+            s["w"] = Int4Weight(s["codes"], s["scale"], s["zero"], k=k, group=case["group"])
+    else:
+        b, page, hkv, d, group = case["b"], case["page"], case["hkv"], case["d"], case["group"]
+        ql, kl = _lens(case, seed)
+        width = (case["kv_max"] + page - 1) // page
+        # a page's slots of one head next to each other in memory
+        for name in ("k", "v"):
+            codes = torch.empty((b * width, hkv, page, d // 2), dtype=torch.uint8, device="cuda")
+            scales = torch.empty((b * width, hkv, page, d // group, 2), dtype=t, device="cuda")
+            for i in range(0, b * width, 1024):
+                n = min(1024, b * width - i)
+                codes[i:i + n], scales[i:i + n] = _quantize_kv(normal(n, hkv, page, d).to(t), group)
+            s[name + "p"], s[name + "s"] = codes.transpose(1, 2), scales.transpose(1, 2)
+        s["table"] = torch.randperm(b * width, generator=g, device="cuda").reshape(b, width).to(torch.int32)
+        starts = [sum(ql[:i]) for i in range(b + 1)]
+        s["cu"] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        s["kl"] = torch.tensor(kl, dtype=torch.int32, device="cuda")
+        s["x"] = normal(starts[-1], case["hq"], d).to(t)
+        s["k"] = normal(starts[-1], hkv, d).to(t)
+        s["v"] = normal(starts[-1], hkv, d).to(t)
+        if own:
+            from onnxsharp_amd.lm_layers import PagedKv4Cache
+            s["cache"] = PagedKv4Cache(s["kp"], s["vp"], s["ks"], s["vs"], s["table"])
+    return s
+
+
+# -------------------------------------------------------------- plain forms
+
+def _activate(y, act):
+    if act == "Relu":
+        return torch.where(y > 0, y, torch.zeros_like(y))
+    if act == "Silu":
+        return y / (1.0 + torch.exp(-y))
+    if act == "Sigmoid":
+        return 1.0 / (1.0 + torch.exp(-y))
+    if act == "Gelu":
+        return 0.5 * y * (1.0 + torch.erf(y * math.sqrt(0.5)))
+    return y
+
+
+def _rms(f, gamma):
+    return f * (1.0 / torch.sqrt((f * f).mean(1, keepdim=True) + _EPS)) * gamma.float()
+
+
+def _plain_norm(s):
+    n = s["branch"].float()
+    if s["post_gamma"] is not None:
+        n = _rms(n, s["post_gamma"])
+    if s["gates"] is not None:
+        n = n * _activate(s["gates"].float(), s["act"])
+    h = (s["a"] * s["x"].float() + s["b"] * n).to(s["x"].dtype)
+    return h, _rms(h.float(), s["gamma"]).to(h.dtype)
+
+
+def _plain_mm(s):
+    k, group = s["k"], s["group"]
+    zero = 8.0 if s["zero"] is None else _one_a_byte(s["zero"])[:, :s["scale"].shape[1]].float().repeat_interleave(
+        group, 1)[:, :k]
+    w = (_one_a_byte(s["codes"])[:, :k].float() - zero) * s["scale"].float().repeat_interleave(group, 1)[:, :k]
+    y = s["x"].float() @ w.t().contiguous()
+    if s["b"] is not None:
+        y = y + s["b"]
+    y = _activate(y, s["act"])
+    if s["r"] is not None:
+        y = y + s["r"].float()
+    return y.to(_DT[s["dtype"]])
+
+
+def _plain_attn(s):
+    b, hq, hkv, d, page, q_max, group = s["b"], s["hq"], s["hkv"], s["d"], s["page"], s["q_max"], s["group"]
+    x, table, cu, kl = s["x"], s["table"].long(), s["cu"].long(), s["kl"].long()
+    # the new tokens' sequences and positions, and their places in the cache
+    tok = torch.arange(x.shape[0], device=x.device)
+    seq = torch.searchsorted(cu, tok, right=True) - 1
+    pos = kl[seq] - (cu[seq + 1] - tok)
+    place = (table[seq, pos // page], pos % page)
+    stored = []
+    for new, codes, scales in ((s["k"], s["kp"], s["ks"]), (s["v"], s["vp"], s["vs"])):
+        c, sc = _quantize_kv(new, group)
+        codes[place], scales[place] = c, sc
+        stored.append(_kv_values(c, sc, group).to(x.dtype))
+    # every sequence's keys and values in order, queries padded to the longest
+    keys = _kv_values(s["kp"][table], s["ks"][table], group).reshape(b, -1, hkv, d).permute(0, 2, 3, 1).contiguous()
+    vals = _kv_values(s["vp"][table], s["vs"][table], group).reshape(b, -1, hkv, d).transpose(1, 2).contiguous()
+    row = tok - cu[seq]
+    q = torch.zeros((b, q_max, hq, d), device=x.device)
+    q[seq, row] = x.float()
+    q = q.reshape(b, q_max, hkv, hq // hkv, d).permute(0, 2, 3, 1, 4).reshape(b, hkv, -1, d)
+    p = torch.zeros((b, q_max), dtype=torch.long, device=x.device)
+    p[seq, row] = pos
+    j = torch.arange(keys.shape[3], device=x.device)
+    seen = (j <= p[..., None]) & ((j > p[..., None] - s["window"]) | (j < s["sinks"]))
+    e = torch.matmul(q, keys).mul_(1.0 / math.sqrt(d)).reshape(b, hkv, hq // hkv, q_max, -1)
+    e = e.masked_fill_(~seen[:, None, None], -math.inf)
+    e = e.sub_(e.amax(-1, keepdim=True)).exp_()
+    e = e.div_(e.sum(-1, keepdim=True)).reshape(b, hkv, -1, keys.shape[3])
+    o = torch.matmul(e, vals).reshape(b, hq, q_max, d).transpose(1, 2)
+    return o[seq, row].to(x.dtype), stored[0], stored[1]
+
+
+# -------------------------------------------------------------------- calls
+
+def _own_norm(s):
+    from onnxsharp_amd.lm_layers import BlockNormLayer
+    layer = BlockNormLayer(eps=_EPS, residual_scale=s["a"], branch_scale=s["b"],
+                           gate_activation=None if s["act"] == "None" else s["act"])
+    return layer.forward(s["x"], s["gamma"], s["branch"], post_gamma=s["post_gamma"], gate=s["gates"])
+
+
+def _own_mm(s):
+    from onnxsharp_amd.lm_layers import Int4MatMulLayer
+    layer = Int4MatMulLayer(activation=None if s["act"] == "None" else s["act"])
+    return layer.forward(s["x"], s["w"], s["b"], s["r"])
+
+
+def _own_attn(s):
+    from onnxsharp_amd.lm_layers import WindowAttentionLayer
+    layer = WindowAttentionLayer(window=s["window"], sinks=s["sinks"])
+    # what the cache holds for the new tokens, as the values that its codes stand for
+    stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+    o = layer.forward(s["x"], s["k"], s["v"], s["cache"], s["cu"], s["kl"], max_q=s["q_max"], max_kv=s["kv_max"],
+                      stored=stored)
+    return o, stored[0], stored[1]
+
+
+def run(state):
+    kind = state["kind"]
+    if kind == "norm":
+        return _own_norm(state) if own else _plain_norm(state)
+    if kind == "mm":
+        return _own_mm(state) if own else _plain_mm(state)
+    return _own_attn(state) if own else _plain_attn(state)
+
+
+# --------------------------------------------------------------------- work
+
+def _pairs(ql, kl, window, sinks):
+    """Visible (query, key) pairs of one sequence, and the keys that any query sees."""
+    start = kl - ql
+    pairs = sum(min(p + 1, window) + min(sinks, max(0, p + 1 - window)) for p in range(start, kl))
+    first = max(0, start - window + 1)
+    return pairs, kl - first + min(sinks, first)
+
+
+def work(case):
+    e = _DT[case["dtype"]].itemsize
+    if case["kind"] == "norm":
+        n = case["rows"] * case["cols"]
+        return dict(bytes=n * (5 if case["gate"] == "rows" else 4) * e
+                    + case["cols"] * e * (1 + case["post"] + (case["gate"] == "cols")), flops=12.0 * n)
+    if case["kind"] == "mm":
+        m, n, k = case["m"], case["n"], case["k"]
+        groups = (k + case["group"] - 1) // case["group"]
+        return dict(bytes=m * k * e + n * ((k + 1) // 2) + n * groups * e + (n * ((groups + 1) // 2) if case["zeros"] else 0)
+                    + (4 * n if case["bias"] else 0) + m * n * e * (2 if case["res"] else 1), flops=2.0 * m * n * k)
+    ql, kl = _lens(case, 0)
+    both = [_pairs(x, y, case["window"], case["sinks"]) for x, y in zip(ql, kl)]
+    d = case["d"]
+    slot = d // 2 + d // case["group"] * 2 * e  # codes and scales of a head in K or V
+    # old keys are read; new ones are read, written in 4 bits and returned as stored
+    old = sum(k for _, k in both) - sum(ql)
+    return dict(bytes=2 * case["hkv"] * (old * slot + sum(ql) * (slot + 2 * e * d)) + 2 * e * d * case["hq"] * sum(ql),
+                flops=4.0 * d * case["hq"] * sum(p for p, _ in both))
+
+
+# ------------------------------------------------------- results in 64 bits
+
+def _codes64(packed):
+    return torch.stack((packed & 15, packed >> 4), -1).flatten(-2).double()
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["kind"] == "norm":
+        x, n = s["x"].double(), s["branch"].double()
+        if case["post"]:
+            n = n / (n.pow(2).sum(1, keepdim=True) / case["cols"] + _EPS).sqrt() * s["post_gamma"].double()
+        if s["gates"] is not None:
+            gate = s["gates"].double()
+            n = n * (torch.sigmoid(gate) if case["act"] == "Sigmoid" else gate)
+        h = (s["a"] * x + s["b"] * n).to(s["x"].dtype).double()
+        return h, h / (h.pow(2).sum(1, keepdim=True) / case["cols"] + _EPS).sqrt() * s["gamma"].double()
+    if case["kind"] == "mm":
+        k, group = case["k"], case["group"]
+        at = torch.arange(k, device="cuda") // group
+        zero = _codes64(s["zero"])[:, at] if case["zeros"] else 8.0
+        w = (_codes64(s["codes"])[:, :k] - zero) * s["scale"].double()[:, at]
+        y = s["x"].double() @ w.T
+        if s["b"] is not None:
+            y += s["b"].double()
+        if case["act"] == "Relu":
+            y = y.clamp(min=0)
+        elif case["act"] == "Silu":
+            y = y * torch.sigmoid(y)
+        elif case["act"] == "Gelu":
+            y = y * 0.5 * torch.erfc(-y / math.sqrt(2.0))
+        return y if s["r"] is None else y + s["r"].double()
+    # one sequence and one head of keys at a time, over its own tokens
+    group, d = case["group"], case["d"]
+    values = []
+    for new in (s["k"], s["v"]):
+        f = new.double().unflatten(-1, (-1, group))
+        lo = f.amin(-1, keepdim=True)
+        scale = ((f.amax(-1, keepdim=True) - lo) / 15).to(new.dtype).double()
+        values.append((lo + scale * ((f - lo) / scale).round().clamp(0, 15)).flatten(-2))
+    out = torch.empty(s["x"].shape, dtype=torch.float64, device="cuda")
+    ql, kl = _lens(case, int(seed) % (1 << 62))
+    groups, page, start = case["hq"] // case["hkv"], case["page"], 0
+    for i, (nq, nk) in enumerate(zip(ql, kl)):
+        at = torch.arange(nk, device="cuda")
+        pages, slots = s["table"][i, at // page].long(), at % page
+        p = at[nk - nq:, None]
+        hidden = (at > p) | ((at <= p - case["window"]) & (at >= case["sinks"]))
+        for h in range(case["hkv"]):
+            kv = []
+            for codes, scales, new in ((s["kp"], s["ks"], values[0]), (s["vp"], s["vs"], values[1])):
+                sc = scales[pages, slots, h].double()
+                v = (sc[..., 1:] + sc[..., :1] * _codes64(codes[pages, slots, h]).unflatten(-1, (-1, group))).flatten(-2)
+                v[nk - nq:] = new[start:start + nq, h]
+                kv.append(v)
+            for u in range(h * groups, (h + 1) * groups):
+                logits = s["x"][start:start + nq, u].double() @ kv[0].T / math.sqrt(d)
+                out[start:start + nq, u] = torch.softmax(logits.masked_fill(hidden, -math.inf), 1) @ kv[1]
+        start += nq
+    return out, values[0], values[1]
