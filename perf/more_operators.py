@@ -142,7 +142,8 @@ def _quantize_kv(v, group):
     group [..., d / group, 2] in v's type."""
     f = v.float().unflatten(-1, (-1, group))
     lo = f.amin(-1, keepdim=True)
-    scale = ((f.amax(-1, keepdim=True) - lo) / 15).to(v.dtype).float()
+    # a tensor's division is rounded once, one by a number may be a product with its reciprocal
+    scale = ((f.amax(-1, keepdim=True) - lo) / torch.full_like(lo, 15.0)).to(v.dtype).float()
     codes = torch.where(scale > 0, torch.round((f - lo) / scale), torch.zeros_like(f)).clamp(0, 15)
     return _two_a_byte(codes.flatten(-2)), torch.cat((scale, lo), -1).to(v.dtype)
 
@@ -392,11 +393,12 @@ def exact(case, seed):
     # one sequence and one head of keys at a time, over its own tokens
     group, d = case["group"], case["d"]
     values = []
-    for new in (s["k"], s["v"]):
-        f = new.double().unflatten(-1, (-1, group))
+    for new in (s["k"], s["v"]):  # scales and codes are defined in FP32, rounding by rounding
+        f = new.float().unflatten(-1, (-1, group))
         lo = f.amin(-1, keepdim=True)
-        scale = ((f.amax(-1, keepdim=True) - lo) / 15).to(new.dtype).double()
-        values.append((lo + scale * ((f - lo) / scale).round().clamp(0, 15)).flatten(-2))
+        scale = ((f.amax(-1, keepdim=True) - lo) / torch.full_like(lo, 15.0)).to(new.dtype)
+        codes = ((f - lo) / scale.float()).round().clamp(0, 15)
+        values.append((lo.double() + scale.double() * codes.double()).flatten(-2))
     out = torch.empty(s["x"].shape, dtype=torch.float64, device="cuda")
     ql, kl = _lens(case, int(seed) % (1 << 62))
     groups, page, start = case["hq"] // case["hkv"], case["page"], 0
