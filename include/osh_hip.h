@@ -618,6 +618,44 @@ OSH_API osh_status osh_quant_matmul(int m, int n, int k, int q_type, const void 
                                     const void *d_w, int64_t ldw, const float *d_sw, const float *d_bias, int act,
                                     int dtype, const void *d_res, int64_t ldr, void *d_y, int64_t ldy, osh_stream s);
 
+/* The norms after a block and before the next one, with the block's gate and the
+ * residual's scale between them, on rows [rows][cols] of type dtype (f32, f16, bf16; pitches
+ * in elements):
+ *   n = b / sqrt(mean(b^2) + eps) * post    (b itself when d_post is NULL)
+ *   h = round(alpha x + beta act(gate) n)   (without act(gate) when d_gate is NULL)
+ *   y = round(h / sqrt(mean(h^2) + eps) * gamma)
+ * Without a branch (d_b NULL; then neither d_post nor d_gate) h is x and d_h is not touched;
+ * without d_gamma only h is computed.  gate: one row for all (ldg 0) or [rows][cols];
+ * gate_act: none or sigmoid.  h may be x or b themselves; no other overlap of an output.
+ * Sums and what lies between two roundings are FP32, rows of any finite size; a NaN or an
+ * infinity in a row that is normed makes all of the norm NaN.  cols <= 32768; any alignment
+ * of whole elements. */
+OSH_API osh_status osh_block_norm(int64_t rows, int cols, int dtype, const void *d_x, int64_t ldx, float alpha,
+                                  const void *d_b, int64_t ldb, float beta, const void *d_post, const void *d_gate,
+                                  int64_t ldg, int gate_act, const void *d_gamma, float eps, void *d_h, int64_t ldh,
+                                  void *d_y, int64_t ldy, osh_stream s);
+
+/* Product with weights of 4 bits, y [m][n] of type dtype (f32, f16, bf16):
+ *   y[i][j] = act(sum_k a[i][k] (c[j][k] - z[j][k / group]) s[j][k / group] + bias[j]) + res[i][j]
+ * osh_int4_pack lays the weights out once: codes [n][ldc bytes], two a byte, the even k in
+ * the low half; scales [n][lds] of type dtype, one for each group of k (the last one may be
+ * cut short); zero points [n][ldz bytes], two groups a byte, or NULL for 8.  d_packed holds
+ * osh_int4_packed_bytes bytes at 16-byte alignment.
+ * a [m][lda] and res [m][ldr] of type dtype at any pitch and alignment of whole elements;
+ * bias FP32 and res may be NULL; act: none, relu, silu or gelu.  res may be y itself (same
+ * pitch); no other overlap of y.  group is 32, 64 or a multiple of 128.  The sums are FP32 and
+ * nothing is rounded before them. */
+OSH_API osh_status osh_int4_packed_bytes(int n, int k, int group, int dtype, int has_zeros, size_t *bytes);
+OSH_API osh_status osh_int4_pack(int n, int k, int group, int dtype, const void *d_codes, int64_t ldc,
+                                 const void *d_scales, int64_t lds, const void *d_zeros, int64_t ldz, void *d_packed,
+                                 osh_stream s);
+/* Scratch of osh_int4_matmul (0 where it needs none); depends on the sizes only. */
+OSH_API osh_status osh_int4_matmul_scratch_bytes(int m, int n, int k, int group, int dtype, size_t *bytes);
+OSH_API osh_status osh_int4_matmul(int m, int n, int k, int group, int dtype, const void *d_a, int64_t lda,
+                                   const void *d_packed, int has_zeros, const float *d_bias, int act,
+                                   const void *d_res, int64_t ldr, void *d_y, int64_t ldy, void *d_scratch,
+                                   osh_stream s);
+
 /* Causal attention with a sliding window and first tokens that stay visible
  * (sinks), over a paged cache.  Sequence b brings d_cu[b+1] - d_cu[b] new tokens
  * (rows d_cu[b].. of q, k_new, v_new and o) and holds d_kl[b] tokens with them.
@@ -668,6 +706,34 @@ typedef struct osh_window_attn {
  * sizes only.  d_scratch may be NULL when it is 0. */
 OSH_API osh_status osh_window_attention_scratch_bytes(const osh_window_attn *p, size_t *bytes);
 OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratch, osh_stream s);
+
+/* The same attention over a cache held in 4 bits.  A slot's head is cut into groups of
+ * `group` values (32, 64 or 128, a divisor of head_dim), each kept as codes 0..15 and a pair
+ * (scale, lo) of type dtype:
+ *   lo = min, scale = round((max - lo) / 15), code = rint((v - lo) / scale) within 0..15
+ *   (0 where scale is 0), in FP32; the cache stands for lo + scale * code.
+ * A group that holds a NaN or an infinity is kept as NaN.  Codes lie two a byte, the even
+ * value in the low half.
+ * The call quantizes the new keys and values into their pages and computes o as
+ * osh_window_attention does, with every key and value, the new ones too, as the cache
+ * stands for it: o depends on the cache alone, not on how its tokens came in calls.  A query
+ * that sees a key whose page id lies outside [0, pages) gets NaN, a new one too.
+ * d_k_stored and d_v_stored (both or neither NULL) receive what the cache stands for at
+ * the new tokens, rounded to dtype; rows that are not kept get NaN.
+ * `w` holds sizes, pointers and strides as above, with codes for k_pages and v_pages and
+ * their strides in bytes; head_dim % 32 == 0.  Codes of a head lie at a multiple of 16 bytes,
+ * its pairs at a multiple of 4.  Scales, codes and stored values share no memory with
+ * anything else. */
+typedef struct osh_kv4_attn {
+    osh_window_attn w;
+    int group, reserved;                                  /* 0 */
+    void *d_k_scales, *d_v_scales;                        /* pairs [head_dim / group][2] of a slot's head */
+    void *d_k_stored, *d_v_stored;                        /* [tokens][kv_heads][head_dim] */
+    int64_t k_scale_stride[3], v_scale_stride[3];         /* page, slot, head, in elements */
+    int64_t k_stored_stride[2], v_stored_stride[2];       /* token, head */
+} osh_kv4_attn;
+OSH_API osh_status osh_kv4_attention_scratch_bytes(const osh_kv4_attn *p, size_t *bytes);
+OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *p, void *d_scratch, osh_stream s);
 
 /* ----------------------------------------------------------- HIP graphs */
 /* A segment's launches recorded once and replayed per Forward, the role of

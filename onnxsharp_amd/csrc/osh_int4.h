@@ -1,0 +1,46 @@
+// osh_int4.h -- codes of 4 bits as the matrix instructions take them.
+#pragma once
+
+#include "osh_lm.h"
+
+namespace osh {
+
+template <typename T> struct Half8;
+template <> struct Half8<_Float16> { using type = f16x8; };
+template <> struct Half8<__bf16> { using type = bf16x8; };
+// FP32 rows are multiplied as three bf16 pieces
+template <> struct Half8<float> { using type = bf16x8; };
+
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The codes of a word, 0..15 each, as 16-bit floats: those at even places (0, 2, 4, 6),
+// then those at odd ones.  A byte 0..15 is code * 2^-9 as e4m3 (its subnormal numbers and
+// the first binade lie evenly), so that the hardware's conversion, two a time and at full
+// rate, does it: 7 instructions for 8 codes.
+__device__ __forceinline__ void codes8(unsigned w, f16x8 &v) {
+    const int b[2] = {(int)(w & 0x0f0f0f0fu), (int)(w >> 4 & 0x0f0f0f0fu)};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const f16x2 p = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b[h], 512.0f, false));
+        const f16x2 q = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b[h], 512.0f, true));
+        v[4 * h] = p[0], v[4 * h + 1] = p[1], v[4 * h + 2] = q[0], v[4 * h + 3] = q[1];
+    }
+}
+__device__ __forceinline__ void codes8(unsigned w, bf16x8 &v) {
+    const int b[2] = {(int)(w & 0x0f0f0f0fu), (int)(w >> 4 & 0x0f0f0f0fu)};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 p = __builtin_bit_cast(bf16x2, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[h], 512.0f, false));
+        const bf16x2 q = __builtin_bit_cast(bf16x2, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[h], 512.0f, true));
+        v[4 * h] = p[0], v[4 * h + 1] = p[1], v[4 * h + 2] = q[0], v[4 * h + 3] = q[1];
+    }
+}
+
+}  // namespace osh

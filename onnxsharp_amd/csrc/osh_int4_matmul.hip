@@ -1,0 +1,372 @@
+// osh_int4_matmul.hip -- product with weights of 4 bits and group scales:
+//
+//   y[i][j] = act(sum_k a[i][k] (c[j][k] - z[j][k / group]) s[j][k / group] + bias[j]) + res[i][j]
+//
+// The weights are laid out once (osh_int4_pack): blocks of 16 outputs by 128 k, in a block
+// 16 bytes for each lane (jl, g) of a wave, in which word t holds output jl, k 32 t + 8 g ..
+// + 7, as the 16x16x32 MFMA takes its A operand.  A wave's load of a block is 1 KB in a row.
+//
+// The MFMAs multiply the codes, which are exact in 16 bits, and add c - z over a group in
+// FP32: sum a c - z sum a, the second sum by an MFMA whose A operand is the constant -8
+// or -1.  A group's sum is scaled once, in FP32.  So nothing is rounded between the operands
+// and the FP32 sums.  FP32 rows are taken as three bf16 pieces (8 + 8 + 8 bits of 24).
+#include <limits.h>
+
+#include <algorithm>
+
+#include "osh_int4.h"
+#include "osh_overlap.h"
+
+using namespace osh;
+
+namespace osh {
+
+struct Int4Args {
+    int m, n, k, act;
+    long long lda, ldr, ldy;
+    const void *a;
+    const uint4 *codes;  // [n / 16][k / 128][64]
+    const void *scales;  // [n / 16][k / 128][groups of a block][16]
+    const void *zeros;   // the same, or NULL: 8
+    const float *bias;
+    const void *res;
+    void *y;
+};
+
+constexpr int KB = 128;  // k of a block
+
+// The pieces of 8 neighbouring values of a row from k0 on, zero from k on.
+template <typename T> constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type load_row8(const T *row, int k0, int k) {
+    typename Vec8<T>::type v = {};
+    if (k0 + 8 <= k) {
+        __builtin_memcpy(&v, row + k0, sizeof(v));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+            if (k0 + i < k) v[i] = row[k0 + i];
+    }
+    return v;
+}
+template <typename T, typename H8>
+__device__ __forceinline__ void split_row8(const typename Vec8<T>::type &v, H8 (&p)[PIECES<T>]) {
+    if constexpr (sizeof(T) == 2) {
+        p[0] = v;
+    } else {
+        // the upper 16 bits of what is left, three times: exact, an infinity apart, whose
+        // rest is not taken
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float rest = v[i];
+#pragma unroll
+            for (int e = 0; e < 3; e++) {
+                unsigned top = __float_as_uint(rest) & 0xffff0000u;
+                if (e == 0 && rest != rest) top |= 0x00400000u;  // stays a NaN
+                p[e][i] = __builtin_bit_cast(__bf16, (unsigned short)(top >> 16));
+                rest -= __uint_as_float(top);
+                if (e == 0 && (top & 0x7f800000u) == 0x7f800000u) rest = 0.0f;
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T int4_finish(const Int4Args &p, float v, int row, int col) {
+    if (p.bias) v += p.bias[col];
+    v = apply_act<sizeof(T) == 4>(p.act, v);
+    if (p.res) v += (float)static_cast<const T *>(p.res)[row * p.ldr + col];
+    return (T)v;
+}
+
+// Few rows: a workgroup takes 16 NB outputs of 16 MB rows, its waves every WAVES-th block
+// of k; the weights go from memory to registers, each byte once.  GS steps of 32 k share a
+// scale.  The waves' sums meet in LDS, in the order of the waves.
+template <typename T, int MB, int NB, int GS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
+    using H8 = typename Half8<T>::type;
+    using V = typename Vec8<T>::type;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr int P = PIECES<T>, NG = 4 / GS;
+    __shared__ f32x4 part[WAVES][MB * NB][64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jl = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * (16 * NB), m0 = blockIdx.y * (16 * MB);
+    const int nkb = cdiv(p.k, KB), whole = p.k / KB;
+    const T *a[MB];
+    long long blk[NB];
+    f32x4 acc[MB][NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) blk[j] = (long long)min(n0 / 16 + j, cdiv(p.n, 16) - 1) * nkb;
+#pragma unroll
+    for (int i = 0; i < MB; i++) {
+        a[i] = static_cast<const T *>(p.a) + (long long)min(m0 + 16 * i + jl, p.m - 1) * p.lda + 8 * g;
+#pragma unroll
+        for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+    }
+    H8 minus;  // sum a times it, in every row of a fragment
+#pragma unroll
+    for (int e = 0; e < 8; e++) minus[e] = p.zeros ? -1.0f : -8.0f;
+
+    auto block = [&](int kb, auto cut) {
+        uint4 w[NB];
+        T4 sc[NB][NG], zp[NB][NG];
+        V x[MB][4];
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            w[j] = p.codes[(blk[j] + kb) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < NG; e++) {
+                const long long at = ((blk[j] + kb) * NG + e) * 16 + 4 * g;
+                sc[j][e] = *reinterpret_cast<const T4 *>(static_cast<const T *>(p.scales) + at);
+                if (p.zeros) zp[j][e] = *reinterpret_cast<const T4 *>(static_cast<const T *>(p.zeros) + at);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                if constexpr (decltype(cut)::value) x[i][t] = load_row8<T>(a[i] - 8 * g, kb * KB + 32 * t + 8 * g, p.k);
+                else __builtin_memcpy(&x[i][t], a[i] + kb * KB + 32 * t, sizeof(V));
+            }
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            H8 xs[MB][GS][P];
+            f32x4 less[MB];
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                less[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < GS; t++) {
+                    split_row8<T>(x[i][e * GS + t], xs[i][t]);
+#pragma unroll
+                    for (int q = 0; q < P; q++) less[i] = mma16(minus, xs[i][t][q], less[i]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                f32x4 sum[MB];
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sum[i][r] = p.zeros ? less[i][r] * (float)zp[j][e][r] : less[i][r];
+#pragma unroll
+                for (int t = 0; t < GS; t++) {
+                    H8 c;
+                    codes8(reinterpret_cast<const unsigned *>(&w[j])[e * GS + t], c);
+#pragma unroll
+                    for (int i = 0; i < MB; i++)
+#pragma unroll
+                        for (int q = 0; q < P; q++) sum[i] = mma16(c, xs[i][t][q], sum[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf((float)sc[j][e][r], sum[i][r], acc[i][j][r]);
+            }
+        }
+    };
+    int kb = wave;
+    for (; kb < whole; kb += WAVES) block(kb, IntC<0>{});
+    if (kb < nkb) block(kb, IntC<1>{});
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++) part[wave][i * NB + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int e = tid; e < MB * NB * 256; e += 64 * WAVES) {
+        // neighbouring threads, neighbouring outputs
+        const int c = e % (16 * NB), r16 = e / (16 * NB), col = n0 + c, row = m0 + r16;
+        const int f = r16 / 16 * NB + c / 16, from = r16 % 16 + 16 * (c / 4 % 4), r = c % 4;
+        float sum = part[0][f][from][r];
+#pragma unroll
+        for (int v = 1; v < WAVES; v++) sum += part[v][f][from][r];
+        if (row < p.m && col < p.n) static_cast<T *>(p.y)[row * p.ldy + col] = int4_finish<T>(p, sum, row, col);
+    }
+}
+
+// Codes [n][pitch] two a byte into blocks; codes past n or k are 0 (their scales and the
+// values that meet them are 0).
+__global__ __launch_bounds__(256) void int4_pack_codes_kernel(int n, int k, const unsigned char *codes, long long pitch,
+                                                              uint4 *out) {
+    const int nkb = cdiv(k, KB);
+    const long long blocks = (long long)cdiv(n, 16) * nkb;
+    for (long long e = blockIdx.x * 256LL + threadIdx.x; e < blocks * 64; e += gridDim.x * 256LL) {
+        const int lane = (int)(e & 63), jl = lane & 15, g = lane >> 4;
+        const long long blk = e >> 6;
+        const long long row = blk / nkb * 16 + jl;
+        const int k0 = (int)(blk % nkb) * KB;
+        unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int at = k0 + 32 * t + 8 * g + i;
+                if (row >= n || at >= k) continue;
+                const unsigned code = codes[row * pitch + at / 2] >> (4 * (at & 1)) & 15u;
+                w[t] |= code << (4 * (2 * (i & 3) + (i >> 2)));  // 0..3 at even places, 4..7 at odd ones
+            }
+        out[e] = uint4{w[0], w[1], w[2], w[3]};
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void int4_pack_scales_kernel(int n, int k, int group, const T *scales,
+                                                               long long lds, const unsigned char *zeros,
+                                                               long long ldz, T *out_s, T *out_z) {
+    const int per = group < KB ? KB / group : 1, nkb = cdiv(k, KB);
+    const long long total = (long long)cdiv(n, 16) * nkb * per * 16;
+    for (long long e = blockIdx.x * 256LL + threadIdx.x; e < total; e += gridDim.x * 256LL) {
+        const long long blk = e / (16 * per), row = blk / nkb * 16 + e % 16;
+        const long long at = (blk % nkb) * KB + e / 16 % per * (KB / per);
+        const bool in = row < n && at < k;
+        const long long gr = at / group;
+        out_s[e] = in ? scales[row * lds + gr] : (T)0.0f;
+        if (zeros) out_z[e] = in ? (T)(float)(zeros[row * ldz + gr / 2] >> (4 * (gr & 1)) & 15u) : (T)0.0f;
+    }
+}
+
+struct Int4Layout {
+    size_t codes, scales, total;
+};
+static Int4Layout int4_layout(int n, int k, int group, int dtype, bool zeros) {
+    const size_t blocks = (size_t)cdiv(n, 16) * cdiv(k, KB);
+    Int4Layout l;
+    l.codes = blocks * 1024;
+    l.scales = blocks * (group < KB ? KB / group : 1) * 16 * elem_bytes(dtype);
+    l.total = l.codes + l.scales * (zeros ? 2 : 1);
+    return l;
+}
+
+template <typename T, int GS>
+static osh_status int4_launch(const Int4Args &p, hipStream_t st) {
+#define OSH_INT4_ROWS(MB, NB)                                                                                  \
+    OSH_LAUNCH((int4_rows_kernel<T, MB, NB, GS, 8>), dim3((unsigned)cdiv(p.n, 16 * NB), (unsigned)cdiv(p.m, 16 * MB)), \
+               dim3(512), 0, st, p)
+    if (p.m <= 16) OSH_INT4_ROWS(1, 1);
+    else if (p.m <= 32) OSH_INT4_ROWS(2, 1);
+    else OSH_INT4_ROWS(4, 1);
+#undef OSH_INT4_ROWS
+    OSH_LAUNCH_CHECK("int4 kernel");
+    return OSH_OK;
+}
+
+template <typename T>
+static osh_status int4_launch_t(const Int4Args &p, int group, hipStream_t st) {
+    if (group == 32) return int4_launch<T, 1>(p, st);
+    if (group == 64) return int4_launch<T, 2>(p, st);
+    return int4_launch<T, 4>(p, st);
+}
+
+static size_t int4_scratch(int m, int n, int k, int dtype) { return 0; }
+
+static osh_status int4_check(int n, int k, int group, int dtype) {
+    if (n < 0 || k < 0) return fail(OSH_E_INVALID, "Int4MatMul: negative sizes");
+    if (dtype != OSH_T_F32 && dtype != OSH_T_F16 && dtype != OSH_T_BF16)
+        return fail(OSH_E_INVALID, "Int4MatMul: rows and scales are f32, f16 or bf16");
+    if (group < 1) return fail(OSH_E_INVALID, "Int4MatMul: groups of %d", group);
+    if (group != 32 && group != 64 && group % KB)
+        return fail(OSH_E_UNSUPPORTED, "Int4MatMul: groups of %d (32, 64 or a multiple of 128)", group);
+    if (n > 0 && k == 0) return fail(OSH_E_INVALID, "Int4MatMul: k is 0");
+    if (k > (1 << 28) || n > (1 << 28)) return fail(OSH_E_UNSUPPORTED, "Int4MatMul: %d x %d weights", n, k);
+    return OSH_OK;
+}
+
+}  // namespace osh
+
+extern "C" {
+
+OSH_API osh_status osh_int4_packed_bytes(int n, int k, int group, int dtype, int has_zeros, size_t *bytes) {
+    if (!bytes) return fail(OSH_E_INVALID, "Int4MatMul: NULL bytes");
+    if (const osh_status st = int4_check(n, k, group, dtype)) return st;
+    *bytes = n ? int4_layout(n, k, group, dtype, has_zeros).total : 0;
+    return OSH_OK;
+}
+
+OSH_API osh_status osh_int4_pack(int n, int k, int group, int dtype, const void *d_codes, int64_t ldc,
+                                 const void *d_scales, int64_t lds, const void *d_zeros, int64_t ldz, void *d_packed,
+                                 osh_stream s) {
+    if (const osh_status st = int4_check(n, k, group, dtype)) return st;
+    if (n == 0) return OSH_OK;
+    if (!d_codes || !d_scales || !d_packed) return fail(OSH_E_INVALID, "Int4MatMul: NULL pointer");
+    const long long groups = cdiv(k, group), e = elem_bytes(dtype);
+    if (ldc < cdiv(k, 2) || lds < groups || (d_zeros && ldz < (groups + 1) / 2))
+        return fail(OSH_E_INVALID, "Int4MatMul: a row pitch below the columns");
+    if ((uintptr_t)d_packed & 15) return fail(OSH_E_INVALID, "Int4MatMul: packed weights need 16-byte alignment");
+    const Int4Layout l = int4_layout(n, k, group, dtype, d_zeros);
+    const Strided out(d_packed, l.total);
+    if (share_bytes(out, strided_rows(d_codes, n, ldc, cdiv(k, 2))) ||
+        share_bytes(out, strided_rows(d_scales, n, lds * e, groups * e)) ||
+        share_bytes(out, strided_rows(d_zeros, n, ldz, (groups + 1) / 2)))
+        return fail(OSH_E_INVALID, "Int4MatMul: the packed weights overlap an operand");
+    const hipStream_t st = to_stream(s);
+    auto grid = [](size_t threads) { return dim3((unsigned)std::min<size_t>((threads + 255) / 256, 1 << 16)); };
+    OSH_LAUNCH(int4_pack_codes_kernel, grid(l.codes / 16), dim3(256), 0, st, n, k,
+               static_cast<const unsigned char *>(d_codes), (long long)ldc, static_cast<uint4 *>(d_packed));
+    OSH_LAUNCH_CHECK("int4_pack_codes_kernel");
+    char *sc = static_cast<char *>(d_packed) + l.codes, *zp = sc + l.scales;
+    const unsigned char *z = static_cast<const unsigned char *>(d_zeros);
+#define OSH_PACK(T)                                                                                              \
+    OSH_LAUNCH(int4_pack_scales_kernel<T>, grid(l.scales / sizeof(T)), dim3(256), 0, st, n, k, group,            \
+               static_cast<const T *>(d_scales), (long long)lds, z, (long long)ldz, reinterpret_cast<T *>(sc),   \
+               reinterpret_cast<T *>(zp))
+    if (dtype == OSH_T_F32) OSH_PACK(float);
+    else if (dtype == OSH_T_F16) OSH_PACK(_Float16);
+    else OSH_PACK(__bf16);
+#undef OSH_PACK
+    OSH_LAUNCH_CHECK("int4_pack_scales_kernel");
+    return OSH_OK;
+}
+
+OSH_API osh_status osh_int4_matmul_scratch_bytes(int m, int n, int k, int group, int dtype, size_t *bytes) {
+    if (!bytes) return fail(OSH_E_INVALID, "Int4MatMul: NULL bytes");
+    if (m < 0) return fail(OSH_E_INVALID, "Int4MatMul: negative sizes");
+    if (const osh_status st = int4_check(n, k, group, dtype)) return st;
+    *bytes = int4_scratch(m, n, k, dtype);
+    return OSH_OK;
+}
+
+OSH_API osh_status osh_int4_matmul(int m, int n, int k, int group, int dtype, const void *d_a, int64_t lda,
+                                   const void *d_packed, int has_zeros, const float *d_bias, int act,
+                                   const void *d_res, int64_t ldr, void *d_y, int64_t ldy, void *d_scratch,
+                                   osh_stream s) {
+    if (m < 0) return fail(OSH_E_INVALID, "Int4MatMul: negative sizes");
+    if (const osh_status st = int4_check(n, k, group, dtype)) return st;
+    if (act != OSH_ACT_NONE && act != OSH_ACT_RELU && act != OSH_ACT_SILU && act != OSH_ACT_GELU)
+        return fail(OSH_E_INVALID, "Int4MatMul: unknown activation %d", act);
+    if (m == 0 || n == 0) return OSH_OK;
+    if (!d_a || !d_packed || !d_y) return fail(OSH_E_INVALID, "Int4MatMul: NULL pointer");
+    if (lda < k || ldy < n || (d_res && ldr < n)) return fail(OSH_E_INVALID, "Int4MatMul: a row pitch below the columns");
+    if ((uintptr_t)d_packed & 15) return fail(OSH_E_INVALID, "Int4MatMul: packed weights need 16-byte alignment");
+    if ((long long)cdiv(m, 64) * cdiv(n, 64) >= (1LL << 23) || m > 64 * 65535)
+        return fail(OSH_E_UNSUPPORTED, "Int4MatMul: %d x %d outputs", m, n);
+    const long long e = elem_bytes(dtype);
+    const Int4Layout l = int4_layout(n, k, group, dtype, has_zeros);
+    const size_t scratch = int4_scratch(m, n, k, dtype);
+    if (scratch && !d_scratch) return fail(OSH_E_INVALID, "Int4MatMul: NULL pointer");
+    const Strided y = strided_rows(d_y, m, ldy * e, n * e), res = strided_rows(d_res, m, ldr * e, n * e);
+    if (share_bytes(y, strided_rows(d_a, m, lda * e, k * e)) || share_bytes(y, Strided(d_packed, l.total)) ||
+        share_bytes(y, Strided(d_bias, n * 4LL)) || (share_bytes(y, res) && !(d_y == d_res && ldy == ldr)))
+        return fail(OSH_E_INVALID, "Int4MatMul: y overlaps an operand");
+    Int4Args p;
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.act = act;
+    p.lda = lda;
+    p.ldr = ldr;
+    p.ldy = ldy;
+    p.a = d_a;
+    const char *base = static_cast<const char *>(d_packed);
+    p.codes = reinterpret_cast<const uint4 *>(base);
+    p.scales = base + l.codes;
+    p.zeros = has_zeros ? base + l.codes + l.scales : nullptr;
+    p.bias = d_bias;
+    p.res = d_res;
+    p.y = d_y;
+    if (dtype == OSH_T_F32) return int4_launch_t<float>(p, group, to_stream(s));
+    if (dtype == OSH_T_F16) return int4_launch_t<_Float16>(p, group, to_stream(s));
+    return int4_launch_t<__bf16>(p, group, to_stream(s));
+}
+
+}  // extern "C"

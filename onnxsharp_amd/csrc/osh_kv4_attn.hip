@@ -1,0 +1,663 @@
+// osh_kv4_attn.hip -- the attention of osh_window_attn.hip over a paged cache held in 4
+// bits (osh_kv4_attention): a group of a head's values is lo + scale * code.
+//
+// The products take the codes, which are exact in 16 bits; scales and minima stay in FP32:
+//   q . k_j = sum over groups of scale_j (q . code_j) + lo_j (sum of q over the group),
+//   sum_j p_j v_j = sum_j (p_j scale_j) (code_j - 8) + sum_j p_j (lo_j + 8 scale_j).
+// Rounded are the weights p_j scale_j alone, half a step of dtype each as the weights are
+// over a 16-bit cache; codes less 8 have the size of the values about the group's middle, so
+// that the roundings weigh what they weigh there.  (8 is taken off the sums by a product
+// with the constant -8.)
+#include <limits.h>
+
+#include "osh_overlap.h"
+#include "osh_window.h"
+
+using namespace osh;
+
+namespace osh {
+
+struct Kv4Args {
+    WinArgs w;
+    const void *ks, *vs;  // scale pairs
+    void *k_stored, *v_stored;
+    long long ks_stride[3], vs_stride[3], k_stored_stride[2], v_stored_stride[2];
+    unsigned page_mul, page_log;  // j / page = umulhi(4 j, page_mul) >> page_log for j < 2^30
+};
+
+// -------------------------------------------------------------- quantization
+
+// Eight neighbouring values a lane, the 4, 8 or 16 lanes of a group next to each other.
+// blockIdx.y is the sequence.
+template <typename T, int GL>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
+    const osh_window_attn &p = a.w.p;
+    const int b = blockIdx.y, chunks = p.head_dim / 8;
+    const WinSeq sq = win_seq(p, b);
+    const long long total = (long long)sq.held * p.kv_heads * 2 * chunks;
+    for (long long e0 = blockIdx.x * 256LL; e0 < total; e0 += gridDim.x * 256LL) {
+        const long long e = e0 + threadIdx.x;
+        const bool in = e < total;
+        const long long item = in ? e / chunks : 0;
+        const int c = in ? (int)(e - item * chunks) : 0;
+        const bool is_v = item & 1;
+        const int h = (int)(item / 2 % p.kv_heads);
+        const long long t = item / 2 / p.kv_heads, row = sq.c0 + t;
+        const T *src = static_cast<const T *>(is_v ? p.d_v_new : p.d_k_new);
+        const int64_t *st = is_v ? p.v_new_stride : p.k_new_stride;
+        f32x8 f = {};
+        if (in) f = load8(src + row * st[0] + h * st[1] + 8 * c);
+        // NaN and infinities are above and below everything, as integers of the floats' order
+        float lo = f[0], hi = f[0];
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            lo = __builtin_fminf(lo, f[i]), hi = __builtin_fmaxf(hi, f[i]);
+            finite &= (__float_as_uint(f[i]) & 0x7f800000u) != 0x7f800000u;
+        }
+        int bad = !finite;
+#pragma unroll
+        for (int o = 1; o < GL; o <<= 1) {
+            lo = __builtin_fminf(lo, __shfl_xor(lo, o));
+            hi = __builtin_fmaxf(hi, __shfl_xor(hi, o));
+            bad |= __shfl_xor(bad, o);
+        }
+        T scale = (T)((hi - lo) / 15.0f), low = (T)lo;
+        if (bad || !(hi - lo < __builtin_inff())) scale = low = (T)__builtin_nanf("");
+        const float s = (float)scale, l = (float)low;
+        unsigned word = 0;
+        f32x8 kept;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float q = s > 0.0f ? __builtin_rintf((f[i] - l) / s) : 0.0f;
+            q = __builtin_fminf(__builtin_fmaxf(q, 0.0f), 15.0f);
+            word |= (unsigned)(int)q << (4 * i);
+            kept[i] = __builtin_fmaf(s, q, l);
+        }
+        if (!in) continue;
+        // where it is kept; a sequence of contradicting lengths is not
+        long long at = -1;
+        const int64_t *cst = is_v ? p.v_stride : p.k_stride;
+        const long long *sst = is_v ? a.vs_stride : a.ks_stride;
+        if (sq.ok) {
+            const int j = sq.past + (int)t, pg = p.d_table[b * p.table_stride + j / p.page], slot = j % p.page;
+            if ((unsigned)pg < (unsigned)p.pages) {
+                at = pg * (long long)cst[0] + (long long)slot * cst[1] + (long long)h * cst[2];
+                unsigned char *codes = static_cast<unsigned char *>(is_v ? p.d_v_pages : p.d_k_pages);
+                *reinterpret_cast<unsigned *>(codes + at + 4 * c) = word;
+                if (c % GL == 0) {
+                    T pair[2] = {scale, low};
+                    T *to = const_cast<T *>(static_cast<const T *>(is_v ? a.vs : a.ks)) + pg * sst[0] + slot * sst[1] +
+                            h * sst[2] + c / GL * 2;
+                    __builtin_memcpy(__builtin_assume_aligned(to, 4), pair, 4);
+                }
+            }
+        }
+        if (T *out = static_cast<T *>(is_v ? a.v_stored : a.k_stored)) {
+            const long long *ost = is_v ? a.v_stored_stride : a.k_stored_stride;
+            if (at < 0) kept = f32x8{} + __builtin_nanf("");
+            store8(out + row * ost[0] + h * ost[1] + 8 * c, kept);
+        }
+    }
+}
+
+// ----------------------------------------------------------------- few rows
+
+// One workgroup: 16 query rows of one key head, one split of their keys; each wave takes
+// every WAVES-th step of 64 keys of the split.
+//
+// S^T = K Q^T: MFMA row rho of block b is key 16 (rho / 4) + 4 b + rho % 4 of the step, so
+// that lane (jl, g) ends with the scores of keys 16 g .. + 15 at query jl, just the operand
+// of O^T = V^T P^T.  Codes pass through the wave's own LDS, loaded directly, CP chunks of 16
+// bytes a key; K's words are read as they lie, V's by the LDS read that transposes 4-bit
+// elements: 16 keys of one value a lane.
+//
+// The next step's codes are loaded while this one is computed.
+// At most N loads in flight.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ unsigned lds_offset(const void *p) {
+    return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+// 8 bytes to LDS.  By hand: in front of an LDS write of its own the compiler waits for all
+// direct loads in flight.  The caller waits for lgkmcnt before it reads.
+__device__ __forceinline__ void write_pair(const float2 *to, float2 v) {
+    asm volatile("ds_write_b64 %0, %1" ::"v"(lds_offset(to)), "v"(v) : "memory");
+}
+
+// Both halves of two or four chunks, transposed among the 16 lanes of a group: a lane's 8
+// bytes at a chunk's half become 16 rows' codes of one column.  By hand for the same reason,
+// with the wait.
+__device__ __forceinline__ void read_transposed4(const void *a, const void *b, unsigned (*to)[2]) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 r[4];
+    asm volatile("ds_read_b64_tr_b4 %0, %4\n\tds_read_b64_tr_b4 %1, %4 offset:8\n\t"
+                 "ds_read_b64_tr_b4 %2, %5\n\tds_read_b64_tr_b4 %3, %5 offset:8\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+                 : "v"(lds_offset(a)), "v"(lds_offset(b))
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; i++) to[i][0] = r[i][0], to[i][1] = r[i][1];
+}
+__device__ __forceinline__ void read_transposed8(const void *a, const void *b, const void *c, const void *d,
+                                                 unsigned (*to)[2]) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 r[8];
+    asm volatile("ds_read_b64_tr_b4 %0, %8\n\tds_read_b64_tr_b4 %1, %8 offset:8\n\t"
+                 "ds_read_b64_tr_b4 %2, %9\n\tds_read_b64_tr_b4 %3, %9 offset:8\n\t"
+                 "ds_read_b64_tr_b4 %4, %10\n\tds_read_b64_tr_b4 %5, %10 offset:8\n\t"
+                 "ds_read_b64_tr_b4 %6, %11\n\tds_read_b64_tr_b4 %7, %11 offset:8\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                 : "v"(lds_offset(a)), "v"(lds_offset(b)), "v"(lds_offset(c)), "v"(lds_offset(d))
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; i++) to[i][0] = r[i][0], to[i][1] = r[i][1];
+}
+// Two words: at a read of a struct the compiler waits too.
+__device__ __forceinline__ float2 read_pair(const float2 *from) {
+    const unsigned *u = reinterpret_cast<const unsigned *>(from);
+    return float2{__uint_as_float(u[0]), __uint_as_float(u[1])};
+}
+
+template <typename T, int CP, int GS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv4Args args) {
+    constexpr int NG = CP / GS;        // groups of a head
+    constexpr int DP = 32 * CP, OB = 2 * CP, KPI = 64 / CP;
+    constexpr int TILE = 64 * CP * 16;
+    using H8 = typename Half8<T>::type;
+    extern __shared__ __align__(16) unsigned char lds[];
+    constexpr int WAVE_LDS = 4 * TILE + 256 + 2 * NG * (256 + 512);
+    const WinArgs &a = args.w;
+    const osh_window_attn &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int jl = lane & 15, g = lane >> 4;
+    const int d = p.head_dim, G = a.group;
+
+    int id = blockIdx.x;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int unit = id;
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int h = id % p.kv_heads, b = id / p.kv_heads;
+    const WinSeq sq = win_seq(p, b);
+    const int rows = sq.ql * G, r0 = tile * 16;
+    if (!sq.ok) {
+        if (tile == 0 && split == 0) win_fill_nan<T>(p, sq, h, G, tid, 64 * WAVES);
+        return;
+    }
+    if (r0 >= rows) return;
+    T *o = static_cast<T *>(p.d_o);
+    const int my_row = min(r0 + jl, rows - 1), my_tok = my_row / G, my_head = h * G + my_row % G;
+
+    // queries: lane (jl, g) holds values 32 s + 8 g + {0, 2, 4, 6, 1, 3, 5, 7} of row jl,
+    // the order of codes8, and their sums over a group
+    H8 q[CP];
+    float qs[NG];
+    {
+        const T *qr = static_cast<const T *>(p.d_q) + (long long)(sq.c0 + my_tok) * p.q_stride[0] +
+                      my_head * p.q_stride[1];
+#pragma unroll
+        for (int e = 0; e < NG; e++) qs[e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < CP; s++) {
+            H8 x = {};
+            if (32 * s < d) __builtin_memcpy(&x, qr + 32 * s + 8 * g, 16);
+#pragma unroll
+            for (int i = 0; i < 8; i++) qs[s / GS] += (float)x[i];
+            q[s] = __builtin_shufflevector(x, x, 0, 2, 4, 6, 1, 3, 5, 7);
+        }
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            qs[e] += __shfl_xor(qs[e], 16);
+            qs[e] += __shfl_xor(qs[e], 32);
+        }
+    }
+    const int tok0 = r0 / G, tok1 = min(r0 + 15, rows - 1) / G;
+    const WinKeys keys = win_keys(p, sq, tok0, tok1);
+    const int nv = keys.count;
+    const int steps = cdiv(nv, 64), per = cdiv(steps, a.splits);
+    const int s_end = min(steps, (split + 1) * per);
+    const int pos0 = sq.past + tok0, pos1 = sq.past + tok1;
+    // by key number, this row sees v <= v_hi with v >= v_lo or v < v_sink
+    const int shift = keys.sink_end - keys.lo, my_pos = sq.past + my_tok;
+    const int v_sink = max(keys.sink_end, win_min(p.sinks, 1 << 30) + shift);
+    const int v_hi = my_pos + shift, v_lo = max(my_pos - p.window + 1, keys.lo) + shift;
+
+    float m = -__builtin_inff(), l = 0.0f, zsum[NG];
+    f32x4 acc[OB], accz[NG];
+#pragma unroll
+    for (int i = 0; i < OB; i++) acc[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < NG; e++) accz[e] = f32x4{0, 0, 0, 0}, zsum[e] = 0.0f;
+    // f16 weights: times 1 / unit, a power of two that keeps p scale / unit within 1, since
+    // f16 has no room for the scales' own range
+    constexpr bool UNIT = sizeof(H8) && __is_same(T, _Float16);
+    float unit_scale = 0x1p-100f;
+    H8 minus8;
+#pragma unroll
+    for (int i = 0; i < 8; i++) minus8[i] = -8.0f;
+
+    unsigned char *mine = lds + wave * WAVE_LDS;
+    const float2 *kpair = reinterpret_cast<const float2 *>(mine + 4 * TILE + 256 + 2 * NG * 256), *vpair = kpair + NG * 64;
+    auto k_swizzle = [](int key) { return CP == 8 ? (key >> 4 & 3) | (key >> 1 & 1) << 2 : key >> 4 & (CP - 1); };
+    auto v_swizzle = [](int key) { return key >> 2 & (CP - 1); };
+
+    // Everything a step reads goes to LDS directly: page ids two steps ahead, codes and scale
+    // pairs one.  Always for a key that there is (past the last key its own again), so that no
+    // load stands under a condition and the waits, which are written by hand, can count them:
+    // loads return in order.
+    unsigned char *raw_ids = mine + 4 * TILE, *raw_sc = raw_ids + 256;
+    unsigned long long k_row, v_row, k_sc, v_sc;  // of key `lane` of the next step
+    bool in = false, bad = false;
+    auto position = [&](int st) { return keys.at(min(st * 64 + lane, nv - 1)); };
+    auto page_of = [&](int j) { return (int)(__umulhi((unsigned)j << 2, args.page_mul) >> args.page_log); };
+    auto load_ids = [&](int st) {
+        copy_to_lds<4>(p.d_table + (b * p.table_stride + page_of(position(st))), raw_ids);
+        __builtin_amdgcn_sched_barrier(0);  // stays in front of the codes
+    };
+    auto place = [&](int st) {
+        int page_id = reinterpret_cast<const int *>(raw_ids)[lane];
+        // in a register before the next ids are on their way: those of a table that the L1
+        // holds arrive before a read that waits in a busy LDS
+        asm volatile("" : "+v"(page_id)::"memory");
+        const int j = position(st), slot = j - page_of(j) * p.page;
+        in = st * 64 + lane < nv;
+        bad = (unsigned)page_id >= (unsigned)p.pages;
+        const unsigned long long zero = (unsigned long long)win_zero_row;
+        auto where = [&](const void *base, int e, long long s0, long long s1, long long s2) {
+            const unsigned long long at = (unsigned long long)base + e * (h * s2) +
+                                          (unsigned long long)(unsigned)page_id * (unsigned)(e * s0) +
+                                          (unsigned long long)(unsigned)slot * (unsigned)(e * s1);
+            return bad ? zero : at;
+        };
+        k_row = where(p.d_k_pages, 1, p.k_stride[0], p.k_stride[1], p.k_stride[2]);
+        v_row = where(p.d_v_pages, 1, p.v_stride[0], p.v_stride[1], p.v_stride[2]);
+        k_sc = where(args.ks, 2, args.ks_stride[0], args.ks_stride[1], args.ks_stride[2]);
+        v_sc = where(args.vs, 2, args.vs_stride[0], args.vs_stride[1], args.vs_stride[2]);
+    };
+    const int last_chunk = d / 32 - 1;  // slots of no value hold a copy of it, and meet queries of 0
+    auto load_codes = [&](int buf) {
+        unsigned char *kt = mine + buf * 2 * TILE, *vt = kt + TILE;
+#pragma unroll
+        for (int i = 0; i < CP; i++) {
+            const int key = i * KPI + lane / CP, slot = lane % CP;
+            copy_to_lds<16>((const char *)__shfl(k_row, key) + 16 * min(slot ^ k_swizzle(key), last_chunk), kt + i * 1024);
+            copy_to_lds<16>((const char *)__shfl(v_row, key) + 16 * min(slot ^ v_swizzle(key), last_chunk), vt + i * 1024);
+        }
+    };
+    constexpr int SC_LOADS = 2 * NG;
+    const int last_pair = d / (32 * GS) - 1;  // likewise
+    auto load_scales = [&] {
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            const int from = 4 * min(e, last_pair);
+            copy_to_lds<4>((const char *)k_sc + from, raw_sc + e * 256);
+            copy_to_lds<4>((const char *)v_sc + from, raw_sc + (NG + e) * 256);
+        }
+    };
+    auto raw_pair = [&](int is_v, int e) {
+        return reinterpret_cast<const unsigned *>(raw_sc + (is_v * NG + e) * 256)[lane];
+    };
+    auto pair_of = [](unsigned u) {
+        T t[2];
+        __builtin_memcpy(t, &u, 4);
+        return float2{(float)t[0], (float)t[1]};
+    };
+    // a step's pairs in FP32 to LDS: K's times the softmax's scale, V's scale and middle
+    auto convert = [&](bool in, bool bad) {
+        float2 kp[NG], vp[NG];
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            kp[e] = pair_of(raw_pair(0, e)), vp[e] = pair_of(raw_pair(1, e));
+            kp[e].x *= a.scale_log2, kp[e].y *= a.scale_log2;
+            if (bad) kp[e].x = __builtin_nanf("");
+            vp[e].y = __builtin_fmaf(8.0f, vp[e].x, vp[e].y);
+            if (!in) vp[e] = float2{0.0f, 0.0f};
+            if (UNIT) top = __builtin_fmaxf(top, vp[e].x);
+        }
+        if (UNIT) {
+#pragma unroll
+            for (int i = 32; i; i >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, i));
+            if (__builtin_amdgcn_readfirstlane(top > unit_scale)) {
+                const float next = __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
+                const float fade = unit_scale / next;
+                unit_scale = next;
+#pragma unroll
+                for (int i = 0; i < OB; i++) acc[i] *= fade;
+#pragma unroll
+                for (int e = 0; e < NG; e++) accz[e] *= fade;
+            }
+            const float inv = 1.0f / unit_scale;
+#pragma unroll
+            for (int e = 0; e < NG; e++) vp[e].x *= inv;
+        }
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            write_pair(kpair + e * 64 + lane, kp[e]);
+            write_pair(vpair + e * 64 + lane, vp[e]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    auto compute = [&](int st, int buf) {
+        const unsigned char *kt = mine + buf * 2 * TILE, *vt = kt + TILE;
+        float s[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+        for (int bl = 0; bl < 4; bl++) {
+            const int key = 16 * (jl >> 2) + 4 * bl + (jl & 3);
+            const unsigned char *row = kt + key * (CP * 16) + 4 * g;
+#pragma unroll
+            for (int e = 0; e < NG; e++) {
+                if (NG > 2) __builtin_amdgcn_sched_barrier(0);
+                f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < GS; t++) {
+                    H8 k;
+                    codes8(*reinterpret_cast<const unsigned *>(row + (((e * GS + t) ^ k_swizzle(key)) << 4)), k);
+                    c = mma16(k, q[e * GS + t], c);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float2 kp = read_pair(kpair + e * 64 + 16 * g + 4 * bl + r);
+                    s[4 * bl + r] = __builtin_fmaf(kp.x, c[r], s[4 * bl + r]);
+                    s[4 * bl + r] = __builtin_fmaf(kp.y, qs[e], s[4 * bl + r]);
+                }
+            }
+        }
+        const int v0 = st * 64, j0 = keys.at(v0), j1 = keys.at(v0 + 63);
+        const bool all = v0 + 63 < nv && j1 <= pos0 &&
+                         (j1 < p.sinks || (v0 >= keys.sink_end && j0 > pos1 - p.window));
+        if (!all) {
+            const int mine0 = v0 + 16 * g, hi = v_hi - mine0, lo = v_lo - mine0, sink = v_sink - mine0;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const bool hidden = (i > hi) | ((i < lo) & (i >= sink));
+                s[i] = hidden ? -__builtin_inff() : s[i];
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = __builtin_fmaxf(top, s[i]);
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+            const float old = m;
+            m = __builtin_fmaxf(m, top);
+            const float fade = old == m ? 1.0f : __builtin_amdgcn_exp2f(old - m);
+            l *= fade;
+#pragma unroll
+            for (int i = 0; i < OB; i++) acc[i] *= fade;
+#pragma unroll
+            for (int e = 0; e < NG; e++) accz[e] *= fade, zsum[e] *= fade;
+        }
+        // lane jl of 16 reads 16 codes of key 16 g + jl and gets 16 keys' codes of value jl
+        unsigned vw[OB][2];
+        {
+            const int key = 16 * g + jl;
+            const unsigned char *row = vt + key * (CP * 16);
+            if constexpr (CP == 2) {
+                read_transposed4(row + (v_swizzle(key) << 4), row + ((1 ^ v_swizzle(key)) << 4), vw);
+            } else {
+#pragma unroll
+                for (int c = 0; c < CP; c += 4)
+                    read_transposed8(row + ((c ^ v_swizzle(key)) << 4), row + (((c + 1) ^ v_swizzle(key)) << 4),
+                                     row + (((c + 2) ^ v_swizzle(key)) << 4), row + (((c + 3) ^ v_swizzle(key)) << 4),
+                                     vw + 2 * c);
+            }
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+            l += s[i];
+        }
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            if (NG > 2) __builtin_amdgcn_sched_barrier(0);
+            f32x8 w0, w1;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float2 vp = read_pair(vpair + e * 64 + 16 * g + i);
+                const int k = (i & 7) >> 1 | (i & 1) << 2;  // the order of codes8
+                if (i < 8) w0[k] = s[i] * vp.x;
+                else w1[k] = s[i] * vp.x;
+                zsum[e] = __builtin_fmaf(s[i], vp.y, zsum[e]);
+            }
+            const H8 p0 = __builtin_convertvector(w0, H8), p1 = __builtin_convertvector(w1, H8);
+            accz[e] = mma16(minus8, p0, accz[e]);
+            accz[e] = mma16(minus8, p1, accz[e]);
+#pragma unroll
+            for (int i = 2 * GS * e; i < 2 * GS * (e + 1); i++) {
+                H8 v;
+                codes8(vw[i][0], v);
+                acc[i] = mma16(v, p0, acc[i]);
+                codes8(vw[i][1], v);
+                acc[i] = mma16(v, p1, acc[i]);
+            }
+        }
+    };
+    int st = split * per + wave;
+    if (st < s_end) {
+        load_ids(st);
+        wait_loads<0>();
+        place(st);
+        load_ids(st + WAVES);
+        load_codes(0);
+        load_scales();
+        int buf = 0;
+        for (; st + WAVES < s_end; st += WAVES, buf ^= 1) {
+            const bool now_in = in, now_bad = bad;
+            wait_loads<2 * CP + SC_LOADS>();
+            place(st + WAVES);
+            load_ids(st + 2 * WAVES);
+            load_codes(buf ^ 1);
+            wait_loads<2 * CP + 1>();
+            convert(now_in, now_bad);
+            load_scales();
+            compute(st, buf);
+        }
+        wait_loads<0>();
+        convert(in, bad);
+        compute(st, buf);
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int e = 0; e < NG; e++) {
+        zsum[e] += __shfl_xor(zsum[e], 16);
+        zsum[e] += __shfl_xor(zsum[e], 32);
+    }
+
+    // join the waves: [WAVES][16] pairs (m, l), then [WAVES][16][DP + 4] sums
+    constexpr int OP = DP + 4;
+    __syncthreads();
+    float *ml = reinterpret_cast<float *>(lds), *os = ml + WAVES * 32;
+    if (g == 0) {
+        ml[(wave * 16 + jl) * 2] = m;
+        ml[(wave * 16 + jl) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < OB; i++) {
+        f32x4 f = acc[i] + accz[i / (2 * GS)];
+        if (UNIT) f *= unit_scale;
+        f += zsum[i / (2 * GS)];
+        *reinterpret_cast<f32x4 *>(os + (wave * 16 + jl) * OP + 16 * i + 4 * g) = f;
+    }
+    __syncthreads();
+    for (int e = tid; e < 16 * DP; e += 64 * WAVES) {
+        const int r = e / DP, c = e % DP, row = r0 + r;
+        if (row >= rows || c >= d) continue;
+        float mm = ml[r * 2];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) mm = __builtin_fmaxf(mm, ml[(w * 16 + r) * 2]);
+        const float base = mm == -__builtin_inff() ? 0.0f : mm;
+        float sum = 0.0f, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + r) * 2] - base);
+            ll += f * ml[(w * 16 + r) * 2 + 1];
+            sum += f * os[(w * 16 + r) * OP + c];
+        }
+        if (a.splits == 1) {
+            o[(long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1] + c] = (T)(sum / ll);
+        } else {
+            const long long u = (long long)unit * a.splits + split;
+            a.part_o[(u * 16 + r) * d + c] = sum;
+            if (c == 0) {
+                a.part_ml[(u * 16 + r) * 2] = mm;
+                a.part_ml[(u * 16 + r) * 2 + 1] = ll;
+            }
+        }
+    }
+}
+
+template <typename T, int CP, int GS>
+static osh_status kv4_rows_launch(const Kv4Args &a, unsigned units, hipStream_t st) {
+    constexpr int WAVES = CP / GS == 8 ? 3 : 4;  // what 160 KB hold
+    constexpr size_t wave_lds = 4 * 64 * CP * 16 + 256 + 2 * (CP / GS) * (256 + 512);
+    constexpr size_t lds = std::max<size_t>(WAVES * wave_lds, WAVES * 16 * (32 * CP + 4 + 2) * sizeof(float));
+    OSH_LAUNCH((kv4_rows_kernel<T, CP, GS, WAVES>), dim3(units * a.w.splits), dim3(64 * WAVES), lds, st, a);
+    OSH_LAUNCH_CHECK("kv4_rows_kernel");
+    return win_join<T>(a.w, units, st);
+}
+
+template <typename T, int GL>
+static osh_status kv4_append(const Kv4Args &a, hipStream_t st) {
+    const osh_window_attn &p = a.w.p;
+    const long long threads = (long long)p.max_q * p.kv_heads * 2 * (p.head_dim / 8);
+    const unsigned x = (unsigned)std::max(1LL, std::min((threads + 255) / 256, std::max(1LL, 65536LL / p.batch)));
+    OSH_LAUNCH((kv4_append_kernel<T, GL>), dim3(x, (unsigned)p.batch), dim3(256), 0, st, a);
+    OSH_LAUNCH_CHECK("kv4_append_kernel");
+    return OSH_OK;
+}
+
+template <typename T, int GS>
+static osh_status kv4_launch_g(const Kv4Args &a, unsigned units, hipStream_t st) {
+    if (const osh_status s = kv4_append<T, 4 * GS>(a, st)) return s;
+    const int d = a.w.p.head_dim;
+    if constexpr (GS <= 2) {
+        if (d <= 64) return kv4_rows_launch<T, 2, GS>(a, units, st);
+    }
+    if (d <= 128) return kv4_rows_launch<T, 4, GS>(a, units, st);
+    return kv4_rows_launch<T, 8, GS>(a, units, st);
+}
+
+template <typename T>
+static osh_status kv4_launch(const Kv4Args &a, int group, unsigned units, hipStream_t st) {
+    if (group == 32) return kv4_launch_g<T, 1>(a, units, st);
+    if (group == 64) return kv4_launch_g<T, 2>(a, units, st);
+    return kv4_launch_g<T, 4>(a, units, st);
+}
+
+static osh_status kv4_plan(const osh_kv4_attn *p, WinArgs &a, size_t &scratch) {
+    if (!p) return fail(OSH_E_INVALID, "Kv4Attention: NULL parameters");
+    if (const osh_status st = win_plan(&p->w, a, scratch)) return st;
+    if (p->group != 32 && p->group != 64 && p->group != 128)
+        return fail(OSH_E_UNSUPPORTED, "Kv4Attention: groups of %d (32, 64 or 128)", p->group);
+    if (p->w.head_dim % p->group)
+        return fail(OSH_E_UNSUPPORTED, "Kv4Attention: heads of %d in groups of %d", p->w.head_dim, p->group);
+    const int rows = p->w.max_q * a.group;
+    a.tile_rows = 16;
+    a.tiles = cdiv(rows, 16);
+    const long long units = (long long)p->w.batch * p->w.kv_heads * a.tiles;
+    if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: too many row blocks (%lld)", units);
+    if (p->w.batch > 65535) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: %d sequences", p->w.batch);
+    const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window + p->w.sinks + 16 / a.group);
+    const long long want = units ? std::max(1LL, 2LL * device_cus() / units) : 1;
+    a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
+    a.wide = false;
+    const long long parts = a.splits > 1 ? units * a.splits : 0;
+    scratch = (size_t)parts * a.tile_rows * (p->w.head_dim + 2) * 4;
+    return OSH_OK;
+}
+
+}  // namespace osh
+
+extern "C" {
+
+OSH_API osh_status osh_kv4_attention_scratch_bytes(const osh_kv4_attn *p, size_t *bytes) {
+    if (!bytes) return fail(OSH_E_INVALID, "Kv4Attention: NULL bytes");
+    WinArgs a;
+    return kv4_plan(p, a, *bytes);
+}
+
+OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *q, void *d_scratch, osh_stream s) {
+    Kv4Args a;
+    size_t scratch = 0;
+    if (const osh_status st = kv4_plan(q, a.w, scratch)) return st;
+    const osh_window_attn *p = &q->w;
+    if (p->batch == 0 || p->max_q == 0 || p->tokens == 0) return OSH_OK;
+    if (!p->d_q || !p->d_k_new || !p->d_v_new || !p->d_o || !p->d_k_pages || !p->d_v_pages || !p->d_table ||
+        !p->d_cu || !p->d_kl || !q->d_k_scales || !q->d_v_scales || (scratch && !d_scratch) ||
+        !q->d_k_stored != !q->d_v_stored)
+        return fail(OSH_E_INVALID, "Kv4Attention: NULL pointer");
+    const long long d = p->head_dim, groups = d / q->group;
+    const int64_t *two[6] = {p->q_stride,     p->o_stride,        p->k_new_stride,
+                             p->v_new_stride, q->k_stored_stride, q->v_stored_stride};
+    for (int i = 0; i < 6; i++)
+        if (two[i][0] < 0 || two[i][1] < 0) return fail(OSH_E_INVALID, "Kv4Attention: negative stride");
+    const int64_t *three[4] = {p->k_stride, p->v_stride, q->k_scale_stride, q->v_scale_stride};
+    const void *base[4] = {p->d_k_pages, p->d_v_pages, q->d_k_scales, q->d_v_scales};
+    for (int i = 0; i < 4; i++) {
+        const int unit = i < 2 ? 16 : 2;
+        if ((uintptr_t)base[i] & (i < 2 ? 15 : 3))
+            return fail(OSH_E_UNSUPPORTED, "Kv4Attention: codes need 16-byte alignment, scales 4-byte");
+        for (int e = 0; e < 3; e++) {
+            if (three[i][e] < 0) return fail(OSH_E_INVALID, "Kv4Attention: negative stride");
+            if (three[i][e] > INT_MAX) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: a stride above 2^31 - 1");
+            if (three[i][e] % unit)
+                return fail(OSH_E_UNSUPPORTED, "Kv4Attention: codes need 16-byte alignment, scales 4-byte");
+        }
+    }
+    if (p->table_stride < (p->batch > 1 ? p->table_width : 0))
+        return fail(OSH_E_INVALID, "Kv4Attention: table stride below its width");
+    auto rows = [&](const void *t, const int64_t *st, int heads) {
+        return Strided(t, d * 2).by(p->tokens, (Strided::wide)st[0] * 2).by(heads, (Strided::wide)st[1] * 2);
+    };
+    auto cache = [&](const void *t, const int64_t *st, int e, long long bytes) {
+        return Strided(t, bytes).by(p->pages, st[0] * e).by(p->page, st[1] * e).by(p->kv_heads, st[2] * e);
+    };
+    // written: o, the four parts of the cache, the stored values, the scratch
+    const Strided out[8] = {rows(p->d_o, p->o_stride, p->q_heads),
+                            cache(p->d_k_pages, p->k_stride, 1, d / 2),
+                            cache(p->d_v_pages, p->v_stride, 1, d / 2),
+                            cache(q->d_k_scales, q->k_scale_stride, 2, groups * 4),
+                            cache(q->d_v_scales, q->v_scale_stride, 2, groups * 4),
+                            rows(q->d_k_stored, q->k_stored_stride, p->kv_heads),
+                            rows(q->d_v_stored, q->v_stored_stride, p->kv_heads),
+                            Strided(d_scratch, scratch)};
+    const Strided in[6] = {rows(p->d_q, p->q_stride, p->q_heads), rows(p->d_k_new, p->k_new_stride, p->kv_heads),
+                           rows(p->d_v_new, p->v_new_stride, p->kv_heads),
+                           strided_rows(p->d_table, p->batch, p->table_stride * 4, p->table_width * 4LL),
+                           Strided(p->d_cu, (p->batch + 1LL) * 4), Strided(p->d_kl, p->batch * 4LL)};
+    for (int i = 0; i < 8; i++) {
+        if (i < 7 && shares_itself(out[i])) return fail(OSH_E_INVALID, "Kv4Attention: an output's rows share memory");
+        for (int e = 0; e < i; e++)
+            if (share_bytes(out[i], out[e])) return fail(OSH_E_INVALID, "Kv4Attention: two outputs share memory");
+        for (const Strided &t : in)
+            if (share_bytes(out[i], t)) return fail(OSH_E_INVALID, "Kv4Attention: an output overlaps an operand");
+    }
+    const long long units = (long long)p->batch * p->kv_heads * a.w.tiles;
+    a.w.part_ml = static_cast<float *>(d_scratch);
+    a.w.part_o = a.w.part_ml + units * a.w.splits * a.w.tile_rows * 2;
+    a.page_log = 0;
+    while ((1LL << a.page_log) < p->page) a.page_log++;
+    a.page_mul = (unsigned)(((1LL << (30 + a.page_log)) + p->page - 1) / p->page);
+    a.ks = q->d_k_scales;
+    a.vs = q->d_v_scales;
+    a.k_stored = q->d_k_stored;
+    a.v_stored = q->d_v_stored;
+    for (int i = 0; i < 3; i++) a.ks_stride[i] = q->k_scale_stride[i], a.vs_stride[i] = q->v_scale_stride[i];
+    for (int i = 0; i < 2; i++)
+        a.k_stored_stride[i] = q->k_stored_stride[i], a.v_stored_stride[i] = q->v_stored_stride[i];
+    return p->dtype == OSH_T_F16 ? kv4_launch<_Float16>(a, q->group, (unsigned)units, to_stream(s))
+                                 : kv4_launch<__bf16>(a, q->group, (unsigned)units, to_stream(s));
+}
+
+}  // extern "C"

@@ -39,23 +39,12 @@ __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v
 // A row is done again in steps that hold for every finite one where its squares left FP32's
 // range (mean of squares infinite: inv and amax are then 0; or below 2^-100 with eps) or its
 // scale is not above FP32's normal numbers (amax <= 2^-117): one scalar test of a row, NaN
-// among what it catches.  Tests at each step cost 10% of 65536 x 1024 (113 us for 103).
+// among what it catches.  Tests at each step cost 10% of 65536 x 1024 (113 us for 103).  The
+// steps are row_shift and row_inv.
 __device__ __forceinline__ bool row_is_rare(float inv, float amax) {
     const unsigned i = __builtin_amdgcn_readfirstlane(__float_as_uint(inv));
     const unsigned m = __builtin_amdgcn_readfirstlane(__float_as_uint(amax));
     return i > 0x58800000u /* 2^50 */ || m <= 0x05000000u /* 2^-117 */ || m > 0x7f800000u;
-}
-// The steps.  The row is taken times the power of two that brings the larger of its largest
-// |h| and sqrt(eps) (of biased exponent eps_exp) to [1, 2), as far as floats go: y is that of
-// the row times it, with eps times its square.
-__device__ __forceinline__ float row_shift(float hmax, int eps_exp) {
-    const int e = max((int)(__float_as_uint(hmax) >> 23), eps_exp);
-    return __uint_as_float((unsigned)min(max(254 - e, 1), 253) << 23);
-}
-// 1 / sqrt; 0 for a row of zeros without eps, NaN for a row that is not finite.
-__device__ __forceinline__ float row_inv(float hmax, float mean, float eps) {
-    if (!(hmax < __builtin_inff())) return __builtin_nanf("");
-    return mean + eps == 0.0f ? 0.0f : 1.0f / __builtin_sqrtf(mean + eps);
 }
 // Where the scale lies below FP32's normal numbers, y does so too and has few bits: it is
 // then taken 2^60 times as large, and `back` is 1 / (2^60 times the scale that is stored), or

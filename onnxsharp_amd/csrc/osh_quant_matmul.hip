@@ -131,43 +131,6 @@ __device__ __forceinline__ i32x4 load_chunk(const unsigned char *row, int k0, in
     return v;
 }
 
-// Activations.  EXACT ones are for FP32 outputs: GELU is x erfc(-x / sqrt 2) / 2, since
-// 1 + erf cancels below zero (4% off at -5, 0 from -5.6 on).  For 16-bit outputs SiLU takes
-// the hardware's reciprocal, and GELU, x - x Q(x) for x > 0 and x Q(-x) below with Q(z) =
-// erfc(z / sqrt 2) / 2, a least-maximum fit of erfc(z) e^(z^2) by t P(t), t = 1 / (1 +
-// 0.4 z): within 7e-8 of erfc in exact arithmetic, and GELU within 8e-8 in FP32.  Of its own
-// size it is 5e-7 off for x > -1, 2e-6 at -3, 3e-5 at -5 (1/16 of f16's half step where f16
-// has normal numbers, from -4 up), 5e-4 at -8 and 2e-3 at -12 (1/8 and 1/2 of bf16's).
-// erff is 45 instructions a value against 17: 8 us of 1028 x 5120 x 1280.
-template <bool EXACT>
-__device__ __forceinline__ float apply_act(int act, float v) {
-    switch (act) {
-    case OSH_ACT_RELU: return v > 0.0f || v != v ? v : 0.0f;
-    case OSH_ACT_SILU: {
-        const float e = 1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f);
-        return EXACT ? v / e : v * __builtin_amdgcn_rcpf(e);
-    }
-    case OSH_ACT_GELU: {
-        if (EXACT) {
-            const float c = v < -64.0f ? -64.0f : v;  // -0 from there on, at -infinity too
-            return 0.5f * c * erfcf(c * -0.70710678118654752f);
-        }
-        const float z = __builtin_fabsf(v) * 0.70710678118654752f;
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, z, 1.0f));
-        float q = -0.20526915788650513f;
-        q = __builtin_fmaf(q, t, 0.7297442555427551f);
-        q = __builtin_fmaf(q, t, -0.4045509994029999f);
-        q = __builtin_fmaf(q, t, 0.4955560863018036f);
-        q = __builtin_fmaf(q, t, 0.15084387362003326f);
-        q = __builtin_fmaf(q, t, 0.23367586731910706f);
-        q *= t * __builtin_amdgcn_exp2f(z * z * -1.4426950408889634f);
-        const float h = 0.5f * __builtin_fminf(__builtin_fabsf(v), 64.0f) * q;  // q is 0 from 64 on
-        return v > 0.0f ? v - h : -h;
-    }
-    default: return v;
-    }
-}
-
 // One output from its sum; scale, bias, activation and residual in FP32, one
 // rounding to T.
 template <typename T>
@@ -188,12 +151,6 @@ __device__ __forceinline__ T finish(const QmmArgs &p, float sum, int row, int co
 // 8192 x 8192 x 4096).  `lds` holds EpiRows * EpiPitch<FN> floats.
 constexpr int EpiRows = 64;
 template <int FN> constexpr int EpiPitch = 16 * FN + 4;
-
-template <int ACT, bool EXACT>
-__device__ __forceinline__ void act8(f32x8 &v) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = apply_act<EXACT>(ACT, v[i]);
-}
 
 template <int Q, typename T, int FM, int FN>
 __device__ __forceinline__ void qmm_epilogue(const QmmArgs &p, const typename QAcc<Q>::type (&acc)[FM][FN], float *lds,

@@ -88,6 +88,14 @@ class WindowAttn(C.Structure):
                 + [(f, C.c_int64 * 3) for f in ("k_stride", "v_stride")] + [("table_stride", C.c_int64)])
 
 
+class Kv4Attn(C.Structure):
+    """osh_kv4_attn: an attention call over a cache held in 4 bits."""
+    _fields_ = ([("w", WindowAttn), ("group", C.c_int), ("reserved", C.c_int)]
+                + [(f, C.c_void_p) for f in ("d_k_scales", "d_v_scales", "d_k_stored", "d_v_stored")]
+                + [(f, C.c_int64 * 3) for f in ("k_scale_stride", "v_scale_stride")]
+                + [(f, C.c_int64 * 2) for f in ("k_stored_stride", "v_stored_stride")])
+
+
 _vp, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 _i64p = C.POINTER(C.c_int64)
 
@@ -152,6 +160,14 @@ _SIGS = {
     "osh_quant_matmul": ([_i, _i, _i, _i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp], _i),
     "osh_window_attention_scratch_bytes": ([C.POINTER(WindowAttn), C.POINTER(_sz)], _i),
     "osh_window_attention": ([C.POINTER(WindowAttn), _vp, _vp], _i),
+    "osh_block_norm": ([_i64, _i, _i, _vp, _i64, C.c_float, _vp, _i64, C.c_float, _vp, _vp, _i64, _i, _vp, C.c_float, _vp,
+                        _i64, _vp, _i64, _vp], _i),
+    "osh_int4_packed_bytes": ([_i, _i, _i, _i, _i, C.POINTER(_sz)], _i),
+    "osh_int4_pack": ([_i, _i, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp], _i),
+    "osh_int4_matmul_scratch_bytes": ([_i, _i, _i, _i, _i, C.POINTER(_sz)], _i),
+    "osh_int4_matmul": ([_i, _i, _i, _i, _i, _vp, _i64, _vp, _i, _vp, _i, _vp, _i64, _vp, _i64, _vp, _vp], _i),
+    "osh_kv4_attention_scratch_bytes": ([C.POINTER(Kv4Attn), C.POINTER(_sz)], _i),
+    "osh_kv4_attention": ([C.POINTER(Kv4Attn), _vp, _vp], _i),
     "osh_graph_begin": ([_vp], _i),
     "osh_graph_end": ([_vp, C.POINTER(_vp)], _i),
     "osh_graph_launch": ([_vp, _vp], _i),

@@ -1,0 +1,457 @@
+"""GPU: WindowAttentionLayer over a PagedKv4Cache against its formula in 64 bits.
+
+What the cache holds is defined in FP32 and compared bit by bit.  Bounds of o, with h = eps / 2
+of the type and w the softmax's weights: a weight times its value's scale is rounded once,
+half a step, and multiplies a code less 8: h sum w 8 scale; the output rounds once more, h |o|.
+f16 weights below 2^-14 of the largest scale's unit (at most twice that scale) are off by 2^-25
+of it instead, at most 8 of it a key and 1 / (largest w) of it in all.  Scores are FP32 sums of
+at most d exact products and three more terms a group, of sizes S = (sum |q| (15 scale + |lo|))
+times the softmax's scale: (d / 8 + 16) 2^-24 S is below 2^-13 for S < 100 and d <= 256; sums
+and joins of weights and values take at most one rounding a key of a lane and one a join:
+2^-11 sum w (|lo| + 15 scale) covers them."""
+import pytest
+import torch
+
+from onnxsharp_amd.lm_layers import PagedKv4Cache, WindowAttentionLayer
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def quantize(v, group):
+    """(codes [..., d], scale, lo [..., groups]) of v [..., d], as the cache defines them."""
+    f = v.float().unflatten(-1, (-1, group))
+    lo, hi = f.amin(-1), f.amax(-1)
+    scale = ((hi - lo) / torch.full_like(hi, 15.0)).to(v.dtype)
+    codes = torch.where(scale[..., None] > 0, ((f - lo[..., None]) / scale.float()[..., None]).round(), 0.0).clamp(0, 15)
+    bad = ~f.isfinite().all(-1)
+    scale, lo = torch.where(bad, torch.nan, scale).to(v.dtype), torch.where(bad, torch.nan, lo).to(v.dtype)
+    return codes.nan_to_num(0).flatten(-2).to(torch.uint8), scale, lo
+
+
+def pack(codes):
+    return codes[..., 0::2] | codes[..., 1::2] << 4
+
+
+def make(cuda, hq, hkv, d, group, page, lens, dtype, seed, spare=3, size=1.0):
+    """lens: (new, whole) of each sequence.  Slots that hold no token have NaN for scales."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    t = TYPES[dtype]
+    rnd = lambda *s: (size * torch.randn(*s, generator=g, device=cuda)).to(t)  # noqa: E731
+    b = len(lens)
+    width = max((kl + page - 1) // page for _, kl in lens) + 1
+    pages = sum((kl + page - 1) // page for _, kl in lens) + spare
+    s = dict(hq=hq, hkv=hkv, d=d, group=group, page=page, lens=lens)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((b, width), -1, dtype=torch.int32)
+    held = torch.zeros(pages, page, dtype=torch.bool)
+    for i, (ql, kl) in enumerate(lens):
+        for j in range((kl + page - 1) // page):
+            table[i, j] = order.pop()
+            held[table[i, j], :max(0, min(page, kl - ql - j * page))] = True
+    s["table"] = table.to(cuda)
+    s["cache"] = PagedKv4Cache.empty(pages, page, hkv, d, s["table"], group, t)
+    held = held.to(cuda)
+    for codes, scales in ((s["cache"].k_codes, s["cache"].k_scales), (s["cache"].v_codes, s["cache"].v_scales)):
+        c, sc, lo = quantize(rnd(pages, page, hkv, d), group)
+        codes.copy_(pack(c))
+        scales.copy_(torch.where(held[..., None, None, None], torch.stack((sc, lo), -1), torch.nan))
+    tokens = sum(ql for ql, _ in lens)
+    s["q"], s["k"], s["v"] = (rnd(tokens, hq, d).float() / size).to(t), rnd(tokens, hkv, d), rnd(tokens, hkv, d)
+    cu = [0]
+    for ql, _ in lens:
+        cu.append(cu[-1] + ql)
+    s["cu"] = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    s["kl"] = torch.tensor([kl for _, kl in lens], dtype=torch.int32, device=cuda)
+    return s
+
+
+def parts(cache):
+    return cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales
+
+
+def copies(cache):
+    return [t.clone(memory_format=torch.preserve_format) for t in parts(cache)]
+
+
+def same(a, b):
+    a, b = (t if t.dtype == torch.uint8 else t.contiguous().view(torch.int16) for t in (a, b))
+    return torch.equal(a, b)
+
+
+def same_bits_or_nan(a, b):
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+
+
+def run(s, window, sinks, scale=None, slack=0, **kw):
+    max_q = max(ql for ql, _ in s["lens"]) + slack
+    max_kv = max(max(kl for _, kl in s["lens"]), 1) + slack
+    return WindowAttentionLayer(window, sinks, scale).forward(s["q"], s["k"], s["v"], s["cache"], s["cu"], s["kl"], max_q,
+                                                              max_kv, **kw)
+
+
+def ref(s, window, sinks, scale=None):
+    """o, its bound, the cache afterwards and what it stands for at the new tokens, from the
+    cache before."""
+    group, page, table, rep = s["group"], s["page"], s["table"].cpu(), s["hq"] // s["hkv"]
+    kc, vc, ks, vs = copies(s["cache"])
+    dev, t = kc.device, s["q"].dtype
+    half, scale = torch.finfo(t).eps / 2, s["d"] ** -0.5 if scale is None else scale
+    o = torch.zeros(s["q"].shape, dtype=torch.float64, device=dev)
+    bound = torch.zeros_like(o)
+    stored = [torch.zeros_like(s["k"]), torch.zeros_like(s["k"])]
+
+    def values(codes, pairs):
+        c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double().unflatten(-1, (-1, group))
+        p = pairs.double()
+        return ((p[..., 1:] + p[..., :1] * c).flatten(-2), p[..., 0].abs().repeat_interleave(group, -1),
+                p[..., 1].abs().repeat_interleave(group, -1))
+
+    c = 0
+    for i, (ql, kl) in enumerate(s["lens"]):
+        at = torch.arange(kl)
+        pg, sl = table[i, at // page].long().to(dev), (at % page).to(dev)
+        for codes, pairs, new, kept in ((kc, ks, s["k"], stored[0]), (vc, vs, s["v"], stored[1])):
+            q, sc, lo = quantize(new[c:c + ql], group)
+            codes[pg[kl - ql:], sl[kl - ql:]] = pack(q)
+            pairs[pg[kl - ql:], sl[kl - ql:]] = torch.stack((sc, lo), -1)
+            kept[c:c + ql] = values(pack(q), torch.stack((sc, lo), -1))[0].to(t)
+        k, (v, sv, lv) = values(kc[pg, sl], ks[pg, sl])[0], values(vc[pg, sl], vs[pg, sl])
+        j = torch.arange(kl, device=dev)
+        p = torch.arange(kl - ql, kl, device=dev)[:, None]
+        seen = (j <= p) & ((j > p - (window or 1 << 30)) | (j < sinks))
+        for h in range(s["hq"] if ql else 0):
+            e = (s["q"][c:c + ql, h].double() @ k[:, h // rep].T.contiguous()) * scale
+            w = torch.softmax(e.masked_fill(~seen, -torch.inf), 1)
+            u = h // rep
+            # what no query sees may hold anything
+            used = seen.any(0)[:, None]
+            hv, hs, hl = (torch.where(used, x[:, u], 0.0) for x in (v, sv, lv))
+            o[c:c + ql, h] = w @ hv
+            b = half * ((w @ hv).abs() + 8 * (w @ hs)) + 2.0 ** -11 * (w @ (hl + 15 * hs)) + torch.finfo(t).smallest_normal
+            if t == torch.float16 and kl:
+                b = b + seen.sum(1, keepdim=True) * 2.0 ** -21 * hs.amax() * w.amax(1, keepdim=True)
+            bound[c:c + ql, h] = b
+        c += ql
+    return o, bound, (kc, vc, ks, vs), stored
+
+
+def check(s, window, sinks, scale=None, **kw):
+    o, bound, cache, kept = ref(s, window, sinks, scale)
+    stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+    out = run(s, window, sinks, scale, stored=stored, **kw)
+    d = (out.double() - o).abs()
+    assert out.shape == o.shape and (d <= bound).all(), (float((d - bound).max()), int((~(d <= bound)).sum()))
+    for got, want in zip(parts(s["cache"]), cache):
+        assert torch.equal(got, want) if got.dtype == torch.uint8 else same_bits_or_nan(got, want)
+    for got, want in zip(stored, kept):
+        assert torch.equal(got, want)
+    return out
+
+
+# hq, hkv, d, group, page, (new, whole), window, sinks
+CASES = [
+    (1, 1, 32, 32, 1, [(1, 1)], 1, 0),
+    (4, 4, 32, 32, 16, [(1, 1), (1, 2), (1, 17), (1, 33), (1, 65)], 16, 0),
+    (12, 4, 64, 32, 16, [(1, 600)], 512, 4),
+    (8, 1, 128, 128, 64, [(1, 1000), (1, 3), (0, 70), (1, 129), (0, 0)], 300, 4),
+    (16, 2, 96, 32, 16, [(1, 77), (1, 400)], 64, 16),
+    (6, 2, 64, 64, 7, [(1, 50), (1, 8)], 20, 3),
+    (4, 2, 256, 32, 32, [(1, 300), (1, 31)], 1000, 0),
+    (4, 2, 256, 128, 32, [(1, 300), (1, 31)], 1000, 0),
+    (3, 3, 192, 64, 16, [(1, 90), (2, 20)], 33, 1),
+    (40, 2, 64, 32, 16, [(1, 100), (2, 40)], 50, 2),
+    (8, 2, 160, 32, 16, [(3, 100), (5, 5), (1, 64), (8, 200)], 32, 4),
+    (4, 1, 64, 64, 16, [(70, 70), (33, 100), (1, 90), (130, 131)], 40, 4),
+    (4, 2, 128, 64, 32, [(200, 500), (64, 64)], 128, 130),
+    (2, 2, 32, 32, 5, [(90, 95)], 1, 0),
+    (2, 1, 64, 32, 16, [(100, 300)], 1, 7),
+    (5, 5, 96, 32, 16, [(40, 40)], None, 0),
+    (8, 8, 128, 32, 128, [(150, 700), (1, 650), (17, 17)], None, 0),
+    (6, 1, 128, 128, 16, [(300, 300), (257, 900)], 100, 1000),
+    (8, 2, 256, 64, 16, [(100, 260), (40, 40)], 90, 3),
+    (8, 8, 256, 32, 16, [(70, 200), (1, 30)], None, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention(cuda, case, dtype):
+    hq, hkv, d, group, page, lens, window, sinks = CASES[case]
+    print(f"attention over 4 bits {CASES[case]} {dtype}", flush=True)
+    check(make(cuda, hq, hkv, d, group, page, lens, dtype, case), window, sinks)
+
+
+@pytest.mark.parametrize("d,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
+def test_long_histories(cuda, d, group):
+    # few sequences: the keys are split and joined
+    check(make(cuda, 4, 1, d, group, 64, [(1, 6000), (1, 100)], "bf16", 1), 5000, 4)
+    check(make(cuda, 4, 1, d, group, 64, [(3, 5000)], "f16", 2), None, 0)
+    check(make(cuda, 2, 1, d, group, 16, [(24, 3001)], "bf16", 3), 2500, 16)
+
+
+def test_long_prompts(cuda):
+    check(make(cuda, 8, 2, 128, 64, 64, [(1100, 1100), (300, 1500)], "bf16", 4), 256, 4)
+    check(make(cuda, 4, 4, 64, 32, 16, [(600, 600)], "f16", 5), None, 0)
+
+
+def test_bounds_above_the_lengths(cuda):
+    s = make(cuda, 4, 2, 64, 32, 16, [(3, 50), (1, 200), (0, 9)], "bf16", 6)
+    s["table"] = torch.cat([s["table"], torch.full((3, 400), -1, dtype=torch.int32, device=cuda)], 1)
+    s["cache"].table = s["table"]
+    check(s, 100, 2, slack=1000)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("size,dtype", [(1e-3, "f16"), (3000.0, "f16"), (1e-20, "bf16"), (1e20, "bf16")])
+def test_sizes_of_values(cuda, size, dtype, new):
+    s = make(cuda, 4, 2, 128, 32, 16, [(new, 400)], dtype, 7, size=size)
+    check(s, 300, 4, scale=0.08 / size)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 40])
+def test_groups_of_different_sizes(cuda, dtype, new):
+    # one key's values far above the others', constant groups, zeros
+    s = make(cuda, 4, 2, 128, 32, 16, [(new, 400)], dtype, 8)
+    pg = s["table"][0, 9].long()
+    s["cache"].v_scales[pg, 3] *= 100.0
+    s["cache"].v_scales[pg, 4, :, 1, 0] = 0
+    s["cache"].k_scales[pg, 5] = 0
+    s["k"][0, :, :64], s["v"][0, :, 32:] = 0.75, 0
+    check(s, 300, 4)
+
+
+def test_one_key_above_all(cuda):
+    s = make(cuda, 2, 2, 64, 64, 16, [(1, 900)], "bf16", 8)
+    s["q"].fill_(8.0)
+    pg = s["table"][0, 20].long()
+    s["cache"].k_codes[pg, 3] = 0xff
+    s["cache"].k_scales[pg, 3] = torch.tensor([0.5, 0.5], device=cuda)
+    out = run(s, None, 0)
+    c = s["cache"].v_codes[pg, 3]
+    c = torch.stack((c & 15, c >> 4), -1).flatten(-2).float()
+    p = s["cache"].v_scales[pg, 3].float()
+    want = p[..., 0, 1:] + p[..., 0, :1] * c
+    assert ((out[0].float() - want).abs() <= 2.0 ** -8 * (want.abs() + 8 * p[..., 0, :1]) + 1e-3).all()
+
+
+def test_strided_operands_and_pages(cuda):
+    hq, hkv, d, page, lens = 8, 2, 64, 16, [(20, 90), (1, 40)]
+    s = make(cuda, hq, hkv, d, 32, page, lens, "bf16", 9)
+    qkv = torch.cat([s[f].reshape(21, -1) for f in "qkv"], 1)
+    s["q"] = qkv[:, :hq * d].view(21, hq, d)
+    s["k"] = qkv[:, hq * d:(hq + hkv) * d].view(21, hkv, d)
+    s["v"] = qkv[:, (hq + hkv) * d:].view(21, hkv, d)
+    # slots in front of heads, K and V and their scales in one buffer each
+    codes = torch.stack(parts(s["cache"])[:2], 3).contiguous()
+    scales = torch.stack(parts(s["cache"])[2:], 3).contiguous()
+    s["cache"] = PagedKv4Cache(codes[:, :, :, 0], codes[:, :, :, 1], scales[:, :, :, 0], scales[:, :, :, 1], s["table"])
+    wide = torch.zeros(21, hq, d + 3, dtype=torch.bfloat16, device=cuda)
+    out = check(s, 32, 4, out=wide[..., 2:d + 2])
+    assert out.data_ptr() == wide.data_ptr() + 4
+    assert not wide[..., :2].any() and not wide[..., d + 2:].any()
+    s["k"] = s["k"].transpose(0, 1).contiguous().transpose(0, 1)
+    check(s, 32, 4)
+
+
+def test_what_no_query_sees(cuda):
+    s = make(cuda, 4, 2, 64, 32, 16, [(1, 400), (30, 300)], "bf16", 10)
+    want = check(s, 64, 4)
+    for i, (ql, kl) in enumerate(s["lens"]):
+        first = kl - ql - 64 + 1
+        for j in range(1, first // 16):
+            pg = int(s["table"][i, j])
+            s["cache"].k_scales[pg], s["cache"].v_scales[pg] = float("inf"), float("nan")
+            s["table"][i, j] = [-1, 1 << 30, -2 ** 31, 999][j % 4]
+        pg = int(s["table"][i, first // 16])
+        s["cache"].k_scales[pg, :first % 16], s["cache"].v_scales[pg, :first % 16] = float("nan"), float("-inf")
+        pg = int(s["table"][i, 0])
+        s["cache"].k_scales[pg, 4:], s["cache"].v_scales[pg, 4:] = float("nan"), float("nan")
+    assert same(run(s, 64, 4), want)
+
+
+def test_bad_pages(cuda):
+    lens = [(1, 100), (1, 100), (40, 100), (1, 97)]
+    s = make(cuda, 4, 2, 64, 64, 16, lens, "f16", 11)
+    good = run(s, 32, 0)
+    before = copies(s["cache"])
+    last = s["table"][3, 6].item()
+    s["table"][0, 5] = s["cache"].k_codes.shape[0]  # positions 80..95, seen by sequence 0's query at 99
+    s["table"][1, 0] = -5                           # positions 0..15, outside sequence 1's window
+    s["table"][2, 6] = -1                           # positions 96..99: sequence 2's last four queries see a part
+    s["table"][3, 6] = 1 << 30                      # sequence 3's new token itself
+    stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+    out = run(s, 32, 0, stored=stored)
+    assert out[0].isnan().all() and same(out[1], good[1]) and out[42].isnan().all()
+    assert same(out[2:38], good[2:38]) and out[38:42].isnan().all()
+    for t in stored:
+        assert t[38:].isnan().all() and t[:38].isfinite().all()
+    for got, want in zip(parts(s["cache"]), before):
+        assert same(got, want)
+    assert last >= 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group,ql,kl", [(64, 32, 3, 40), (128, 64, 90, 130), (128, 32, 60, 90), (256, 128, 60, 90)])
+def test_keys_that_are_not_finite(cuda, d, group, ql, kl, dtype):
+    s, window = make(cuda, 4, 2, d, group, 16, [(ql, kl)], dtype, d + ql), 24
+    past = kl - ql
+    old, tk = past - 10, ql - 2
+    good = run(s, window, 2)
+    s["k"][tk, 0, 1] = float("nan")
+    s["cache"].k_scales[int(s["table"][0, old // 16]), old % 16, 0, 0] = float("nan")
+    stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+    out = run(s, window, 2, stored=stored)
+    pos = past + torch.arange(ql, device=cuda)
+    want = torch.zeros(out.shape, dtype=torch.bool, device=cuda)
+    for j in (past + tk, old):
+        want[(j <= pos) & (j > pos - window), :2] = True
+    assert torch.equal(out.isnan(), want)
+    assert torch.equal(out[~want], good[~want])
+    assert stored[0][tk, 0, :group].isnan().all() and int(stored[0].isnan().sum()) == group
+
+
+def test_values_that_are_not_finite(cuda):
+    s = make(cuda, 4, 2, 64, 32, 16, [(1, 100), (1, 50)], "bf16", 17)
+    good = run(s, 64, 4)
+    s["v"][0, 1, 40] = float("-inf")
+    out = run(s, 64, 4)
+    assert out[0, 2:, 32:].isnan().all() and same(out[0, :2], good[0, :2]) and same(out[1], good[1])
+    assert same(out[0, 2:, :32], good[0, 2:, :32])
+    pg, slot = s["table"][0, 6].long(), 99 % 16
+    assert s["cache"].v_scales[pg, slot, 1, 1].isnan().all() and s["cache"].v_scales[pg, slot, 1, 0].isfinite().all()
+
+
+def test_lengths_that_contradict(cuda):
+    s = make(cuda, 4, 2, 64, 32, 16, [(2, 50), (3, 60), (1, 20)], "bf16", 12)
+    good = run(s, 32, 2)
+    before = copies(s["cache"])
+    for kl in (2, 10 ** 6, -1):
+        s["kl"][1] = kl
+        stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+        out = run(s, 32, 2, stored=stored)
+        assert out[2:5].isnan().all() and same(out[:2], good[:2]) and same(out[5:], good[5:])
+        assert stored[0][2:5].isnan().all() and stored[0][:2].isfinite().all() and stored[1][5:].isfinite().all()
+        for got, want in zip(parts(s["cache"]), before):
+            assert same(got, want)
+
+
+def test_rows_of_no_sequence_stay(cuda):
+    s = make(cuda, 4, 2, 64, 32, 16, [(3, 50), (2, 40), (4, 30)], "f16", 24)
+    s["cu"].copy_(torch.tensor([2, 5, 7, 7]))
+    s["kl"][2] = 26
+    stored = torch.full_like(s["k"], 7.0), torch.full_like(s["v"], 7.0)
+    out = run(s, 32, 2, out=torch.full_like(s["q"], 7.0), stored=stored)
+    for t in (out, *stored):
+        assert (t[:2] == 7.0).all() and (t[7:] == 7.0).all() and (t[2:7] != 7.0).any(-1).all()
+
+
+@pytest.mark.parametrize("max_q", [1, 3, 40, 200])
+def test_more_new_tokens_than_the_bound(cuda, max_q):
+    s = make(cuda, 4, 2, 64, 32, 16, [(max_q, 300), (max_q + 157, 400), (1, 20)], "bf16", 23)
+    before = copies(s["cache"])
+    stored = torch.full_like(s["k"], 7.0), torch.full_like(s["v"], 7.0)
+    out = WindowAttentionLayer(32, 2).forward(s["q"], s["k"], s["v"], s["cache"], s["cu"], s["kl"], max_q, 400,
+                                              out=torch.full_like(s["q"], 7.0), stored=stored)
+    first, last = max_q, 2 * max_q + 157
+    for t in (out, *stored):
+        assert t[first:last].isnan().all() and t[:first].isfinite().all() and t[last:].isfinite().all()
+    for i in range(400):
+        at = int(s["table"][1, i // 16]), i % 16
+        for got, want in zip(parts(s["cache"]), before):
+            assert same(got[at], want[at])
+
+
+def test_the_way_tokens_came_does_not_matter(cuda):
+    # a prompt at once, in pieces, and token by token leave the same cache, and its last
+    # query the same output within two bounds
+    outs, caches = [], []
+    for cut in ([90], [37, 20, 33], [60] + [1] * 30):
+        s = make(cuda, 8, 2, 128, 64, 16, [(90, 90)], "bf16", 18)
+        full, at = {f: s[f] for f in "qkv"}, 0
+        bound = ref(s, 50, 4)[1][-1]
+        for n in cut:
+            for f in "qkv":
+                s[f] = full[f][at:at + n]
+            at += n
+            s["lens"], s["kl"] = [(n, at)], torch.tensor([at], dtype=torch.int32, device=cuda)
+            s["cu"] = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+            o = run(s, 50, 4)
+        outs.append(o[-1].double())
+        pages = s["table"][0, :6].long()
+        caches.append([t[pages].flatten(0, 1)[:90].clone() for t in parts(s["cache"])])
+    for o, c in zip(outs[1:], caches[1:]):
+        assert ((o - outs[0]).abs() <= 2 * bound).all()
+        assert all(same(x, y) for x, y in zip(c, caches[0]))
+
+
+@pytest.mark.parametrize("lens,window", [([(1, 500), (1, 77), (1, 1)], 100), ([(150, 400), (1, 90), (40, 40)], 64)])
+def test_alone_and_in_a_batch(cuda, lens, window):
+    # a sequence's bits under the same bounds and splits
+    s = make(cuda, 8, 2, 128, 64, 16, lens, "bf16", 31)
+    before = copies(s["cache"])
+    out, cu = run(s, window, 4), s["cu"].tolist()
+    bounds = max(q for q, _ in lens), max(k for _, k in lens)
+    for i in range(len(lens)):
+        rows = slice(cu[i], cu[i + 1])
+        cache = PagedKv4Cache(*[t.clone(memory_format=torch.preserve_format) for t in before], s["table"][i:i + 1])
+        new = torch.tensor([0, cu[i + 1] - cu[i]], dtype=torch.int32, device=cuda)
+        one = WindowAttentionLayer(window, 4).forward(s["q"][rows], s["k"][rows], s["v"][rows], cache, new,
+                                                      s["kl"][i:i + 1], *bounds)
+        assert same(out[rows], one)
+    assert same(out, run(s, window, 4))
+
+
+def test_empty(cuda):
+    s = make(cuda, 4, 2, 64, 32, 16, [(0, 40), (0, 0)], "f16", 14)
+    before = copies(s["cache"])
+    assert run(s, 32, 2).shape == (0, 4, 64)
+    assert all(same(a, b) for a, b in zip(parts(s["cache"]), before))
+
+
+@pytest.mark.parametrize("lens", [[(1, 700), (1, 30)], [(1, 6000)], [(150, 400), (1, 90)]])
+def test_on_a_stream_and_in_a_graph(cuda, lens):
+    s = make(cuda, 8, 1, 128, 32, 16, lens, "bf16", 15)
+    stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+    run(s, 4000, 4)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        run(s, 4000, 4)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out = run(s, 4000, 4, stored=stored)
+    torch.cuda.current_stream().wait_stream(st)
+    at = [(int(s["table"][i, j // 16]), j % 16) for i, (ql, kl) in enumerate(lens) for j in range(kl - ql, kl)]
+    pages, slots = (torch.tensor(t, device=cuda) for t in zip(*at))
+    for _ in range(3):
+        for f in "qkv":
+            s[f].mul_(0.9)
+        want_stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+        want = run(s, 4000, 4, stored=want_stored)
+        cache = copies(s["cache"])
+        for t in parts(s["cache"]):
+            t[pages, slots] = 5
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert same(out, want) and all(same(a, b) for a, b in zip(parts(s["cache"]), cache))
+        assert all(same(a, b) for a, b in zip(stored, want_stored))
+
+
+def test_offsets_past_32_bits(cuda):
+    # 2^31 bytes of codes in front of the pages that are used
+    hkv, d, page = 8, 128, 16
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 8 GiB")
+    s = make(cuda, 8, hkv, d, 128, page, [(1, 300), (40, 60)], "f16", 16)
+    old = s["cache"]
+    n = old.k_codes.shape[0]
+    front = 2 ** 31 // (page * hkv * d // 2) + 40
+    o, bound, _, _ = ref(s, 100, 4)
+    table = torch.where(s["table"] >= 0, s["table"] + front, s["table"])
+    s["table"], s["cache"] = table, PagedKv4Cache.empty(front + n, page, hkv, d, table, 128, torch.float16)
+    for to, t in zip(parts(s["cache"]), parts(old)):
+        to[front:] = t
+    assert ((run(s, 100, 4).double() - o).abs() <= bound).all()
