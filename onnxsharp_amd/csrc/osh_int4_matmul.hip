@@ -79,6 +79,29 @@ __device__ __forceinline__ T int4_finish(const Int4Args &p, float v, int row, in
     return (T)v;
 }
 
+// Eight neighbouring outputs of a row, as far as they are there.
+template <typename T>
+__device__ __forceinline__ void int4_store8(const Int4Args &p, f32x8 f, int row, int col) {
+    if (row >= p.m || col >= p.n) return;
+    T *y = static_cast<T *>(p.y) + row * p.ldy + col;
+    const T *res = static_cast<const T *>(p.res) + row * p.ldr + col;
+    if (col + 8 <= p.n) {
+        if (p.bias) f += load8(p.bias + col);
+        switch (p.act) {
+        case OSH_ACT_RELU: act8<OSH_ACT_RELU, sizeof(T) == 4>(f); break;
+        case OSH_ACT_SILU: act8<OSH_ACT_SILU, sizeof(T) == 4>(f); break;
+        case OSH_ACT_GELU: act8<OSH_ACT_GELU, sizeof(T) == 4>(f); break;
+        default: break;
+        }
+        if (p.res) f += load8(res);
+        store8(y, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 7; i++)
+            if (col + i < p.n) y[i] = int4_finish<T>(p, f[i], row, col + i);
+    }
+}
+
 // Few rows: a workgroup takes 16 NB outputs of 16 MB rows, its waves every WAVES-th block
 // of k; the weights go from memory to registers, each byte once.  GS steps of 32 k share a
 // scale.  The waves' sums meet in LDS, in the order of the waves.
@@ -186,6 +209,247 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
     }
 }
 
+
+// ---------------------------------------------------------------- many rows
+
+// What the tile kernel reads of the rows: their 16-bit pieces (the rows themselves where
+// they are 16-bit and whole chunks long) and the sums over groups.
+struct Int4Prep {
+    const unsigned short *a;
+    long long pitch, plane;  // of a row and of a piece, in values
+    int chunks;              // of 8 values in a row; what lies past them is 0
+    int groups;
+    const uint4 *sums;       // of 16-bit rows, [m][groups]: -sum a in three bf16 pieces
+};
+
+// -sum_k a z s over the groups is a product of its own, of FP32 factors: pieces a0 + a1 + a2 =
+// -sum a and s0 + s1 + s2 = z s of 8 bits each, in eight places of k a group:
+//   a0 a1 a2 a0 a1 a0 0 0  times  s0 s0 s0 s1 s1 s2 0 0.
+__device__ __forceinline__ void pieces3(float v, unsigned (&top)[3]) {
+    float rest = v;
+#pragma unroll
+    for (int e = 0; e < 3; e++) {
+        top[e] = __float_as_uint(rest) & 0xffff0000u;
+        if (e == 0 && rest != rest) top[e] |= 0x00400000u;
+        rest -= __uint_as_float(top[e]);
+        if (e == 0 && (top[e] & 0x7f800000u) == 0x7f800000u) rest = 0.0f;
+    }
+}
+
+// Sums of the rows' groups, and with COPY their pieces [P][m][128 nkb], zero past k.  GL
+// lanes a group.
+template <typename T, int GL, bool COPY>
+__global__ __launch_bounds__(256) void int4_prep_kernel(Int4Args p, int group, int groups, uint4 *sums,
+                                                        unsigned short *planes, long long pitch, long long plane) {
+    constexpr int P = PIECES<T>;
+    const int all = COPY ? max(groups, (int)cdiv((int)pitch, group)) : groups;  // what the copy is padded to
+    const long long total = (long long)p.m * all;
+    const int sub = threadIdx.x % GL;
+    // whole rounds: the lanes of a group stay together
+    for (long long i0 = blockIdx.x * (256LL / GL); i0 < total; i0 += gridDim.x * (256LL / GL)) {
+        const long long item = i0 + threadIdx.x / GL;
+        const bool in = item < total;
+        const int row = in ? (int)(item / all) : 0, gr = in ? (int)(item - (long long)row * all) : 0;
+        const T *a = static_cast<const T *>(p.a) + row * p.lda;
+        float sum = 0.0f;
+        for (int c = 8 * sub; c < group; c += 8 * GL) {
+            const int k0 = gr * group + c;
+            const typename Vec8<T>::type v = load_row8<T>(a, k0, in ? p.k : 0);
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum += (float)v[i];
+            if (COPY && in && k0 < pitch) {
+                typename Half8<T>::type h[P];
+                split_row8<T>(v, h);
+#pragma unroll
+                for (int e = 0; e < P; e++) *reinterpret_cast<typename Half8<T>::type *>(planes + e * plane + row * pitch + k0) = h[e];
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < GL; o <<= 1) sum += __shfl_xor(sum, o);
+        if (P == 1 && in && sub == 0 && gr < groups) {
+            unsigned t[3];
+            pieces3(-sum, t);
+            sums[(long long)row * groups + gr] = uint4{t[0] >> 16 | t[1], t[2] >> 16 | t[0], t[1] >> 16 | t[0], 0u};
+        }
+    }
+}
+
+static __device__ const uint4 int4_zero_chunk = {0, 0, 0, 0};
+
+// A workgroup takes 32 MB WM rows by 32 NB WN outputs, a wave 32 MB by 32 NB.  The rows pass
+// through two LDS buffers of 128 k, loaded directly (chunk c of row r at c ^ r % 16); codes go
+// from memory to registers a block ahead and become 16-bit floats in front of the MFMAs that
+// take them.  A group's sum has its own registers, and is scaled into the wave's sums in FP32.
+// For 16-bit rows the zero points' part is added at the end (see Int4Prep); for FP32 ones, three
+// MFMAs a fragment of codes, the zero points come off the codes, which the vector unit has time
+// for and which loses nothing to the difference of two sums.
+template <typename T, int MB, int NB, int WM, int WN, int GS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void int4_tile_kernel(Int4Args p, Int4Prep q, int group) {
+    using H8 = typename Half8<T>::type;
+    constexpr int P = PIECES<T>, NG = 4 / GS, WAVES = WM * WN, R = 32 * MB * WM;
+    constexpr int STAGE = P * R * 256, COPIES = P * R / 4 / WAVES;
+    static_assert(COPIES * 4 * WAVES == P * R, "copies are dealt evenly");
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hl = lane >> 5, wm = wave / WN, wn = wave % WN;
+    const int nkb = cdiv(p.k, KB);
+
+    // bands of eight row blocks: those that run at once share rows and weights in an L2
+    int mt, nt;
+    {
+        const int tn = cdiv(p.n, 32 * NB * WN), tm = cdiv(p.m, R);
+        const int id = xcd_band(blockIdx.x, gridDim.x);
+        const int band = id / (8 * tn), high = min(8, tm - 8 * band), in = id - band * 8 * tn;
+        mt = 8 * band + in % high;
+        nt = in / high;
+    }
+    const int m0 = mt * R, n0 = nt * 32 * NB * WN;
+
+    const unsigned short *from[COPIES];
+    int chunk0[COPIES];
+#pragma unroll
+    for (int e = 0; e < COPIES; e++) {
+        const int i = wave + WAVES * e, r = i % (R / 4) * 4 + (lane >> 4);
+        chunk0[e] = (lane & 15) ^ (r & 15);
+        from[e] = q.a + i / (R / 4) * q.plane + min(m0 + r, p.m - 1) * q.pitch + 8 * chunk0[e];
+    }
+    auto load_rows = [&](int kb, int buf) {
+#pragma unroll
+        for (int e = 0; e < COPIES; e++) {
+            const bool in = kb * 16 + chunk0[e] < q.chunks;
+            const void *at = from[e] + kb * KB;
+            copy_to_lds<16>(in ? at : &int4_zero_chunk, lds + buf * STAGE + (wave + WAVES * e) * 1024);
+        }
+    };
+    long long blk[NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+        blk[j] = (long long)min((n0 + 32 * (wn * NB + j) + l32) / 16, cdiv(p.n, 16) - 1) * nkb;
+    const int jl = lane & 15;
+    uint4 w[NB][2], w_next[NB][2];
+    T sc[NB][NG], sc_next[NB][NG], zp[NB][NG], zp_next[NB][NG];
+    auto load_codes = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) w_next[j][e] = p.codes[(blk[j] + kb) * 64 + 32 * e + 16 * hl + jl];
+#pragma unroll
+            for (int e = 0; e < NG; e++) {
+                const long long at = ((blk[j] + kb) * NG + e) * 16 + jl;
+                sc_next[j][e] = static_cast<const T *>(p.scales)[at];
+                if (P > 1) zp_next[j][e] = p.zeros ? static_cast<const T *>(p.zeros)[at] : (T)8.0f;
+            }
+        }
+    };
+    f32x16 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++) acc[i][j] = f32x16{};
+    load_rows(0, 0);
+    load_codes(0);
+    int buf = 0;
+    for (int kb = 0; kb < nkb; kb++, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) w[j][e] = w_next[j][e];
+#pragma unroll
+            for (int e = 0; e < NG; e++) {
+                sc[j][e] = sc_next[j][e];
+                if (P > 1) zp[j][e] = zp_next[j][e];
+            }
+        }
+        if (kb + 1 < nkb) {
+            load_rows(kb + 1, buf ^ 1);
+            load_codes(kb + 1);
+        }
+        const unsigned char *rows = lds + buf * STAGE;
+        f32x16 sum[MB][NB];
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            H8 c[NB];
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const unsigned word = reinterpret_cast<const unsigned *>(&w[j][s & 1])[s >> 1];
+                if constexpr (P > 1) codes8_less(word, zp[j][s / (2 * GS)], c[j]);
+                else codes8(word, c[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int e = 0; e < P; e++) {
+                    const int r = 32 * (wm * MB + i) + l32;
+                    H8 x;
+                    __builtin_memcpy(&x, rows + e * (R * 256) + r * 256 + (((2 * s + hl) ^ (r & 15)) << 4), 16);
+#pragma unroll
+                    for (int j = 0; j < NB; j++)
+                        sum[i][j] = mma32(x, c[j], s % (2 * GS) == 0 && e == 0 ? f32x16{} : sum[i][j]);
+                }
+            if (s % (2 * GS) == 2 * GS - 1) {
+#pragma unroll
+                for (int j = 0; j < NB; j++) {
+                    const float f = (float)sc[j][s / (2 * GS)];
+#pragma unroll
+                    for (int i = 0; i < MB; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(f, sum[i][j][r], acc[i][j][r]);
+                }
+            }
+        }
+    }
+    for (int g0 = 0; P == 1 && g0 < q.groups; g0 += 2) {
+        const int gr = g0 + hl;
+        bf16x8 x[MB], z[NB];
+        const int at_k = min(gr, q.groups - 1) * group, kb = at_k / KB, e = NG > 1 ? at_k % KB / (32 * GS) : 0;
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            const int row = min(m0 + 32 * (wm * MB + i) + l32, p.m - 1);
+            uint4 u = q.sums[(long long)row * q.groups + min(gr, q.groups - 1)];
+            __builtin_memcpy(&x[i], &u, 16);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const long long at = ((blk[j] + kb) * NG + e) * 16 + jl;
+            float f = (float)static_cast<const T *>(p.scales)[at];
+            f *= p.zeros ? (float)static_cast<const T *>(p.zeros)[at] : 8.0f;
+            if (gr >= q.groups) f = 0.0f;
+            unsigned t[3];
+            pieces3(f, t);
+            const uint4 u = {t[0] >> 16 | t[0], t[0] >> 16 | t[1], t[1] >> 16 | t[2], 0u};
+            __builtin_memcpy(&z[j], &u, 16);
+        }
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++) acc[i][j] = mma32(x[i], z[j], acc[i][j]);
+    }
+    // through LDS, 32 rows of a wave at a time, to eight neighbouring outputs a lane
+    constexpr int PITCH = 32 * NB + 4;
+    float *mine = reinterpret_cast<float *>(lds) + wave * (32 * PITCH);
+    const int nw = n0 + 32 * NB * wn;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MB; i++) {
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) mine[(8 * (r >> 2) + 4 * hl + (r & 3)) * PITCH + 32 * j + l32] = acc[i][j][r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int e = 0; e < 32 * 32 * NB / 8 / 64; e++) {
+            const int at = e * 64 + lane, r = at / (4 * NB), c = at % (4 * NB) * 8;
+            f32x8 f;
+            __builtin_memcpy(&f, mine + r * PITCH + c, 16);
+            __builtin_memcpy(reinterpret_cast<float *>(&f) + 4, mine + r * PITCH + c + 4, 16);
+            int4_store8<T>(p, f, m0 + 32 * (wm * MB + i) + r, nw + c);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
 // Codes [n][pitch] two a byte into blocks; codes past n or k are 0 (their scales and the
 // values that meet them are 0).
 __global__ __launch_bounds__(256) void int4_pack_codes_kernel(int n, int k, const unsigned char *codes, long long pitch,
@@ -238,27 +502,82 @@ static Int4Layout int4_layout(int n, int k, int group, int dtype, bool zeros) {
     return l;
 }
 
+// What a call with many rows keeps beside its operands.
+struct Int4Room {
+    bool tile, copy;
+    size_t sums, plane, total;  // plane in values
+    int pitch;
+};
+static Int4Room int4_room(int m, int k, int group, int dtype) {
+    Int4Room r = {};
+    r.tile = m > 64;
+    if (!r.tile) return r;
+    r.copy = dtype == OSH_T_F32 || k % 8;
+    r.sums = dtype == OSH_T_F32 ? 0 : (size_t)m * cdiv(k, group) * 16;
+    r.pitch = cdiv(k, KB) * KB;
+    r.plane = r.copy ? (size_t)m * r.pitch : 0;
+    r.total = r.sums + r.plane * (dtype == OSH_T_F32 ? 6 : 2);
+    return r;
+}
+
+template <typename T, int MB, int NB, int WM, int WN, int GS>
+static void int4_tile(const Int4Args &p, const Int4Prep &q, int group, hipStream_t st) {
+    constexpr size_t lds = std::max<size_t>(2 * PIECES<T> * 32 * MB * WM * 256, WM * WN * 32 * (32 * NB + 4) * 4);
+    OSH_LAUNCH((int4_tile_kernel<T, MB, NB, WM, WN, GS>),
+               dim3((unsigned)cdiv(p.m, 32 * MB * WM) * cdiv(p.n, 32 * NB * WN)), dim3(64 * WM * WN), lds, st, p, q, group);
+}
+
 template <typename T, int GS>
-static osh_status int4_launch(const Int4Args &p, hipStream_t st) {
+static osh_status int4_launch(const Int4Args &p, int group, const Int4Room &room, void *scratch, hipStream_t st) {
+    if (!room.tile) {
 #define OSH_INT4_ROWS(MB, NB)                                                                                  \
     OSH_LAUNCH((int4_rows_kernel<T, MB, NB, GS, 8>), dim3((unsigned)cdiv(p.n, 16 * NB), (unsigned)cdiv(p.m, 16 * MB)), \
                dim3(512), 0, st, p)
-    if (p.m <= 16) OSH_INT4_ROWS(1, 1);
-    else if (p.m <= 32) OSH_INT4_ROWS(2, 1);
-    else OSH_INT4_ROWS(4, 1);
+        if (p.m <= 16) OSH_INT4_ROWS(1, 1);
+        else if (p.m <= 32) OSH_INT4_ROWS(2, 1);
+        else OSH_INT4_ROWS(4, 1);
 #undef OSH_INT4_ROWS
-    OSH_LAUNCH_CHECK("int4 kernel");
+        OSH_LAUNCH_CHECK("int4_rows_kernel");
+        return OSH_OK;
+    }
+    Int4Prep q;
+    uint4 *sums = static_cast<uint4 *>(scratch);
+    unsigned short *planes = reinterpret_cast<unsigned short *>(static_cast<char *>(scratch) + room.sums);
+    q.sums = sums;
+    q.groups = cdiv(p.k, group);
+    q.a = room.copy ? planes : static_cast<const unsigned short *>(p.a);
+    q.pitch = room.copy ? room.pitch : p.lda;
+    q.plane = room.plane;
+    q.chunks = (room.copy ? room.pitch : p.k) / 8;
+    constexpr int GL = 4 * GS;
+    const long long items = (long long)p.m * cdiv(room.pitch, 32 * GS);
+    const dim3 grid((unsigned)std::min((items + 256 / GL - 1) / (256 / GL), 1LL << 16));
+    if (room.copy) {
+        OSH_LAUNCH((int4_prep_kernel<T, GL, true>), grid, dim3(256), 0, st, p, group, q.groups, sums, planes,
+                   (long long)room.pitch, (long long)room.plane);
+    } else if constexpr (sizeof(T) == 2) {
+        OSH_LAUNCH((int4_prep_kernel<T, GL, false>), grid, dim3(256), 0, st, p, group, q.groups, sums, planes,
+                   (long long)room.pitch, (long long)room.plane);
+    }
+    OSH_LAUNCH_CHECK("int4_prep_kernel");
+    const long long big = (long long)cdiv(p.m, 128) * cdiv(p.n, 256);
+    if constexpr (sizeof(T) == 2) {
+        if (big >= device_cus()) int4_tile<T, 2, 2, 2, 4, GS>(p, q, group, st);
+        else int4_tile<T, 1, 1, 2, 2, GS>(p, q, group, st);
+    } else {
+        if (big >= device_cus()) int4_tile<T, 2, 2, 1, 4, GS>(p, q, group, st);
+        else int4_tile<T, 1, 1, 2, 2, GS>(p, q, group, st);
+    }
+    OSH_LAUNCH_CHECK("int4_tile_kernel");
     return OSH_OK;
 }
 
 template <typename T>
-static osh_status int4_launch_t(const Int4Args &p, int group, hipStream_t st) {
-    if (group == 32) return int4_launch<T, 1>(p, st);
-    if (group == 64) return int4_launch<T, 2>(p, st);
-    return int4_launch<T, 4>(p, st);
+static osh_status int4_launch_t(const Int4Args &p, int group, const Int4Room &room, void *scratch, hipStream_t st) {
+    if (group == 32) return int4_launch<T, 1>(p, group, room, scratch, st);
+    if (group == 64) return int4_launch<T, 2>(p, group, room, scratch, st);
+    return int4_launch<T, 4>(p, group, room, scratch, st);
 }
-
-static size_t int4_scratch(int m, int n, int k, int dtype) { return 0; }
 
 static osh_status int4_check(int n, int k, int group, int dtype) {
     if (n < 0 || k < 0) return fail(OSH_E_INVALID, "Int4MatMul: negative sizes");
@@ -322,7 +641,7 @@ OSH_API osh_status osh_int4_matmul_scratch_bytes(int m, int n, int k, int group,
     if (!bytes) return fail(OSH_E_INVALID, "Int4MatMul: NULL bytes");
     if (m < 0) return fail(OSH_E_INVALID, "Int4MatMul: negative sizes");
     if (const osh_status st = int4_check(n, k, group, dtype)) return st;
-    *bytes = int4_scratch(m, n, k, dtype);
+    *bytes = m && n ? int4_room(m, k, group, dtype).total : 0;
     return OSH_OK;
 }
 
@@ -342,12 +661,16 @@ OSH_API osh_status osh_int4_matmul(int m, int n, int k, int group, int dtype, co
         return fail(OSH_E_UNSUPPORTED, "Int4MatMul: %d x %d outputs", m, n);
     const long long e = elem_bytes(dtype);
     const Int4Layout l = int4_layout(n, k, group, dtype, has_zeros);
-    const size_t scratch = int4_scratch(m, n, k, dtype);
-    if (scratch && !d_scratch) return fail(OSH_E_INVALID, "Int4MatMul: NULL pointer");
+    const Int4Room room = int4_room(m, k, group, dtype);
+    if (room.total && (!d_scratch || ((uintptr_t)d_scratch & 15))) return fail(OSH_E_INVALID, "Int4MatMul: no scratch at 16-byte alignment");
     const Strided y = strided_rows(d_y, m, ldy * e, n * e), res = strided_rows(d_res, m, ldr * e, n * e);
     if (share_bytes(y, strided_rows(d_a, m, lda * e, k * e)) || share_bytes(y, Strided(d_packed, l.total)) ||
         share_bytes(y, Strided(d_bias, n * 4LL)) || (share_bytes(y, res) && !(d_y == d_res && ldy == ldr)))
         return fail(OSH_E_INVALID, "Int4MatMul: y overlaps an operand");
+    const Strided own(d_scratch, room.total);
+    if (share_bytes(own, y) || share_bytes(own, res) || share_bytes(own, strided_rows(d_a, m, lda * e, k * e)) ||
+        share_bytes(own, Strided(d_packed, l.total)) || share_bytes(own, Strided(d_bias, n * 4LL)))
+        return fail(OSH_E_INVALID, "Int4MatMul: the scratch overlaps an operand");
     Int4Args p;
     p.m = m;
     p.n = n;
@@ -364,9 +687,9 @@ OSH_API osh_status osh_int4_matmul(int m, int n, int k, int group, int dtype, co
     p.bias = d_bias;
     p.res = d_res;
     p.y = d_y;
-    if (dtype == OSH_T_F32) return int4_launch_t<float>(p, group, to_stream(s));
-    if (dtype == OSH_T_F16) return int4_launch_t<_Float16>(p, group, to_stream(s));
-    return int4_launch_t<__bf16>(p, group, to_stream(s));
+    if (dtype == OSH_T_F32) return int4_launch_t<float>(p, group, room, d_scratch, to_stream(s));
+    if (dtype == OSH_T_F16) return int4_launch_t<_Float16>(p, group, room, d_scratch, to_stream(s));
+    return int4_launch_t<__bf16>(p, group, room, d_scratch, to_stream(s));
 }
 
 }  // extern "C"

@@ -21,7 +21,6 @@ struct WinArgs {
 
 constexpr int WIN_MAX_SPLITS = 64;  // a lane a split in the join
 
-
 // l plus the eight values of w, in FP32, two an instruction.
 __device__ __forceinline__ float add8(f16x8 w, float l) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -131,22 +130,6 @@ __device__ __forceinline__ int win_page(const osh_window_attn &p, const WinSeq &
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-// N bytes (4 or 16) a lane from `from` to LDS: lane i's to dst + N i.
-template <int N = 16>
-__device__ __forceinline__ void copy_to_lds(const void *from, unsigned char *dst) {
-    const auto *src = (const __attribute__((address_space(1))) void *)from;
-    auto *to = (__attribute__((address_space(3))) void *)dst;
-    static_assert(N == 4 || N == 16);
-    if constexpr (N == 4) __builtin_amdgcn_global_load_lds(src, to, 4, 0, 0);
-    else __builtin_amdgcn_global_load_lds(src, to, 16, 0, 0);
-}
 // Of the 16 lanes of a group, lane 4 j + q reads values 4 q .. 4 q + 3 of row j; lane i
 // gets value i of rows 0..3.
 __device__ __forceinline__ s16x4 read_transposed(const unsigned char *at) {

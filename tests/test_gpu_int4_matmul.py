@@ -81,6 +81,16 @@ def test_int4_matmul(cuda, m, n, k, group, dtype):
         check(t, Int4MatMulLayer().forward(t["x"], weight(t)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("m,n,k", [(4101, 2055, 300), (2050, 4200, 264)])
+def test_many_rows(cuda, m, n, k, group, dtype):
+    print(f"int4 {m} x {n} x {k} groups of {group} {dtype}", flush=True)
+    for zeros in (False, True):
+        t = make(cuda, m, n, k, group, zeros, TYPES[dtype])
+        check(t, Int4MatMulLayer("Silu").forward(t["x"], weight(t), t["bias"], t["res"]), "Silu", t["bias"], t["res"])
+
+
 @pytest.mark.parametrize("act", [None, "Relu", "Silu", "Gelu"])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 768, 768), (24, 500, 4096), (200, 512, 1024), (129, 131, 200)])
