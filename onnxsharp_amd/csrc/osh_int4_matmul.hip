@@ -276,13 +276,35 @@ __global__ __launch_bounds__(256) void int4_prep_kernel(Int4Args p, int group, i
 
 static __device__ const uint4 int4_zero_chunk = {0, 0, 0, 0};
 
+// A group's scale s = unit * 2^e: the power of two goes into the codes, which stay exact, and
+// the unit (1/2 to 1 in size but at the ends of the type's range) into the sums.
+template <typename T>
+__device__ __forceinline__ float int4_unit(float s, float &times512) {
+    // c 2^e stays a number of T: 15 * 2^12 < 65504, and 2^-24 is f16's smallest
+    constexpr bool F16 = __is_same(T, _Float16);
+    int e = __builtin_amdgcn_frexp_expf(s);
+    e = min(max(e, F16 ? -24 : -100), F16 ? 12 : 100);
+    times512 = __builtin_amdgcn_ldexpf(512.0f, e);
+    return __builtin_amdgcn_ldexpf(s, -e);
+}
+// a / b, within 2^-23 of it.
+__device__ __forceinline__ float int4_ratio(float a, float b) {
+    const float r = __builtin_amdgcn_rcpf(b), q = a * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, b, a), r, q);
+}
+
 // A workgroup takes 32 MB WM rows by 32 NB WN outputs, a wave 32 MB by 32 NB.  The rows pass
 // through two LDS buffers of 128 k, loaded directly (chunk c of row r at c ^ r % 16); codes go
 // from memory to registers a block ahead and become 16-bit floats in front of the MFMAs that
-// take them.  A group's sum has its own registers, and is scaled into the wave's sums in FP32.
-// For 16-bit rows the zero points' part is added at the end (see Int4Prep); for FP32 ones, three
-// MFMAs a fragment of codes, the zero points come off the codes, which the vector unit has time
-// for and which loses nothing to the difference of two sums.
+// take them.
+//
+// 16-bit rows: a lane's sums, all of one output j, are kept in the unit of the group at hand
+// (int4_unit), so that the MFMAs add onto them directly, and between two groups are taken times
+// the ratio of their units: one product a sum, no registers for a group's own sums.  The zero
+// points' part is added at the end (see Int4Prep).
+// FP32 rows, three MFMAs a fragment of codes: the zero points come off the codes, which the
+// vector unit has time for and which loses nothing to the difference of two sums; a group's
+// sum has its own registers and is scaled into the wave's sums.
 template <typename T, int MB, int NB, int WM, int WN, int GS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void int4_tile_kernel(Int4Args p, Int4Prep q, int group) {
     using H8 = typename Half8<T>::type;
@@ -343,10 +365,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int4_tile_kernel(Int4Args p, 
         }
     };
     f32x16 acc[MB][NB];
+    float unit[NB], times512[NB];
 #pragma unroll
-    for (int i = 0; i < MB; i++)
+    for (int j = 0; j < NB; j++) {
+        unit[j] = 1.0f, times512[j] = 512.0f;
 #pragma unroll
-        for (int j = 0; j < NB; j++) acc[i][j] = f32x16{};
+        for (int i = 0; i < MB; i++) acc[i][j] = f32x16{};
+    }
     load_rows(0, 0);
     load_codes(0);
     int buf = 0;
@@ -367,64 +392,96 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int4_tile_kernel(Int4Args p, 
             load_codes(kb + 1);
         }
         const unsigned char *rows = lds + buf * STAGE;
-        f32x16 sum[MB][NB];
+        f32x16 sum[P > 1 ? MB : 1][P > 1 ? NB : 1];
 #pragma unroll
         for (int s = 0; s < 8; s++) {
+            const int e = s / (2 * GS);
+            const bool first = s % (2 * GS) == 0, last = s % (2 * GS) == 2 * GS - 1;
             H8 c[NB];
 #pragma unroll
             for (int j = 0; j < NB; j++) {
                 const unsigned word = reinterpret_cast<const unsigned *>(&w[j][s & 1])[s >> 1];
-                if constexpr (P > 1) codes8_less(word, zp[j][s / (2 * GS)], c[j]);
-                else codes8(word, c[j]);
+                if constexpr (P > 1) {
+                    codes8_less(word, zp[j][e], c[j]);
+                } else {
+                    if (first) {
+                        const float f = (float)sc[j][e];
+                        float t512;
+                        const float next = int4_unit<T>(f, t512), by = f != 0.0f ? int4_ratio(unit[j], next) : 1.0f;
+                        unit[j] = f != 0.0f ? next : unit[j];  // a scale of 0 has codes of 0
+                        times512[j] = t512;
+#pragma unroll
+                        for (int i = 0; i < MB; i++) acc[i][j] *= by;
+                    }
+                    codes8(word, c[j], times512[j]);
+                }
             }
 #pragma unroll
             for (int i = 0; i < MB; i++)
 #pragma unroll
-                for (int e = 0; e < P; e++) {
+                for (int u = 0; u < P; u++) {
                     const int r = 32 * (wm * MB + i) + l32;
-                    H8 x;
-                    __builtin_memcpy(&x, rows + e * (R * 256) + r * 256 + (((2 * s + hl) ^ (r & 15)) << 4), 16);
+                    const H8 x = lds_chunk<H8>(rows + u * (R * 256) + r * 256 + (((2 * s + hl) ^ (r & 15)) << 4));
+#pragma unroll
+                    for (int j = 0; j < NB; j++) {
+                        if constexpr (P > 1) sum[i][j] = mma32(x, c[j], first && u == 0 ? f32x16{} : sum[i][j]);
+                        else acc[i][j] = mma32(x, c[j], acc[i][j]);
+                    }
+                }
+            if constexpr (P > 1) {
+                if (last) {
 #pragma unroll
                     for (int j = 0; j < NB; j++)
-                        sum[i][j] = mma32(x, c[j], s % (2 * GS) == 0 && e == 0 ? f32x16{} : sum[i][j]);
-                }
-            if (s % (2 * GS) == 2 * GS - 1) {
 #pragma unroll
-                for (int j = 0; j < NB; j++) {
-                    const float f = (float)sc[j][s / (2 * GS)];
+                        for (int i = 0; i < MB; i++)
 #pragma unroll
-                    for (int i = 0; i < MB; i++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(f, sum[i][j][r], acc[i][j][r]);
+                            for (int r = 0; r < 16; r++)
+                                acc[i][j][r] = __builtin_fmaf((float)sc[j][e], sum[i][j][r], acc[i][j][r]);
                 }
             }
         }
     }
-    for (int g0 = 0; P == 1 && g0 < q.groups; g0 += 2) {
-        const int gr = g0 + hl;
-        bf16x8 x[MB], z[NB];
-        const int at_k = min(gr, q.groups - 1) * group, kb = at_k / KB, e = NG > 1 ? at_k % KB / (32 * GS) : 0;
 #pragma unroll
-        for (int i = 0; i < MB; i++) {
-            const int row = min(m0 + 32 * (wm * MB + i) + l32, p.m - 1);
-            uint4 u = q.sums[(long long)row * q.groups + min(gr, q.groups - 1)];
-            __builtin_memcpy(&x[i], &u, 16);
-        }
-#pragma unroll
-        for (int j = 0; j < NB; j++) {
-            const long long at = ((blk[j] + kb) * NG + e) * 16 + jl;
-            float f = (float)static_cast<const T *>(p.scales)[at];
-            f *= p.zeros ? (float)static_cast<const T *>(p.zeros)[at] : 8.0f;
-            if (gr >= q.groups) f = 0.0f;
-            unsigned t[3];
-            pieces3(f, t);
-            const uint4 u = {t[0] >> 16 | t[0], t[0] >> 16 | t[1], t[1] >> 16 | t[2], 0u};
-            __builtin_memcpy(&z[j], &u, 16);
-        }
+    for (int j = 0; j < NB; j++)
 #pragma unroll
         for (int i = 0; i < MB; i++)
+            if (P == 1) acc[i][j] *= unit[j];
+    // four pairs of groups at a time, so that their loads share one wait for memory
+    for (int g0 = 0; P == 1 && g0 < q.groups; g0 += 8) {
+        uint4 u[4][MB];
+        T s[4][NB], z[4][NB];
 #pragma unroll
-            for (int j = 0; j < NB; j++) acc[i][j] = mma32(x[i], z[j], acc[i][j]);
+        for (int v = 0; v < 4; v++) {
+            const int gr = min(g0 + 2 * v + hl, q.groups - 1), at_k = gr * group, kb = at_k / KB;
+            const int e = NG > 1 ? at_k % KB / (32 * GS) : 0;
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+                u[v][i] = q.sums[(long long)min(m0 + 32 * (wm * MB + i) + l32, p.m - 1) * q.groups + gr];
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                const long long at = ((blk[j] + kb) * NG + e) * 16 + jl;
+                s[v][j] = static_cast<const T *>(p.scales)[at];
+                z[v][j] = p.zeros ? static_cast<const T *>(p.zeros)[at] : (T)8.0f;
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            bf16x8 b[NB];
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                unsigned t[3];
+                pieces3(g0 + 2 * v + hl < q.groups ? (float)s[v][j] * (float)z[v][j] : 0.0f, t);
+                const uint4 c = {t[0] >> 16 | t[0], t[0] >> 16 | t[1], t[1] >> 16 | t[2], 0u};
+                __builtin_memcpy(&b[j], &c, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                bf16x8 a;
+                __builtin_memcpy(&a, &u[v][i], 16);
+#pragma unroll
+                for (int j = 0; j < NB; j++) acc[i][j] = mma32(a, b[j], acc[i][j]);
+            }
+        }
     }
     // through LDS, 32 rows of a wave at a time, to eight neighbouring outputs a lane
     constexpr int PITCH = 32 * NB + 4;
@@ -451,9 +508,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void int4_tile_kernel(Int4Args p, 
 }
 
 // Codes [n][pitch] two a byte into blocks; codes past n or k are 0 (their scales and the
-// values that meet them are 0).
-__global__ __launch_bounds__(256) void int4_pack_codes_kernel(int n, int k, const unsigned char *codes, long long pitch,
-                                                              uint4 *out) {
+// values that meet them are 0), and so are those of groups whose scale is 0.
+template <typename T>
+__global__ __launch_bounds__(256) void int4_pack_codes_kernel(int n, int k, int group, const unsigned char *codes,
+                                                              long long pitch, const T *scales, long long lds, uint4 *out) {
     const int nkb = cdiv(k, KB);
     const long long blocks = (long long)cdiv(n, 16) * nkb;
     for (long long e = blockIdx.x * 256LL + threadIdx.x; e < blocks * 64; e += gridDim.x * 256LL) {
@@ -467,7 +525,7 @@ __global__ __launch_bounds__(256) void int4_pack_codes_kernel(int n, int k, cons
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int at = k0 + 32 * t + 8 * g + i;
-                if (row >= n || at >= k) continue;
+                if (row >= n || at >= k || (float)scales[row * lds + at / group] == 0.0f) continue;
                 const unsigned code = codes[row * pitch + at / 2] >> (4 * (at & 1)) & 15u;
                 w[t] |= code << (4 * (2 * (i & 3) + (i >> 2)));  // 0..3 at even places, 4..7 at odd ones
             }
@@ -560,14 +618,10 @@ static osh_status int4_launch(const Int4Args &p, int group, const Int4Room &room
                    (long long)room.pitch, (long long)room.plane);
     }
     OSH_LAUNCH_CHECK("int4_prep_kernel");
-    const long long big = (long long)cdiv(p.m, 128) * cdiv(p.n, 256);
-    if constexpr (sizeof(T) == 2) {
-        if (big >= device_cus()) int4_tile<T, 2, 2, 2, 4, GS>(p, q, group, st);
-        else int4_tile<T, 1, 1, 2, 2, GS>(p, q, group, st);
-    } else {
-        if (big >= device_cus()) int4_tile<T, 2, 2, 1, 4, GS>(p, q, group, st);
-        else int4_tile<T, 1, 1, 2, 2, GS>(p, q, group, st);
-    }
+    // 64 x 256 tiles where they fill the card, else 64 x 64 ones: 512 x 4096 x 4096 in bf16 takes
+    // 56 us as 128 large tiles, 36 as 512 small ones; 1024 x 8192 x 8192 168 and 250
+    if ((long long)cdiv(p.m, 64) * cdiv(p.n, 256) >= device_cus()) int4_tile<T, 2, 2, 1, 4, GS>(p, q, group, st);
+    else int4_tile<T, 1, 1, 2, 2, GS>(p, q, group, st);
     OSH_LAUNCH_CHECK("int4_tile_kernel");
     return OSH_OK;
 }
@@ -620,20 +674,21 @@ OSH_API osh_status osh_int4_pack(int n, int k, int group, int dtype, const void 
         return fail(OSH_E_INVALID, "Int4MatMul: the packed weights overlap an operand");
     const hipStream_t st = to_stream(s);
     auto grid = [](size_t threads) { return dim3((unsigned)std::min<size_t>((threads + 255) / 256, 1 << 16)); };
-    OSH_LAUNCH(int4_pack_codes_kernel, grid(l.codes / 16), dim3(256), 0, st, n, k,
-               static_cast<const unsigned char *>(d_codes), (long long)ldc, static_cast<uint4 *>(d_packed));
-    OSH_LAUNCH_CHECK("int4_pack_codes_kernel");
     char *sc = static_cast<char *>(d_packed) + l.codes, *zp = sc + l.scales;
-    const unsigned char *z = static_cast<const unsigned char *>(d_zeros);
+    const unsigned char *c = static_cast<const unsigned char *>(d_codes), *z = static_cast<const unsigned char *>(d_zeros);
 #define OSH_PACK(T)                                                                                              \
-    OSH_LAUNCH(int4_pack_scales_kernel<T>, grid(l.scales / sizeof(T)), dim3(256), 0, st, n, k, group,            \
-               static_cast<const T *>(d_scales), (long long)lds, z, (long long)ldz, reinterpret_cast<T *>(sc),   \
-               reinterpret_cast<T *>(zp))
+    do {                                                                                                         \
+        const T *from = static_cast<const T *>(d_scales);                                                        \
+        OSH_LAUNCH(int4_pack_codes_kernel<T>, grid(l.codes / 16), dim3(256), 0, st, n, k, group, c, (long long)ldc, \
+                   from, (long long)lds, static_cast<uint4 *>(d_packed));                                        \
+        OSH_LAUNCH(int4_pack_scales_kernel<T>, grid(l.scales / sizeof(T)), dim3(256), 0, st, n, k, group, from,  \
+                   (long long)lds, z, (long long)ldz, reinterpret_cast<T *>(sc), reinterpret_cast<T *>(zp));     \
+    } while (0)
     if (dtype == OSH_T_F32) OSH_PACK(float);
     else if (dtype == OSH_T_F16) OSH_PACK(_Float16);
     else OSH_PACK(__bf16);
 #undef OSH_PACK
-    OSH_LAUNCH_CHECK("int4_pack_scales_kernel");
+    OSH_LAUNCH_CHECK("int4 pack kernels");
     return OSH_OK;
 }
 
