@@ -23,7 +23,14 @@ struct Kv4Args {
     void *k_stored, *v_stored;
     long long ks_stride[3], vs_stride[3], k_stored_stride[2], v_stored_stride[2];
     unsigned page_mul, page_log;  // j / page = umulhi(4 j, page_mul) >> page_log for j < 2^30
+    // many rows: the visible cache in 16 bits, and what the 16-bit kernel is told about it
+    void *k_fresh, *v_fresh;      // new tokens [tokens][kv_heads][head_dim], or NULL
+    void *k_wide, *v_wide;        // [batch * wide_blocks][kv_heads][WIDE_PAGE][head_dim]
+    int32_t *wide_table, *wide_kl;
+    int wide_blocks, wide_width;  // pages of a sequence, entries of its table
 };
+
+constexpr int WIDE_PAGE = 64;
 
 // -------------------------------------------------------------- quantization
 
@@ -95,8 +102,55 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
         }
         if (T *out = static_cast<T *>(is_v ? a.v_stored : a.k_stored)) {
             const long long *ost = is_v ? a.v_stored_stride : a.k_stored_stride;
-            if (at < 0) kept = f32x8{} + __builtin_nanf("");
-            store8(out + row * ost[0] + h * ost[1] + 8 * c, kept);
+            store8(out + row * ost[0] + h * ost[1] + 8 * c, at < 0 ? f32x8{} + __builtin_nanf("") : kept);
+        }
+        if (T *out = static_cast<T *>(is_v ? a.v_fresh : a.k_fresh))  // NaN reaches who sees the key, by the key
+            store8(out + (row * p.kv_heads + h) * p.head_dim + 8 * c,
+                   at < 0 ? f32x8{} + (is_v ? 0.0f : __builtin_nanf("")) : kept);
+    }
+}
+
+// What the cached keys and values that any query sees stand for, rounded to T, into pages of
+// their own, and the table of those: first the blocks of the sinks, then those of the window.
+// blockIdx.y is the sequence, blockIdx.x deals out its pages.
+template <typename T>
+__global__ __launch_bounds__(256) void kv4_expand_kernel(Kv4Args a, int group_log) {
+    const osh_window_attn &p = a.w.p;
+    const int b = blockIdx.y, d = p.head_dim, chunks = d / 8;
+    const WinSeq sq = win_seq(p, b);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.wide_kl[b] = sq.ok ? sq.kl : -1;
+    if (!sq.ok || sq.ql == 0) return;
+    const WinKeys keys = win_keys(p, sq, 0, sq.ql - 1);
+    const int sink_blocks = cdiv(min(p.sinks, p.max_kv), WIDE_PAGE);
+    const int first = max(keys.lo / WIDE_PAGE, sink_blocks), count = cdiv(sq.kl, WIDE_PAGE);
+    for (int at = blockIdx.x; at < a.wide_blocks; at += gridDim.x) {
+        const int block = at < sink_blocks ? at : first + at - sink_blocks;
+        if (block >= count) return;
+        const long long page = (long long)b * a.wide_blocks + at;
+        if (threadIdx.x == 0) a.wide_table[(long long)b * a.wide_width + block] = (int)page;
+        for (int e = threadIdx.x; e < p.kv_heads * WIDE_PAGE * chunks; e += 256) {
+            const int c = e % chunks, in = e / chunks % WIDE_PAGE, h = e / chunks / WIDE_PAGE;
+            const int j = block * WIDE_PAGE + in;
+            if (j >= sq.past || (j < keys.lo && j >= p.sinks)) continue;
+            const int slot = j % p.page, id = p.d_table[b * p.table_stride + j / p.page];
+            f32x8 k = f32x8{} + __builtin_nanf(""), v = {};
+            if ((unsigned)id < (unsigned)p.pages) {
+                auto load = [&](const void *codes, const int64_t *st, const void *pairs, const long long *pst) {
+                    const unsigned w = *reinterpret_cast<const unsigned *>(static_cast<const char *>(codes) + id * st[0] +
+                                                                           slot * st[1] + h * st[2] + 4 * c);
+                    const T *pair = static_cast<const T *>(pairs) + id * pst[0] + slot * pst[1] + h * pst[2] +
+                                    2 * (8 * c >> group_log);
+                    f32x8 f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) f[i] = __builtin_fmaf((float)pair[0], (float)(w >> (4 * i) & 15u), (float)pair[1]);
+                    return f;
+                };
+                k = load(p.d_k_pages, p.k_stride, a.ks, a.ks_stride);
+                v = load(p.d_v_pages, p.v_stride, a.vs, a.vs_stride);
+            }
+            const long long to = ((page * p.kv_heads + h) * WIDE_PAGE + in) * d + 8 * c;
+            store8(static_cast<T *>(a.k_wide) + to, k);
+            store8(static_cast<T *>(a.v_wide) + to, v);
         }
     }
 }
@@ -549,31 +603,87 @@ static osh_status kv4_launch_g(const Kv4Args &a, unsigned units, hipStream_t st)
 }
 
 template <typename T>
-static osh_status kv4_launch(const Kv4Args &a, int group, unsigned units, hipStream_t st) {
+static osh_status kv4_wide(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
+    const osh_status s = group == 32   ? kv4_append<T, 4>(a, st)
+                         : group == 64 ? kv4_append<T, 8>(a, st)
+                                       : kv4_append<T, 16>(a, st);
+    if (s) return s;
+    const int x = std::min(a.wide_blocks, std::max(1, 65536 / a.w.p.batch));
+    OSH_LAUNCH(kv4_expand_kernel<T>, dim3((unsigned)x, (unsigned)a.w.p.batch), dim3(256), 0, st, a, __builtin_ctz(group));
+    OSH_LAUNCH_CHECK("kv4_expand_kernel");
+    return win_run(wide, units, st);
+}
+
+template <typename T>
+static osh_status kv4_launch(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
+    if (a.wide_blocks) return kv4_wide<T>(a, wide, group, units, st);
     if (group == 32) return kv4_launch_g<T, 1>(a, units, st);
     if (group == 64) return kv4_launch_g<T, 2>(a, units, st);
     return kv4_launch_g<T, 4>(a, units, st);
 }
 
-static osh_status kv4_plan(const osh_kv4_attn *p, WinArgs &a, size_t &scratch) {
+// Where the parts of the scratch lie: a.w's own or, with many rows, `wide`, the 16-bit call.
+struct Kv4Room {
+    bool wide;
+    size_t part, fresh, page, table, kl, total;  // bytes, of one tensor of K and V
+};
+
+// Rows of a key head from which the visible cache is first expanded to 16 bits, and the room
+// that may take.
+constexpr int WIDE_ROWS = 512;
+constexpr size_t WIDE_MAX = (size_t)16 << 30;
+
+static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, Kv4Room &room) {
     if (!p) return fail(OSH_E_INVALID, "Kv4Attention: NULL parameters");
-    if (const osh_status st = win_plan(&p->w, a, scratch)) return st;
+    WinArgs &a = args.w;
+    room = {};
+    args = {};
+    if (const osh_status st = win_plan(&p->w, a, room.part)) return st;
     if (p->group != 32 && p->group != 64 && p->group != 128)
         return fail(OSH_E_UNSUPPORTED, "Kv4Attention: groups of %d (32, 64 or 128)", p->group);
     if (p->w.head_dim % p->group)
         return fail(OSH_E_UNSUPPORTED, "Kv4Attention: heads of %d in groups of %d", p->w.head_dim, p->group);
+    if (p->w.batch > 65535) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: %d sequences", p->w.batch);
     const int rows = p->w.max_q * a.group;
+    auto align = [](size_t n) { return (n + 255) / 256 * 256; };
+    if (rows >= WIDE_ROWS && p->w.batch) {
+        const long long most = cdiv(p->w.max_kv, WIDE_PAGE), sinks = cdiv(std::min(p->w.sinks, p->w.max_kv), WIDE_PAGE);
+        const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window - 1 + p->w.max_q);
+        args.wide_blocks = (int)std::min(most, sinks + (span + WIDE_PAGE - 1) / WIDE_PAGE + 1);
+        args.wide_width = (int)most;
+        osh_window_attn w = p->w;
+        w.page = WIDE_PAGE;
+        w.table_width = args.wide_width;
+        w.table_stride = args.wide_width;
+        const long long pages = (long long)w.batch * args.wide_blocks, head = (long long)w.head_dim;
+        w.pages = (int)std::min<long long>(pages, INT_MAX);
+        w.k_stride[0] = w.v_stride[0] = w.kv_heads * WIDE_PAGE * head;
+        w.k_stride[1] = w.v_stride[1] = head;
+        w.k_stride[2] = w.v_stride[2] = WIDE_PAGE * head;
+        w.k_new_stride[0] = w.v_new_stride[0] = w.kv_heads * head;
+        w.k_new_stride[1] = w.v_new_stride[1] = head;
+        if (const osh_status st = win_plan(&w, wide, room.part)) return st;
+        room.part = align(room.part);
+        room.fresh = align((size_t)w.tokens * w.kv_heads * head * 2);
+        room.table = align((size_t)w.batch * args.wide_width * 4);
+        room.kl = align((size_t)w.batch * 4);
+        const double bytes = 4.0 * pages * w.kv_heads * WIDE_PAGE * head;
+        room.wide = pages <= INT_MAX && w.k_stride[0] <= INT_MAX && bytes <= (double)WIDE_MAX;
+        room.page = room.wide ? (size_t)bytes / 2 : 0;
+        room.total = room.part + 2 * room.fresh + 2 * room.page + room.table + room.kl;
+        if (room.wide) return OSH_OK;
+        args.wide_blocks = 0;
+    }
     a.tile_rows = 16;
     a.tiles = cdiv(rows, 16);
     const long long units = (long long)p->w.batch * p->w.kv_heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: too many row blocks (%lld)", units);
-    if (p->w.batch > 65535) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: %d sequences", p->w.batch);
     const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window + p->w.sinks + 16 / a.group);
     const long long want = units ? std::max(1LL, 2LL * device_cus() / units) : 1;
     a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
     a.wide = false;
     const long long parts = a.splits > 1 ? units * a.splits : 0;
-    scratch = (size_t)parts * a.tile_rows * (p->w.head_dim + 2) * 4;
+    room.part = room.total = (size_t)parts * a.tile_rows * (p->w.head_dim + 2) * 4;
     return OSH_OK;
 }
 
@@ -583,18 +693,24 @@ extern "C" {
 
 OSH_API osh_status osh_kv4_attention_scratch_bytes(const osh_kv4_attn *p, size_t *bytes) {
     if (!bytes) return fail(OSH_E_INVALID, "Kv4Attention: NULL bytes");
-    WinArgs a;
-    return kv4_plan(p, a, *bytes);
+    Kv4Args a;
+    WinArgs wide;
+    Kv4Room room;
+    const osh_status st = kv4_plan(p, a, wide, room);
+    *bytes = room.total;
+    return st;
 }
 
 OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *q, void *d_scratch, osh_stream s) {
     Kv4Args a;
-    size_t scratch = 0;
-    if (const osh_status st = kv4_plan(q, a.w, scratch)) return st;
+    WinArgs wide;
+    Kv4Room room;
+    if (const osh_status st = kv4_plan(q, a, wide, room)) return st;
+    const size_t scratch = room.total;
     const osh_window_attn *p = &q->w;
     if (p->batch == 0 || p->max_q == 0 || p->tokens == 0) return OSH_OK;
     if (!p->d_q || !p->d_k_new || !p->d_v_new || !p->d_o || !p->d_k_pages || !p->d_v_pages || !p->d_table ||
-        !p->d_cu || !p->d_kl || !q->d_k_scales || !q->d_v_scales || (scratch && !d_scratch) ||
+        !p->d_cu || !p->d_kl || !q->d_k_scales || !q->d_v_scales || (scratch && (!d_scratch || ((uintptr_t)d_scratch & 15))) ||
         !q->d_k_stored != !q->d_v_stored)
         return fail(OSH_E_INVALID, "Kv4Attention: NULL pointer");
     const long long d = p->head_dim, groups = d / q->group;
@@ -643,9 +759,20 @@ OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *q, void *d_scratch, osh
         for (const Strided &t : in)
             if (share_bytes(out[i], t)) return fail(OSH_E_INVALID, "Kv4Attention: an output overlaps an operand");
     }
-    const long long units = (long long)p->batch * p->kv_heads * a.w.tiles;
-    a.w.part_ml = static_cast<float *>(d_scratch);
-    a.w.part_o = a.w.part_ml + units * a.w.splits * a.w.tile_rows * 2;
+    WinArgs &call = room.wide ? wide : a.w;
+    const long long units = (long long)p->batch * p->kv_heads * call.tiles;
+    call.part_ml = static_cast<float *>(d_scratch);
+    call.part_o = call.part_ml + units * call.splits * call.tile_rows * 2;
+    if (room.wide) {
+        char *at = static_cast<char *>(d_scratch) + room.part;
+        auto take = [&](size_t n) { return at += n, at - n; };
+        wide.p.d_k_new = a.k_fresh = take(room.fresh);
+        wide.p.d_v_new = a.v_fresh = take(room.fresh);
+        wide.p.d_k_pages = a.k_wide = take(room.page);
+        wide.p.d_v_pages = a.v_wide = take(room.page);
+        wide.p.d_table = a.wide_table = reinterpret_cast<int32_t *>(take(room.table));
+        wide.p.d_kl = a.wide_kl = reinterpret_cast<int32_t *>(take(room.kl));
+    }
     a.page_log = 0;
     while ((1LL << a.page_log) < p->page) a.page_log++;
     a.page_mul = (unsigned)(((1LL << (30 + a.page_log)) + p->page - 1) / p->page);
@@ -656,8 +783,8 @@ OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *q, void *d_scratch, osh
     for (int i = 0; i < 3; i++) a.ks_stride[i] = q->k_scale_stride[i], a.vs_stride[i] = q->v_scale_stride[i];
     for (int i = 0; i < 2; i++)
         a.k_stored_stride[i] = q->k_stored_stride[i], a.v_stored_stride[i] = q->v_stored_stride[i];
-    return p->dtype == OSH_T_F16 ? kv4_launch<_Float16>(a, q->group, (unsigned)units, to_stream(s))
-                                 : kv4_launch<__bf16>(a, q->group, (unsigned)units, to_stream(s));
+    return p->dtype == OSH_T_F16 ? kv4_launch<_Float16>(a, wide, q->group, (unsigned)units, to_stream(s))
+                                 : kv4_launch<__bf16>(a, wide, q->group, (unsigned)units, to_stream(s));
 }
 
 }  // extern "C"

@@ -195,6 +195,9 @@ static osh_status win_join(const WinArgs &a, unsigned units, hipStream_t st) {
     return OSH_OK;
 }
 
+// The attention over 16-bit pages of a planned and checked call (osh_window_attn.hip).
+osh_status win_run(const WinArgs &a, unsigned units, hipStream_t st);
+
 // Row blocks, splits and scratch of a call.
 static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch) {
     if (!p) return fail(OSH_E_INVALID, "WindowAttention: NULL parameters");

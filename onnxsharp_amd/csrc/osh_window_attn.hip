@@ -574,6 +574,10 @@ static osh_status win_launch_t(const WinArgs &a, unsigned units, hipStream_t st)
     return win_launch<T, 256, 4>(a, units, st);
 }
 
+osh_status win_run(const WinArgs &a, unsigned units, hipStream_t st) {
+    return a.p.dtype == OSH_T_F16 ? win_launch_t<_Float16>(a, units, st) : win_launch_t<__bf16>(a, units, st);
+}
+
 }  // namespace osh
 
 extern "C" {
@@ -630,8 +634,7 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
     const long long units = (long long)p->batch * p->kv_heads * a.tiles;
     a.part_ml = static_cast<float *>(d_scratch);
     a.part_o = a.part_ml + units * a.splits * a.tile_rows * 2;
-    return p->dtype == OSH_T_F16 ? win_launch_t<_Float16>(a, (unsigned)units, to_stream(s))
-                                 : win_launch_t<__bf16>(a, (unsigned)units, to_stream(s));
+    return win_run(a, (unsigned)units, to_stream(s));
 }
 
 }  // extern "C"

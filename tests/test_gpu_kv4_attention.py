@@ -8,7 +8,12 @@ of it instead, at most 8 of it a key and 1 / (largest w) of it in all.  Scores a
 at most d exact products and three more terms a group, of sizes S = (sum |q| (15 scale + |lo|))
 times the softmax's scale: (d / 8 + 16) 2^-24 S is below 2^-13 for S < 100 and d <= 256; sums
 and joins of weights and values take at most one rounding a key of a lane and one a join:
-2^-11 sum w (|lo| + 15 scale) covers them."""
+2^-11 sum w (|lo| + 15 scale) covers them.
+
+Where max_q times the heads of a group reaches 512, keys and values are first rounded to the
+type, half a step each: a score is off by e_j <= h sum |q| |k| times the softmax's scale, so a
+weight by a factor within exp(+-2 E), E the largest e_j seen: (exp(2 E) - 1) (sum w |v| + |o|);
+a value by h |v|, and the weights are rounded against values, not codes: 2 h sum w |v|."""
 import pytest
 import torch
 
@@ -107,6 +112,7 @@ def ref(s, window, sinks, scale=None):
         return ((p[..., 1:] + p[..., :1] * c).flatten(-2), p[..., 0].abs().repeat_interleave(group, -1),
                 p[..., 1].abs().repeat_interleave(group, -1))
 
+    wide = max(ql for ql, _ in s["lens"]) * rep >= 512
     c = 0
     for i, (ql, kl) in enumerate(s["lens"]):
         at = torch.arange(kl)
@@ -131,6 +137,11 @@ def ref(s, window, sinks, scale=None):
             b = half * ((w @ hv).abs() + 8 * (w @ hs)) + 2.0 ** -11 * (w @ (hl + 15 * hs)) + torch.finfo(t).smallest_normal
             if t == torch.float16 and kl:
                 b = b + seen.sum(1, keepdim=True) * 2.0 ** -21 * hs.amax() * w.amax(1, keepdim=True)
+            if wide and ql:
+                size = s["q"][c:c + ql, h].double().abs() @ torch.where(used, k[:, u].abs(), 0.0).T.contiguous()
+                off = (half * scale * size).masked_fill(~seen, 0.0).amax(1, keepdim=True)
+                wv = w @ hv.abs()
+                b = b + 2 * half * wv + torch.expm1(2 * off) * (wv + (w @ hv).abs())
             bound[c:c + ql, h] = b
         c += ql
     return o, bound, (kc, vc, ks, vs), stored
@@ -193,6 +204,25 @@ def test_long_histories(cuda, d, group):
 def test_long_prompts(cuda):
     check(make(cuda, 8, 2, 128, 64, 64, [(1100, 1100), (300, 1500)], "bf16", 4), 256, 4)
     check(make(cuda, 4, 4, 64, 32, 16, [(600, 600)], "f16", 5), None, 0)
+
+
+# hq, hkv, d, group, page, (new, whole), window, sinks: rows enough for the 16-bit kernel
+WIDE_CASES = [
+    (4, 1, 64, 32, 16, [(130, 130), (33, 100), (1, 90), (0, 5), (128, 900)], 100, 4),
+    (8, 1, 128, 64, 7, [(70, 500), (64, 64), (3, 40)], 33, 130),
+    (16, 2, 96, 32, 64, [(64, 1000), (64, 65)], None, 0),
+    (4, 1, 256, 128, 128, [(128, 2000), (1, 1)], 1, 70),
+    (64, 1, 32, 32, 16, [(8, 3000), (8, 8), (2, 700)], 1000, 3),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(WIDE_CASES)))
+def test_many_rows(cuda, case, dtype):
+    hq, hkv, d, group, page, lens, window, sinks = WIDE_CASES[case]
+    print(f"attention over 4 bits {WIDE_CASES[case]} {dtype}", flush=True)
+    check(make(cuda, hq, hkv, d, group, page, lens, dtype, case), window, sinks)
+    check(make(cuda, hq, hkv, d, group, page, lens, dtype, case), window, sinks, slack=300)
 
 
 def test_bounds_above_the_lengths(cuda):
@@ -292,8 +322,44 @@ def test_bad_pages(cuda):
     assert last >= 0
 
 
+def test_bad_pages_under_many_rows(cuda):
+    s = make(cuda, 8, 1, 64, 64, 16, [(70, 300), (5, 290), (1, 97)], "f16", 41)
+    good = run(s, 32, 0)
+    before = copies(s["cache"])
+    s["table"][0, 14] = s["cache"].k_codes.shape[0]  # positions 224..239, 230 on new: queries 230..270 see some of them
+    s["table"][0, 18] = -1                           # positions 288..299: the last twelve queries, new there
+    s["table"][1, 0] = -7                            # outside sequence 1's window
+    s["table"][2, 6] = 1 << 30                       # sequence 2's new token itself
+    stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+    out = run(s, 32, 0, stored=stored)
+    pos = torch.arange(230, 300, device=cuda)
+    nan = (pos - 32 < 239) & (pos > 223) | (pos >= 288)
+    assert torch.equal(out[:70].isnan().all(2).all(1), nan) and torch.equal(out[:70].isnan().any(2).any(1), nan)
+    assert same(out[:70][~nan], good[:70][~nan]) and same(out[70:75], good[70:75]) and out[75].isnan().all()
+    for t in stored:
+        assert t[58:70].isnan().all() and t[75].isnan().all() and t[:10].isnan().all()
+        assert t[10:58].isfinite().all() and t[70:75].isfinite().all()
+    for got, want in zip(parts(s["cache"]), before):
+        assert same(got, want)
+
+
+def test_lengths_that_contradict_under_many_rows(cuda):
+    s = make(cuda, 8, 1, 64, 32, 16, [(2, 50), (70, 160), (1, 20)], "bf16", 42)
+    good = run(s, 32, 2)
+    before = copies(s["cache"])
+    for kl in (2, 10 ** 6, -1, 161, 12 * 16):  # 161: above the bound
+        s["kl"][1] = kl
+        stored = torch.empty_like(s["k"]), torch.empty_like(s["v"])
+        out = run(s, 32, 2, stored=stored)
+        assert out[2:72].isnan().all() and same(out[:2], good[:2]) and same(out[72:], good[72:])
+        assert stored[0][2:72].isnan().all() and stored[0][:2].isfinite().all() and stored[1][72:].isfinite().all()
+        for got, want in zip(parts(s["cache"]), before):
+            assert same(got, want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("d,group,ql,kl", [(64, 32, 3, 40), (128, 64, 90, 130), (128, 32, 60, 90), (256, 128, 60, 90)])
+@pytest.mark.parametrize("d,group,ql,kl", [(64, 32, 3, 40), (128, 64, 90, 130), (128, 32, 60, 90), (256, 128, 60, 90),
+                                           (64, 64, 300, 340)])
 def test_keys_that_are_not_finite(cuda, d, group, ql, kl, dtype):
     s, window = make(cuda, 4, 2, d, group, 16, [(ql, kl)], dtype, d + ql), 24
     past = kl - ql
@@ -386,7 +452,8 @@ def test_the_way_tokens_came_does_not_matter(cuda):
         assert all(same(x, y) for x, y in zip(c, caches[0]))
 
 
-@pytest.mark.parametrize("lens,window", [([(1, 500), (1, 77), (1, 1)], 100), ([(150, 400), (1, 90), (40, 40)], 64)])
+@pytest.mark.parametrize("lens,window", [([(1, 500), (1, 77), (1, 1)], 100), ([(100, 400), (1, 90), (40, 40)], 64),
+                                         ([(150, 400), (1, 90), (40, 40)], 64)])
 def test_alone_and_in_a_batch(cuda, lens, window):
     # a sequence's bits under the same bounds and splits
     s = make(cuda, 8, 2, 128, 64, 16, lens, "bf16", 31)
