@@ -247,8 +247,9 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     T *o = static_cast<T *>(p.d_o);
     const int my_row = min(r0 + jl, rows - 1), my_tok = my_row / G, my_head = h * G + my_row % G;
 
-    // queries: lane (jl, g) holds values 32 s + 8 g + {0, 2, 4, 6, 1, 3, 5, 7} of row jl,
-    // the order of codes8, and their sums over a group
+    // queries: step t of group e takes of lane (jl, g) the 8 values from 32 GS e + 8 (GS g + t) on
+    // of row jl, so that the lane's codes of a group are GS words in a row, in codes8's order;
+    // and their sums over a group
     H8 q[CP];
     float qs[NG];
     {
@@ -259,7 +260,8 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
 #pragma unroll
         for (int s = 0; s < CP; s++) {
             H8 x = {};
-            if (32 * s < d) __builtin_memcpy(&x, qr + 32 * s + 8 * g, 16);
+            const int from = 32 * GS * (s / GS) + 8 * (GS * g + s % GS);
+            if (from < d) __builtin_memcpy(&x, qr + from, 16);
 #pragma unroll
             for (int i = 0; i < 8; i++) qs[s / GS] += (float)x[i];
             q[s] = __builtin_shufflevector(x, x, 0, 2, 4, 6, 1, 3, 5, 7);
@@ -336,11 +338,18 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     const int last_chunk = d / 32 - 1;  // slots of no value hold a copy of it, and meet queries of 0
     auto load_codes = [&](int buf) {
         unsigned char *kt = mine + buf * 2 * TILE, *vt = kt + TILE;
+        const char *kr[CP], *vr[CP];  // all of them before the first copy: one wait for the LDS
+#pragma unroll
+        for (int i = 0; i < CP; i++) {
+            const int key = i * KPI + lane / CP;
+            kr[i] = (const char *)__shfl(k_row, key), vr[i] = (const char *)__shfl(v_row, key);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < CP; i++) {
             const int key = i * KPI + lane / CP, slot = lane % CP;
-            copy_to_lds<16>((const char *)__shfl(k_row, key) + 16 * min(slot ^ k_swizzle(key), last_chunk), kt + i * 1024);
-            copy_to_lds<16>((const char *)__shfl(v_row, key) + 16 * min(slot ^ v_swizzle(key), last_chunk), vt + i * 1024);
+            copy_to_lds<16>(kr[i] + 16 * min(slot ^ k_swizzle(key), last_chunk), kt + i * 1024);
+            copy_to_lds<16>(vr[i] + 16 * min(slot ^ v_swizzle(key), last_chunk), vt + i * 1024);
         }
     };
     constexpr int SC_LOADS = 2 * NG;
@@ -397,33 +406,49 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
+    // products of the queries with a step's codes of K: they need no scales
+    f32x4 prod[4][NG];
+    auto multiply = [&](int buf) {
+        const unsigned char *kt = mine + buf * 2 * TILE;
+        unsigned w[4][CP];
+#pragma unroll
+        for (int bl = 0; bl < 4; bl++) {
+            const int key = 16 * (jl >> 2) + 4 * bl + (jl & 3);
+#pragma unroll
+            for (int e = 0; e < NG; e++) {
+                const int chunk = e * GS + g * GS / 4;
+                const unsigned *from = static_cast<const unsigned *>(__builtin_assume_aligned(
+                    kt + key * (CP * 16) + ((chunk ^ k_swizzle(key)) << 4) + (g * GS * 4 & 15), GS * 4));
+#pragma unroll
+                for (int t = 0; t < GS; t++) w[bl][e * GS + t] = from[t];
+            }
+        }
+#pragma unroll
+        for (int bl = 0; bl < 4; bl++)
+#pragma unroll
+            for (int e = 0; e < NG; e++)
+#pragma unroll
+                for (int t = 0; t < GS; t++) {
+                    H8 k;
+                    codes8(w[bl][e * GS + t], k);
+                    prod[bl][e] = mma16(k, q[e * GS + t], t == 0 ? f32x4{0, 0, 0, 0} : prod[bl][e]);
+                }
+    };
     auto compute = [&](int st, int buf) {
-        const unsigned char *kt = mine + buf * 2 * TILE, *vt = kt + TILE;
+        const unsigned char *vt = mine + buf * 2 * TILE + TILE;
         float s[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
 #pragma unroll
-        for (int bl = 0; bl < 4; bl++) {
-            const int key = 16 * (jl >> 2) + 4 * bl + (jl & 3);
-            const unsigned char *row = kt + key * (CP * 16) + 4 * g;
+        for (int bl = 0; bl < 4; bl++)
 #pragma unroll
-            for (int e = 0; e < NG; e++) {
-                if (NG > 2) __builtin_amdgcn_sched_barrier(0);
-                f32x4 c = {0, 0, 0, 0};
-#pragma unroll
-                for (int t = 0; t < GS; t++) {
-                    H8 k;
-                    codes8(*reinterpret_cast<const unsigned *>(row + (((e * GS + t) ^ k_swizzle(key)) << 4)), k);
-                    c = mma16(k, q[e * GS + t], c);
-                }
+            for (int e = 0; e < NG; e++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float2 kp = read_pair(kpair + e * 64 + 16 * g + 4 * bl + r);
-                    s[4 * bl + r] = __builtin_fmaf(kp.x, c[r], s[4 * bl + r]);
+                    s[4 * bl + r] = __builtin_fmaf(kp.x, prod[bl][e][r], s[4 * bl + r]);
                     s[4 * bl + r] = __builtin_fmaf(kp.y, qs[e], s[4 * bl + r]);
                 }
-            }
-        }
         const int v0 = st * 64, j0 = keys.at(v0), j1 = keys.at(v0 + 63);
         const bool all = v0 + 63 < nv && j1 <= pos0 &&
                          (j1 < p.sinks || (v0 >= keys.sink_end && j0 > pos1 - p.window));
@@ -512,11 +537,13 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
             load_ids(st + 2 * WAVES);
             load_codes(buf ^ 1);
             wait_loads<2 * CP + 1>();
+            multiply(buf);
             convert(now_in, now_bad);
             load_scales();
             compute(st, buf);
         }
         wait_loads<0>();
+        multiply(buf);
         convert(in, bad);
         compute(st, buf);
     }
