@@ -215,8 +215,13 @@ __device__ __forceinline__ float2 read_pair(const float2 *from) {
     return float2{__uint_as_float(u[0]), __uint_as_float(u[1])};
 }
 
-template <typename T, int CP, int GS, int WAVES>
+// With SUB 2 or 4 at most 16 / SUB rows are there, and column jl of the products stands for row
+// jl % (16 / SUB) over every SUB-th part of each 16 keys: a lane has KPL = 16 / SUB scores a
+// step in place of 16, of which most would belong to no row.  Its weights of other keys are 0,
+// and its columns' maxima and sums are joined with those of the waves.
+template <typename T, int CP, int GS, int WAVES, int SUB>
 __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv4Args args) {
+    constexpr int RP = 16 / SUB, KPL = 16 / SUB;
     constexpr int NG = CP / GS;        // groups of a head
     constexpr int DP = 32 * CP, OB = 2 * CP, KPI = 64 / CP;
     constexpr int TILE = 64 * CP * 16;
@@ -238,14 +243,15 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     id /= a.tiles;
     const int h = id % p.kv_heads, b = id / p.kv_heads;
     const WinSeq sq = win_seq(p, b);
-    const int rows = sq.ql * G, r0 = tile * 16;
+    const int rows = sq.ql * G, r0 = tile * RP;
     if (!sq.ok) {
         if (tile == 0 && split == 0) win_fill_nan<T>(p, sq, h, G, tid, 64 * WAVES);
         return;
     }
     if (r0 >= rows) return;
     T *o = static_cast<T *>(p.d_o);
-    const int my_row = min(r0 + jl, rows - 1), my_tok = my_row / G, my_head = h * G + my_row % G;
+    const int sub = jl / RP;
+    const int my_row = min(r0 + jl % RP, rows - 1), my_tok = my_row / G, my_head = h * G + my_row % G;
 
     // queries: step t of group e takes of lane (jl, g) the 8 values from 32 GS e + 8 (GS g + t) on
     // of row jl, so that the lane's codes of a group are GS words in a row, in codes8's order;
@@ -272,7 +278,7 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
             qs[e] += __shfl_xor(qs[e], 32);
         }
     }
-    const int tok0 = r0 / G, tok1 = min(r0 + 15, rows - 1) / G;
+    const int tok0 = r0 / G, tok1 = min(r0 + RP - 1, rows - 1) / G;
     const WinKeys keys = win_keys(p, sq, tok0, tok1);
     const int nv = keys.count;
     const int steps = cdiv(nv, 64), per = cdiv(steps, a.splits);
@@ -436,33 +442,39 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     };
     auto compute = [&](int st, int buf) {
         const unsigned char *vt = mine + buf * 2 * TILE + TILE;
-        float s[16];
+        float s[KPL];
+        const int mine16 = 16 * g + KPL * sub;  // this lane's keys of the step
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+        for (int i = 0; i < KPL; i++) s[i] = 0.0f;
 #pragma unroll
-        for (int bl = 0; bl < 4; bl++)
+        for (int e = 0; e < NG; e++)
 #pragma unroll
-            for (int e = 0; e < NG; e++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float2 kp = read_pair(kpair + e * 64 + 16 * g + 4 * bl + r);
-                    s[4 * bl + r] = __builtin_fmaf(kp.x, prod[bl][e][r], s[4 * bl + r]);
-                    s[4 * bl + r] = __builtin_fmaf(kp.y, qs[e], s[4 * bl + r]);
+            for (int i = 0; i < KPL; i++) {
+                float c = prod[i / 4][e][i % 4];
+                if constexpr (SUB == 2) c = sub ? prod[2 + i / 4][e][i % 4] : c;
+                if constexpr (SUB == 4) {
+                    const float hi = sub & 1 ? prod[3][e][i] : prod[2][e][i];
+                    c = sub & 1 ? prod[1][e][i] : c;
+                    c = sub & 2 ? hi : c;
                 }
+                const float2 kp = read_pair(kpair + e * 64 + mine16 + i);
+                s[i] = __builtin_fmaf(kp.x, c, s[i]);
+                s[i] = __builtin_fmaf(kp.y, qs[e], s[i]);
+            }
         const int v0 = st * 64, j0 = keys.at(v0), j1 = keys.at(v0 + 63);
         const bool all = v0 + 63 < nv && j1 <= pos0 &&
                          (j1 < p.sinks || (v0 >= keys.sink_end && j0 > pos1 - p.window));
         if (!all) {
-            const int mine0 = v0 + 16 * g, hi = v_hi - mine0, lo = v_lo - mine0, sink = v_sink - mine0;
+            const int mine0 = v0 + mine16, hi = v_hi - mine0, lo = v_lo - mine0, sink = v_sink - mine0;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
+            for (int i = 0; i < KPL; i++) {
                 const bool hidden = (i > hi) | ((i < lo) & (i >= sink));
                 s[i] = hidden ? -__builtin_inff() : s[i];
             }
         }
         float top = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = __builtin_fmaxf(top, s[i]);
+        for (int i = 1; i < KPL; i++) top = __builtin_fmaxf(top, s[i]);
         top = __builtin_fmaxf(top, __shfl_xor(top, 16));
         top = __builtin_fmaxf(top, __shfl_xor(top, 32));
         if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
@@ -492,23 +504,36 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
         }
         const float ref = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < KPL; i++) {
             s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
             l += s[i];
         }
 #pragma unroll
         for (int e = 0; e < NG; e++) {
-            if (NG > 2) __builtin_amdgcn_sched_barrier(0);
-            f32x8 w0, w1;
+            if (NG > 2 && SUB == 1) __builtin_amdgcn_sched_barrier(0);
+            // weights in the order of codes8: of 8 keys the even ones, then the odd ones
+            float w[KPL];
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float2 vp = read_pair(vpair + e * 64 + 16 * g + i);
-                const int k = (i & 7) >> 1 | (i & 1) << 2;  // the order of codes8
-                if (i < 8) w0[k] = s[i] * vp.x;
-                else w1[k] = s[i] * vp.x;
+            for (int i = 0; i < KPL; i++) {
+                const float2 vp = read_pair(vpair + e * 64 + mine16 + i);
+                w[i] = s[i] * vp.x;
                 zsum[e] = __builtin_fmaf(s[i], vp.y, zsum[e]);
             }
-            const H8 p0 = __builtin_convertvector(w0, H8), p1 = __builtin_convertvector(w1, H8);
+            unsigned pw[8];
+            auto two = [&](int i, int j) {
+                typedef T T2 __attribute__((ext_vector_type(2)));
+                const T2 v = {(T)w[i], (T)w[j]};
+                return __builtin_bit_cast(unsigned, v);
+            };
+#pragma unroll
+            for (int i = 0; i < 8; i++) {  // registers 0..3 are of the first 8 keys
+                if constexpr (SUB == 1) pw[i] = two(8 * (i >> 2) + 4 * (i & 1) + (i >> 1 & 1), 8 * (i >> 2) + 4 * (i & 1) + (i >> 1 & 1) + 2);
+                if constexpr (SUB == 2) pw[i] = sub == i >> 2 ? two(4 * (i & 1) + (i >> 1 & 1), 4 * (i & 1) + (i >> 1 & 1) + 2) : 0u;
+                if constexpr (SUB == 4) pw[i] = sub == 2 * (i >> 2) + (i & 1) ? two(i >> 1 & 1, (i >> 1 & 1) + 2) : 0u;
+            }
+            H8 p0, p1;
+            __builtin_memcpy(&p0, pw, 16);
+            __builtin_memcpy(&p1, pw + 4, 16);
             accz[e] = mma16(minus8, p0, accz[e]);
             accz[e] = mma16(minus8, p1, accz[e]);
 #pragma unroll
@@ -571,41 +596,48 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
         *reinterpret_cast<f32x4 *>(os + (wave * 16 + jl) * OP + 16 * i + 4 * g) = f;
     }
     __syncthreads();
-    for (int e = tid; e < 16 * DP; e += 64 * WAVES) {
+    for (int e = tid; e < RP * DP; e += 64 * WAVES) {
         const int r = e / DP, c = e % DP, row = r0 + r;
         if (row >= rows || c >= d) continue;
         float mm = ml[r * 2];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) mm = __builtin_fmaxf(mm, ml[(w * 16 + r) * 2]);
+        for (int w = 1; w < WAVES * SUB; w++) mm = __builtin_fmaxf(mm, ml[(w * RP + r) * 2]);
         const float base = mm == -__builtin_inff() ? 0.0f : mm;
         float sum = 0.0f, ll = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float f = __builtin_amdgcn_exp2f(ml[(w * 16 + r) * 2] - base);
-            ll += f * ml[(w * 16 + r) * 2 + 1];
-            sum += f * os[(w * 16 + r) * OP + c];
+        for (int w = 0; w < WAVES * SUB; w++) {
+            const float f = __builtin_amdgcn_exp2f(ml[(w * RP + r) * 2] - base);
+            ll += f * ml[(w * RP + r) * 2 + 1];
+            sum += f * os[(w * RP + r) * OP + c];
         }
         if (a.splits == 1) {
             o[(long long)(sq.c0 + row / G) * p.o_stride[0] + (h * G + row % G) * p.o_stride[1] + c] = (T)(sum / ll);
         } else {
             const long long u = (long long)unit * a.splits + split;
-            a.part_o[(u * 16 + r) * d + c] = sum;
+            a.part_o[(u * RP + r) * d + c] = sum;
             if (c == 0) {
-                a.part_ml[(u * 16 + r) * 2] = mm;
-                a.part_ml[(u * 16 + r) * 2 + 1] = ll;
+                a.part_ml[(u * RP + r) * 2] = mm;
+                a.part_ml[(u * RP + r) * 2 + 1] = ll;
             }
         }
     }
 }
 
-template <typename T, int CP, int GS>
-static osh_status kv4_rows_launch(const Kv4Args &a, unsigned units, hipStream_t st) {
+template <typename T, int CP, int GS, int SUB>
+static osh_status kv4_rows_launch_s(const Kv4Args &a, unsigned units, hipStream_t st) {
     constexpr int WAVES = CP / GS == 8 ? 3 : 4;  // what 160 KB hold
     constexpr size_t wave_lds = 4 * 64 * CP * 16 + 256 + 2 * (CP / GS) * (256 + 512);
     constexpr size_t lds = std::max<size_t>(WAVES * wave_lds, WAVES * 16 * (32 * CP + 4 + 2) * sizeof(float));
-    OSH_LAUNCH((kv4_rows_kernel<T, CP, GS, WAVES>), dim3(units * a.w.splits), dim3(64 * WAVES), lds, st, a);
+    OSH_LAUNCH((kv4_rows_kernel<T, CP, GS, WAVES, SUB>), dim3(units * a.w.splits), dim3(64 * WAVES), lds, st, a);
     OSH_LAUNCH_CHECK("kv4_rows_kernel");
     return win_join<T>(a.w, units, st);
+}
+
+template <typename T, int CP, int GS>
+static osh_status kv4_rows_launch(const Kv4Args &a, unsigned units, hipStream_t st) {
+    if (a.w.tile_rows == 4) return kv4_rows_launch_s<T, CP, GS, 4>(a, units, st);
+    if (a.w.tile_rows == 8) return kv4_rows_launch_s<T, CP, GS, 2>(a, units, st);
+    return kv4_rows_launch_s<T, CP, GS, 1>(a, units, st);
 }
 
 template <typename T, int GL>
@@ -701,8 +733,8 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
         if (room.wide) return OSH_OK;
         args.wide_blocks = 0;
     }
-    a.tile_rows = 16;
-    a.tiles = cdiv(rows, 16);
+    a.tile_rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    a.tiles = cdiv(rows, a.tile_rows);
     const long long units = (long long)p->w.batch * p->w.kv_heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: too many row blocks (%lld)", units);
     const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window + p->w.sinks + 16 / a.group);
