@@ -34,22 +34,23 @@ constexpr int WIDE_PAGE = 64;
 
 // -------------------------------------------------------------- quantization
 
-// Eight neighbouring values a lane, the 4, 8 or 16 lanes of a group next to each other.
-// blockIdx.y is the sequence.
+// Tokens t0 .. t1 of the sequence's new ones into the cache, at key heads h0 .. h1, dealt out to
+// `threads` threads (whole waves).  Eight neighbouring values a lane, the GL lanes of a group
+// next to each other.
 template <typename T, int GL>
-__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
+__device__ __forceinline__ void kv4_append(const Kv4Args &a, const WinSeq &sq, int b, int h0, int h1, int t0, int t1,
+                                           long long tid, long long threads) {
     const osh_window_attn &p = a.w.p;
-    const int b = blockIdx.y, chunks = p.head_dim / 8;
-    const WinSeq sq = win_seq(p, b);
-    const long long total = (long long)sq.held * p.kv_heads * 2 * chunks;
-    for (long long e0 = blockIdx.x * 256LL; e0 < total; e0 += gridDim.x * 256LL) {
-        const long long e = e0 + threadIdx.x;
+    const int chunks = p.head_dim / 8, heads = h1 - h0;
+    const long long total = (long long)(t1 - t0) * heads * 2 * chunks;
+    for (long long e0 = tid & ~63LL; e0 < total; e0 += threads) {
+        const long long e = e0 + (tid & 63);
         const bool in = e < total;
         const long long item = in ? e / chunks : 0;
         const int c = in ? (int)(e - item * chunks) : 0;
         const bool is_v = item & 1;
-        const int h = (int)(item / 2 % p.kv_heads);
-        const long long t = item / 2 / p.kv_heads, row = sq.c0 + t;
+        const int h = h0 + (int)(item / 2 % heads);
+        const long long t = t0 + item / 2 / heads, row = sq.c0 + t;
         const T *src = static_cast<const T *>(is_v ? p.d_v_new : p.d_k_new);
         const int64_t *st = is_v ? p.v_new_stride : p.k_new_stride;
         f32x8 f = {};
@@ -108,6 +109,13 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
             store8(out + (row * p.kv_heads + h) * p.head_dim + 8 * c,
                    at < 0 ? f32x8{} + (is_v ? 0.0f : __builtin_nanf("")) : kept);
     }
+}
+
+// All new tokens.  blockIdx.y is the sequence.
+template <typename T, int GL>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
+    const WinSeq sq = win_seq(a.w.p, blockIdx.y);
+    kv4_append<T, GL>(a, sq, blockIdx.y, 0, a.w.p.kv_heads, 0, sq.held, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
 }
 
 // What the cached keys and values that any query sees stand for, rounded to T, into pages of
@@ -245,7 +253,10 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     const WinSeq sq = win_seq(p, b);
     const int rows = sq.ql * G, r0 = tile * RP;
     if (!sq.ok) {
-        if (tile == 0 && split == 0) win_fill_nan<T>(p, sq, h, G, tid, 64 * WAVES);
+        if (tile == 0 && split == 0) {
+            win_fill_nan<T>(p, sq, h, G, tid, 64 * WAVES);
+            kv4_append<T, 4 * GS>(args, sq, b, h, h + 1, 0, sq.held, tid, 64 * WAVES);  // NaN to the stored values
+        }
         return;
     }
     if (r0 >= rows) return;
@@ -283,6 +294,15 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     const int nv = keys.count;
     const int steps = cdiv(nv, 64), per = cdiv(steps, a.splits);
     const int s_end = min(steps, (split + 1) * per);
+    // the new ones among this workgroup's keys go to the cache first, from where all keys are
+    // read; another row block may write the same bytes there
+    {
+        const int v0 = split * per * 64, v1 = min(nv, s_end * 64);
+        const int t0 = max(0, (v0 < nv ? keys.at(v0) : sq.kl) - sq.past), t1 = v1 > v0 ? keys.at(v1 - 1) + 1 - sq.past : 0;
+        if (t1 > t0) kv4_append<T, 4 * GS>(args, sq, b, h, h + 1, t0, t1, tid, 64 * WAVES);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
     const int pos0 = sq.past + tok0, pos1 = sq.past + tok1;
     // by key number, this row sees v <= v_hi with v >= v_lo or v < v_sink
     const int shift = keys.sink_end - keys.lo, my_pos = sq.past + my_tok;
@@ -623,9 +643,8 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     }
 }
 
-template <typename T, int CP, int GS, int SUB>
-static osh_status kv4_rows_launch_s(const Kv4Args &a, unsigned units, hipStream_t st) {
-    constexpr int WAVES = CP / GS == 8 ? 3 : 4;  // what 160 KB hold
+template <typename T, int CP, int GS, int SUB, int WAVES>
+static osh_status kv4_rows_launch_w(const Kv4Args &a, unsigned units, hipStream_t st) {
     constexpr size_t wave_lds = 4 * 64 * CP * 16 + 256 + 2 * (CP / GS) * (256 + 512);
     constexpr size_t lds = std::max<size_t>(WAVES * wave_lds, WAVES * 16 * (32 * CP + 4 + 2) * sizeof(float));
     OSH_LAUNCH((kv4_rows_kernel<T, CP, GS, WAVES, SUB>), dim3(units * a.w.splits), dim3(64 * WAVES), lds, st, a);
@@ -633,15 +652,27 @@ static osh_status kv4_rows_launch_s(const Kv4Args &a, unsigned units, hipStream_
     return win_join<T>(a.w, units, st);
 }
 
+template <typename T, int CP, int GS, int SUB>
+static osh_status kv4_rows_launch_s(const Kv4Args &a, unsigned units, hipStream_t st) {
+    constexpr int NG = CP / GS;
+    if constexpr (SUB > 1 && CP <= 4 && NG <= 2) {
+        if (a.w.wide) return kv4_rows_launch_w<T, CP, GS, SUB, 8>(a, units, st);
+    }
+    return kv4_rows_launch_w<T, CP, GS, SUB, NG == 8 ? 3 : 4>(a, units, st);  // what 160 KB hold
+}
+
 template <typename T, int CP, int GS>
 static osh_status kv4_rows_launch(const Kv4Args &a, unsigned units, hipStream_t st) {
     if (a.w.tile_rows == 4) return kv4_rows_launch_s<T, CP, GS, 4>(a, units, st);
-    if (a.w.tile_rows == 8) return kv4_rows_launch_s<T, CP, GS, 2>(a, units, st);
-    return kv4_rows_launch_s<T, CP, GS, 1>(a, units, st);
+    if constexpr (CP / GS < 8) {
+        if (a.w.tile_rows == 8) return kv4_rows_launch_s<T, CP, GS, 2>(a, units, st);
+    }
+    if constexpr (CP / GS < 4) return kv4_rows_launch_s<T, CP, GS, 1>(a, units, st);
+    return fail(OSH_E_UNSUPPORTED, "Kv4Attention: no kernel for %d rows", a.w.tile_rows);
 }
 
 template <typename T, int GL>
-static osh_status kv4_append(const Kv4Args &a, hipStream_t st) {
+static osh_status kv4_append_all(const Kv4Args &a, hipStream_t st) {
     const osh_window_attn &p = a.w.p;
     const long long threads = (long long)p.max_q * p.kv_heads * 2 * (p.head_dim / 8);
     const unsigned x = (unsigned)std::max(1LL, std::min((threads + 255) / 256, std::max(1LL, 65536LL / p.batch)));
@@ -652,7 +683,6 @@ static osh_status kv4_append(const Kv4Args &a, hipStream_t st) {
 
 template <typename T, int GS>
 static osh_status kv4_launch_g(const Kv4Args &a, unsigned units, hipStream_t st) {
-    if (const osh_status s = kv4_append<T, 4 * GS>(a, st)) return s;
     const int d = a.w.p.head_dim;
     if constexpr (GS <= 2) {
         if (d <= 64) return kv4_rows_launch<T, 2, GS>(a, units, st);
@@ -663,9 +693,9 @@ static osh_status kv4_launch_g(const Kv4Args &a, unsigned units, hipStream_t st)
 
 template <typename T>
 static osh_status kv4_wide(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
-    const osh_status s = group == 32   ? kv4_append<T, 4>(a, st)
-                         : group == 64 ? kv4_append<T, 8>(a, st)
-                                       : kv4_append<T, 16>(a, st);
+    const osh_status s = group == 32   ? kv4_append_all<T, 4>(a, st)
+                         : group == 64 ? kv4_append_all<T, 8>(a, st)
+                                       : kv4_append_all<T, 16>(a, st);
     if (s) return s;
     const int x = std::min(a.wide_blocks, std::max(1, 65536 / a.w.p.batch));
     OSH_LAUNCH(kv4_expand_kernel<T>, dim3((unsigned)x, (unsigned)a.w.p.batch), dim3(256), 0, st, a, __builtin_ctz(group));
@@ -733,14 +763,23 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
         if (room.wide) return OSH_OK;
         args.wide_blocks = 0;
     }
-    a.tile_rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    // four or eight groups a head leave no registers for 16 rows' scores: 16 rows of 64 sequences
+    // of 5000 keys, 8 heads of 128 in groups of 32, take 465 us in one block (spilled), 250 in two
+    const int groups = cdiv(p->w.head_dim, 128) * (p->w.head_dim <= 64 ? 64 : 128) / p->group;
+    const int most = groups >= 8 ? 4 : groups >= 4 ? 8 : 16;
+    a.tile_rows = std::min(most, rows <= 4 ? 4 : rows <= 8 ? 8 : 16);
     a.tiles = cdiv(rows, a.tile_rows);
     const long long units = (long long)p->w.batch * p->w.kv_heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: too many row blocks (%lld)", units);
     const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window + p->w.sinks + 16 / a.group);
     const long long want = units ? std::max(1LL, 2LL * device_cus() / units) : 1;
     a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
-    a.wide = false;
+    // One launch of eight waves for short spans, where 160 KB hold them, else four waves, splits
+    // and a join.  Eight against four over 200, 640, 1024 and 1500 keys: one sequence of 12 heads
+    // of 64 on 4 in groups of 32: 9.5 (8.9), 10.8 (13.3), 12.0 (12.2), 13.6 (12.2) us; 32 of 32
+    // heads of 128 on 8 in groups of 64: 13.1 (12.8), 16.1 (20.0), 18.3 (22.1), 23.2 (26.8).
+    a.wide = a.tile_rows < 16 && span <= 1024 && units <= device_cus() && p->w.head_dim <= 128 && groups <= 2;
+    if (a.wide) a.splits = 1;
     const long long parts = a.splits > 1 ? units * a.splits : 0;
     room.part = room.total = (size_t)parts * a.tile_rows * (p->w.head_dim + 2) * 4;
     return OSH_OK;
