@@ -132,27 +132,31 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
 #pragma unroll
     for (int e = 0; e < 8; e++) minus[e] = p.zeros ? -1.0f : -8.0f;
 
-    auto block = [&](int kb, auto cut) {
+    struct Block {
         uint4 w[NB];
         T4 sc[NB][NG], zp[NB][NG];
         V x[MB][4];
+    };
+    auto load = [&](int kb, Block &v, auto cut) {
 #pragma unroll
         for (int j = 0; j < NB; j++) {
-            w[j] = p.codes[(blk[j] + kb) * 64 + lane];
+            v.w[j] = p.codes[(blk[j] + kb) * 64 + lane];
 #pragma unroll
             for (int e = 0; e < NG; e++) {
                 const long long at = ((blk[j] + kb) * NG + e) * 16 + 4 * g;
-                sc[j][e] = *reinterpret_cast<const T4 *>(static_cast<const T *>(p.scales) + at);
-                if (p.zeros) zp[j][e] = *reinterpret_cast<const T4 *>(static_cast<const T *>(p.zeros) + at);
+                v.sc[j][e] = *reinterpret_cast<const T4 *>(static_cast<const T *>(p.scales) + at);
+                if (p.zeros) v.zp[j][e] = *reinterpret_cast<const T4 *>(static_cast<const T *>(p.zeros) + at);
             }
         }
 #pragma unroll
         for (int i = 0; i < MB; i++)
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                if constexpr (decltype(cut)::value) x[i][t] = load_row8<T>(a[i] - 8 * g, kb * KB + 32 * t + 8 * g, p.k);
-                else __builtin_memcpy(&x[i][t], a[i] + kb * KB + 32 * t, sizeof(V));
+                if constexpr (decltype(cut)::value) v.x[i][t] = load_row8<T>(a[i] - 8 * g, kb * KB + 32 * t + 8 * g, p.k);
+                else __builtin_memcpy(&v.x[i][t], a[i] + kb * KB + 32 * t, sizeof(V));
             }
+    };
+    auto compute = [&](const Block &v) {
 #pragma unroll
         for (int e = 0; e < NG; e++) {
             H8 xs[MB][GS][P];
@@ -162,7 +166,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
                 less[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int t = 0; t < GS; t++) {
-                    split_row8<T>(x[i][e * GS + t], xs[i][t]);
+                    split_row8<T>(v.x[i][e * GS + t], xs[i][t]);
 #pragma unroll
                     for (int q = 0; q < P; q++) less[i] = mma16(minus, xs[i][t][q], less[i]);
                 }
@@ -173,11 +177,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
 #pragma unroll
                 for (int i = 0; i < MB; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) sum[i][r] = p.zeros ? less[i][r] * (float)zp[j][e][r] : less[i][r];
+                    for (int r = 0; r < 4; r++) sum[i][r] = p.zeros ? less[i][r] * (float)v.zp[j][e][r] : less[i][r];
 #pragma unroll
                 for (int t = 0; t < GS; t++) {
                     H8 c;
-                    codes8(reinterpret_cast<const unsigned *>(&w[j])[e * GS + t], c);
+                    codes8(reinterpret_cast<const unsigned *>(&v.w[j])[e * GS + t], c);
 #pragma unroll
                     for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -186,13 +190,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
 #pragma unroll
                 for (int i = 0; i < MB; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf((float)sc[j][e][r], sum[i][r], acc[i][j][r]);
+                    for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf((float)v.sc[j][e][r], sum[i][r], acc[i][j][r]);
             }
         }
     };
     int kb = wave;
-    for (; kb < whole; kb += WAVES) block(kb, IntC<0>{});
-    if (kb < nkb) block(kb, IntC<1>{});
+    Block v;
+    for (; kb < whole; kb += WAVES) load(kb, v, IntC<0>{}), compute(v);
+    if (kb < nkb) load(kb, v, IntC<1>{}), compute(v);
 #pragma unroll
     for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -209,6 +214,156 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_rows_kernel(Int4Args p) {
     }
 }
 
+
+// ---------------------------------------------------- few rows, large weights
+
+// A workgroup takes 128 outputs (32 a wave) of up to 16 MB rows over up to KR blocks of k: all its
+// codes are on their way before the first one is used, the rows' pieces and the scales pass
+// through LDS once for its four waves (chunk c of row r at c ^ r % 16), and one barrier is all.
+// The sums of the parts of k go to memory in FP32 and are joined in their order.  In
+// int4_rows_kernel each 16 outputs read the rows again, which binds it: 32 rows of 8192 against
+// 16384 outputs are 537 MB from the L2.
+template <typename T, int MB> constexpr int SLIM_KR = sizeof(T) == 4 ? (MB == 1 ? 4 : 2) : MB == 4 ? 4 : 8;
+
+template <typename T, int MB, int GS>
+__global__ __launch_bounds__(256, 2) void int4_slim_kernel(Int4Args p, int kr, float *part, long long pitch) {
+    using H8 = typename Half8<T>::type;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr int P = PIECES<T>, NG = 4 / GS, KR = SLIM_KR<T, MB>, ROWS = 16 * MB;
+    constexpr int SC = KR * NG * 16;  // scales of 16 outputs
+    __shared__ __align__(16) H8 rows[P][ROWS][KR * 16];
+    __shared__ __align__(16) T scales[8][SC], zeros[8][SC];
+    const int tid = threadIdx.x, lane = tid & 63, jl = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nkb = cdiv(p.k, KB), nblk = cdiv(p.n, 16);
+    const int kb0 = blockIdx.y * kr, count = min(kr, nkb - kb0), b0 = blockIdx.x * 8, m0 = blockIdx.z * ROWS;
+
+    // rows and scales first: loads return in order
+    constexpr int PER = KR * 16 * ROWS / 256;  // chunks of a thread
+    typename Vec8<T>::type x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int e = i * 256 + tid, r = e / (KR * 16), c = e % (KR * 16);
+        const T *row = static_cast<const T *>(p.a) + (long long)min(m0 + r, p.m - 1) * p.lda;
+        x[i] = load_row8<T>(row, kb0 * KB + 8 * c, c < count * 16 ? p.k : 0);
+    }
+    constexpr int VEC = 16 / sizeof(T);
+    for (int e = tid; e < 8 * (SC / VEC); e += 256) {
+        const int j = e / (SC / VEC), c = e % (SC / VEC) * VEC;
+        if (c >= count * NG * 16) continue;
+        const long long at = ((long long)min(b0 + j, nblk - 1) * nkb + kb0) * NG * 16 + c;
+        __builtin_memcpy(&scales[j][c], static_cast<const T *>(p.scales) + at, 16);
+        if (p.zeros) __builtin_memcpy(&zeros[j][c], static_cast<const T *>(p.zeros) + at, 16);
+    }
+    uint4 w[KR][2];
+#pragma unroll
+    for (int kb = 0; kb < KR; kb++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const long long blk = (long long)min(b0 + 2 * wave + j, nblk - 1) * nkb + kb0 + min(kb, count - 1);
+            w[kb][j] = p.codes[blk * 64 + lane];
+        }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int e = i * 256 + tid, r = e / (KR * 16), c = e % (KR * 16);
+        H8 h[P];
+        split_row8<T>(x[i], h);
+#pragma unroll
+        for (int u = 0; u < P; u++) rows[u][r][c ^ (r & 15)] = h[u];
+    }
+    __syncthreads();
+    H8 minus;
+#pragma unroll
+    for (int e = 0; e < 8; e++) minus[e] = p.zeros ? -1.0f : -8.0f;
+    f32x4 acc[MB][2];
+#pragma unroll
+    for (int i = 0; i < MB; i++) acc[i][0] = acc[i][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int kb = 0; kb < KR; kb++) {
+        if (kb >= count) break;
+#pragma unroll
+        for (int e = 0; e < NG; e++) {
+            H8 xs[MB][GS][P];
+            f32x4 less[MB];
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                less[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < GS; s++)
+#pragma unroll
+                    for (int u = 0; u < P; u++) {
+                        xs[i][s][u] = rows[u][16 * i + jl][(kb * 16 + 4 * (e * GS + s) + g) ^ jl];
+                        less[i] = mma16(minus, xs[i][s][u], less[i]);
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const T4 sc = *reinterpret_cast<const T4 *>(&scales[2 * wave + j][(kb * NG + e) * 16 + 4 * g]);
+                f32x4 sum[MB];
+#pragma unroll
+                for (int i = 0; i < MB; i++) sum[i] = less[i];
+                if (p.zeros) {
+                    const T4 zp = *reinterpret_cast<const T4 *>(&zeros[2 * wave + j][(kb * NG + e) * 16 + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < MB; i++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) sum[i][r] *= (float)zp[r];
+                }
+#pragma unroll
+                for (int s = 0; s < GS; s++) {
+                    H8 c;
+                    codes8(reinterpret_cast<const unsigned *>(&w[kb][j])[e * GS + s], c);
+#pragma unroll
+                    for (int i = 0; i < MB; i++)
+#pragma unroll
+                        for (int u = 0; u < P; u++) sum[i] = mma16(c, xs[i][s][u], sum[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf((float)sc[r], sum[i][r], acc[i][j][r]);
+            }
+        }
+    }
+    // lane (jl, g): outputs 4 g .. + 3 of row jl
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int row = m0 + 16 * i + jl, col = (b0 + 2 * wave + j) * 16 + 4 * g;
+            if (row >= p.m) continue;
+            if (gridDim.y > 1) {
+                *reinterpret_cast<f32x4 *>(part + ((long long)blockIdx.y * p.m + row) * pitch + col) = acc[i][j];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (col + r < p.n) static_cast<T *>(p.y)[row * p.ldy + col + r] = int4_finish<T>(p, acc[i][j][r], row, col + r);
+            }
+        }
+}
+
+// The parts' sums, four outputs a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void int4_join_kernel(Int4Args p, int parts, const float *part, long long pitch) {
+    const int quads = (int)(pitch / 4);
+    const long long at = blockIdx.x * 256LL + threadIdx.x;
+    if (at >= (long long)p.m * quads) return;
+    const int row = (int)(at / quads), col = (int)(at - (long long)row * quads) * 4;
+    const float *from = part + row * pitch + col;
+    const long long next = (long long)p.m * pitch;
+    f32x4 sum = {0, 0, 0, 0};
+    for (int s = 0; s < parts; s += 8) {
+        f32x4 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = *reinterpret_cast<const f32x4 *>(from + min(s + e, parts - 1) * next);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (s + e < parts) sum += v[e];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (col + r < p.n) static_cast<T *>(p.y)[row * p.ldy + col + r] = int4_finish<T>(p, sum[r], row, col + r);
+}
 
 // ---------------------------------------------------------------- many rows
 
@@ -560,22 +715,58 @@ static Int4Layout int4_layout(int n, int k, int group, int dtype, bool zeros) {
     return l;
 }
 
-// What a call with many rows keeps beside its operands.
+// Which kernel a call takes, and what it keeps beside its operands.
 struct Int4Room {
-    bool tile, copy;
+    bool tile, copy, slim;
+    int kr, parts, pitch;       // slim: blocks of k and their number; of a row of sums, or of a piece
     size_t sums, plane, total;  // plane in values
-    int pitch;
 };
-static Int4Room int4_room(int m, int k, int group, int dtype) {
+static Int4Room int4_room(int m, int n, int k, int group, int dtype) {
     Int4Room r = {};
-    r.tile = m > 64;
-    if (!r.tile) return r;
-    r.copy = dtype == OSH_T_F32 || k % 8;
-    r.sums = dtype == OSH_T_F32 ? 0 : (size_t)m * cdiv(k, group) * 16;
-    r.pitch = cdiv(k, KB) * KB;
+    const bool f32 = dtype == OSH_T_F32;
+    const int nkb = cdiv(k, KB);
+    // Small tiles wait for memory once a block of k, the slim kernel once in all but reads the
+    // weights again for each 64 rows (32 in FP32).  Tile against slim: 128 rows of 4096 against
+    // 4096 outputs 26.3 (22.2) us, 54.4 (39.7) in FP32; of 1024 against 4096 10.8 (16.0), 18.9
+    // (16.9); 256 of 8192 against 8192 63.5 (93.7), 144 (286).
+    r.tile = m > 64 && ((long long)m * n > (f32 ? 1 << 19 : 1 << 20) || (!f32 && k < 2048));
+    if (!r.tile) {
+        // Against a launch of int4_rows_kernel, two launches of the slim one cost 4 to 10 us more,
+        // by the rows' blocks; it gains what the 16 outputs' own copies of the rows take (11
+        // TB/s) and 0.07 us a MB of weights.  FP32 rows gain where a wave has much to split.
+        const double copies = (double)cdiv(n, 16) * m * k * 2e-6 / 11, weights = (double)n * k * 0.5e-6 * 0.07;
+        const double cost = m <= 16 ? 4.2 : m <= 32 ? 7.3 : 10.1;
+        r.slim = f32 ? (long long)n * k >= 1 << 24 || m > 32 : copies + weights > cost || m > 64;
+        if (!r.slim) return r;
+        const int mb = m <= 16 ? 1 : m <= 32 || f32 ? 2 : 4;
+        const int most = f32 ? (mb == 1 ? 4 : 2) : mb == 4 ? 4 : 8;  // SLIM_KR
+        const long long tiles = (long long)cdiv(n, 128) * cdiv(m, 16 * mb);
+        r.kr = (int)std::max(1LL, std::min<long long>(most, tiles * nkb / device_cus()));
+        r.parts = cdiv(nkb, r.kr);
+        r.pitch = cdiv(n, 128) * 128;
+        r.total = r.parts > 1 ? (size_t)r.parts * m * r.pitch * 4 : 0;
+        return r;
+    }
+    r.copy = f32 || k % 8;
+    r.sums = f32 ? 0 : (size_t)m * cdiv(k, group) * 16;
+    r.pitch = nkb * KB;
     r.plane = r.copy ? (size_t)m * r.pitch : 0;
-    r.total = r.sums + r.plane * (dtype == OSH_T_F32 ? 6 : 2);
+    r.total = r.sums + r.plane * (f32 ? 6 : 2);
     return r;
+}
+
+template <typename T, int MB, int GS>
+static osh_status int4_slim(const Int4Args &p, const Int4Room &room, float *part, hipStream_t st) {
+    OSH_LAUNCH((int4_slim_kernel<T, MB, GS>), dim3((unsigned)cdiv(p.n, 128), (unsigned)room.parts, (unsigned)cdiv(p.m, 16 * MB)), dim3(256), 0, st, p,
+               room.kr, part, (long long)room.pitch);
+    OSH_LAUNCH_CHECK("int4_slim_kernel");
+    if (room.parts > 1) {
+        const long long threads = (long long)p.m * (room.pitch / 4);
+        OSH_LAUNCH(int4_join_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, p, room.parts, part,
+                   (long long)room.pitch);
+        OSH_LAUNCH_CHECK("int4_join_kernel");
+    }
+    return OSH_OK;
 }
 
 template <typename T, int MB, int NB, int WM, int WN, int GS>
@@ -587,13 +778,21 @@ static void int4_tile(const Int4Args &p, const Int4Prep &q, int group, hipStream
 
 template <typename T, int GS>
 static osh_status int4_launch(const Int4Args &p, int group, const Int4Room &room, void *scratch, hipStream_t st) {
+    if (room.slim) {
+        float *part = static_cast<float *>(scratch);
+        if (p.m <= 16) return int4_slim<T, 1, GS>(p, room, part, st);
+        if constexpr (sizeof(T) == 2) {
+            if (p.m > 32) return int4_slim<T, 4, GS>(p, room, part, st);
+        }
+        return int4_slim<T, 2, GS>(p, room, part, st);
+    }
     if (!room.tile) {
-#define OSH_INT4_ROWS(MB, NB)                                                                                  \
-    OSH_LAUNCH((int4_rows_kernel<T, MB, NB, GS, 8>), dim3((unsigned)cdiv(p.n, 16 * NB), (unsigned)cdiv(p.m, 16 * MB)), \
+#define OSH_INT4_ROWS(MB)                                                                                        \
+    OSH_LAUNCH((int4_rows_kernel<T, MB, 1, GS, 8>), dim3((unsigned)cdiv(p.n, 16), (unsigned)cdiv(p.m, 16 * MB)), \
                dim3(512), 0, st, p)
-        if (p.m <= 16) OSH_INT4_ROWS(1, 1);
-        else if (p.m <= 32) OSH_INT4_ROWS(2, 1);
-        else OSH_INT4_ROWS(4, 1);
+        if (p.m <= 16) OSH_INT4_ROWS(1);
+        else if (p.m <= 32) OSH_INT4_ROWS(2);
+        else OSH_INT4_ROWS(4);
 #undef OSH_INT4_ROWS
         OSH_LAUNCH_CHECK("int4_rows_kernel");
         return OSH_OK;
@@ -618,10 +817,10 @@ static osh_status int4_launch(const Int4Args &p, int group, const Int4Room &room
                    (long long)room.pitch, (long long)room.plane);
     }
     OSH_LAUNCH_CHECK("int4_prep_kernel");
-    // 64 x 256 tiles where they fill the card, else 64 x 64 ones: 512 x 4096 x 4096 in bf16 takes
-    // 56 us as 128 large tiles, 36 as 512 small ones; 1024 x 8192 x 8192 168 and 250
+    // 64 x 256 tiles where they fill the card, else 32 x 128 ones: 512 x 4096 x 4096 in bf16 takes
+    // 56 us as 128 large tiles, 35 as 512 small ones
     if ((long long)cdiv(p.m, 64) * cdiv(p.n, 256) >= device_cus()) int4_tile<T, 2, 2, 1, 4, GS>(p, q, group, st);
-    else int4_tile<T, 1, 1, 2, 2, GS>(p, q, group, st);
+    else int4_tile<T, 1, 1, 1, 4, GS>(p, q, group, st);
     OSH_LAUNCH_CHECK("int4_tile_kernel");
     return OSH_OK;
 }
@@ -696,7 +895,7 @@ OSH_API osh_status osh_int4_matmul_scratch_bytes(int m, int n, int k, int group,
     if (!bytes) return fail(OSH_E_INVALID, "Int4MatMul: NULL bytes");
     if (m < 0) return fail(OSH_E_INVALID, "Int4MatMul: negative sizes");
     if (const osh_status st = int4_check(n, k, group, dtype)) return st;
-    *bytes = m && n ? int4_room(m, k, group, dtype).total : 0;
+    *bytes = m && n ? int4_room(m, n, k, group, dtype).total : 0;
     return OSH_OK;
 }
 
@@ -716,7 +915,7 @@ OSH_API osh_status osh_int4_matmul(int m, int n, int k, int group, int dtype, co
         return fail(OSH_E_UNSUPPORTED, "Int4MatMul: %d x %d outputs", m, n);
     const long long e = elem_bytes(dtype);
     const Int4Layout l = int4_layout(n, k, group, dtype, has_zeros);
-    const Int4Room room = int4_room(m, k, group, dtype);
+    const Int4Room room = int4_room(m, n, k, group, dtype);
     if (room.total && (!d_scratch || ((uintptr_t)d_scratch & 15))) return fail(OSH_E_INVALID, "Int4MatMul: no scratch at 16-byte alignment");
     const Strided y = strided_rows(d_y, m, ldy * e, n * e), res = strided_rows(d_res, m, ldr * e, n * e);
     if (share_bytes(y, strided_rows(d_a, m, lda * e, k * e)) || share_bytes(y, Strided(d_packed, l.total)) ||
