@@ -644,12 +644,14 @@ OSH_API osh_status osh_block_norm(int64_t rows, int cols, int dtype, const void 
  * a [m][lda] and res [m][ldr] of type dtype at any pitch and alignment of whole elements;
  * bias FP32 and res may be NULL; act: none, relu, silu or gelu.  res may be y itself (same
  * pitch); no other overlap of y.  group is 32, 64 or a multiple of 128.  The sums are FP32 and
- * nothing is rounded before them. */
+ * nothing is rounded before them.  Weights of one group with a scale of 0 are 0.  A row that
+ * holds a NaN or an infinity gives outputs that are not finite; n, k <= 2^28, m <= 64 * 65535. */
 OSH_API osh_status osh_int4_packed_bytes(int n, int k, int group, int dtype, int has_zeros, size_t *bytes);
 OSH_API osh_status osh_int4_pack(int n, int k, int group, int dtype, const void *d_codes, int64_t ldc,
                                  const void *d_scales, int64_t lds, const void *d_zeros, int64_t ldz, void *d_packed,
                                  osh_stream s);
-/* Scratch of osh_int4_matmul (0 where it needs none); depends on the sizes only. */
+/* Scratch of osh_int4_matmul (0 where it needs none), at 16-byte alignment; depends on the sizes
+ * only. */
 OSH_API osh_status osh_int4_matmul_scratch_bytes(int m, int n, int k, int group, int dtype, size_t *bytes);
 OSH_API osh_status osh_int4_matmul(int m, int n, int k, int group, int dtype, const void *d_a, int64_t lda,
                                    const void *d_packed, int has_zeros, const float *d_bias, int act,
@@ -718,12 +720,18 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
  * osh_window_attention does, with every key and value, the new ones too, as the cache
  * stands for it: o depends on the cache alone, not on how its tokens came in calls.  A query
  * that sees a key whose page id lies outside [0, pages) gets NaN, a new one too.
+ * Scores are FP32 sums of the exact values.  What is rounded: a weight times a value's scale, to
+ * dtype.  From 512 rows a key head on (max_q * (q_heads / kv_heads)) bf16 calls take keys,
+ * values and weights in f16, times a power of two that puts a head's largest visible key, and
+ * value, between 1/2 and 1: what lies below 2^-14 of it keeps fewer than f16's 11 bits.  A value
+ * that is not finite may make other queries of its sequence NaN, as above.
  * d_k_stored and d_v_stored (both or neither NULL) receive what the cache stands for at
  * the new tokens, rounded to dtype; rows that are not kept get NaN.
  * `w` holds sizes, pointers and strides as above, with codes for k_pages and v_pages and
  * their strides in bytes; head_dim % 32 == 0.  Codes of a head lie at a multiple of 16 bytes,
- * its pairs at a multiple of 4.  Scales, codes and stored values share no memory with
- * anything else. */
+ * its pairs at a multiple of 4; group 32, 64 or 128; d_scratch at a multiple of 16.  Strides of
+ * codes and pairs < 2^31.  Scales, codes and stored values share no memory with anything else.
+ * Up to 65535 sequences, and fewer than 2^22 row blocks of 4 to 16 rows (128 from 512 on). */
 typedef struct osh_kv4_attn {
     osh_window_attn w;
     int group, reserved;                                  /* 0 */

@@ -1,13 +1,16 @@
 // osh_kv4_attn.hip -- the attention of osh_window_attn.hip over a paged cache held in 4
 // bits (osh_kv4_attention): a group of a head's values is lo + scale * code.
 //
-// The products take the codes, which are exact in 16 bits; scales and minima stay in FP32:
+// Up to 512 rows of a key head, and f16 calls (kv4_rows_kernel): the products take the codes,
+// which are exact in 16 bits; scales and minima stay in FP32:
 //   q . k_j = sum over groups of scale_j (q . code_j) + lo_j (sum of q over the group),
 //   sum_j p_j v_j = sum_j (p_j scale_j) (code_j - 8) + sum_j p_j (lo_j + 8 scale_j).
 // Rounded are the weights p_j scale_j alone, half a step of dtype each as the weights are
 // over a 16-bit cache; codes less 8 have the size of the values about the group's middle, so
 // that the roundings weigh what they weigh there.  (8 is taken off the sums by a product
 // with the constant -8.)
+// More rows in bf16: the visible cache is expanded to f16 pages once, and the kernel of
+// osh_window_attn.hip reads those.
 #include <limits.h>
 
 #include "osh_overlap.h"
@@ -23,9 +26,9 @@ struct Kv4Args {
     void *k_stored, *v_stored;
     long long ks_stride[3], vs_stride[3], k_stored_stride[2], v_stored_stride[2];
     unsigned page_mul, page_log;  // j / page = umulhi(4 j, page_mul) >> page_log for j < 2^30
-    // many rows: the visible cache in 16 bits, and what the 16-bit kernel is told about it
-    void *k_fresh, *v_fresh;      // new tokens [tokens][kv_heads][head_dim], or NULL
-    void *k_wide, *v_wide;        // [batch * wide_blocks][kv_heads][WIDE_PAGE][head_dim]
+    // many bf16 rows: the visible cache in f16, and what the 16-bit kernel is told about it
+    _Float16 *k_wide, *v_wide;    // [batch * wide_blocks][kv_heads][WIDE_PAGE][head_dim]
+    float *wide_by;               // [batch][kv_heads][2]: what K and V are taken times
     int32_t *wide_table, *wide_kl;
     int wide_blocks, wide_width;  // pages of a sequence, entries of its table
 };
@@ -105,9 +108,6 @@ __device__ __forceinline__ void kv4_append(const Kv4Args &a, const WinSeq &sq, i
             const long long *ost = is_v ? a.v_stored_stride : a.k_stored_stride;
             store8(out + row * ost[0] + h * ost[1] + 8 * c, at < 0 ? f32x8{} + __builtin_nanf("") : kept);
         }
-        if (T *out = static_cast<T *>(is_v ? a.v_fresh : a.k_fresh))  // NaN reaches who sees the key, by the key
-            store8(out + (row * p.kv_heads + h) * p.head_dim + 8 * c,
-                   at < 0 ? f32x8{} + (is_v ? 0.0f : __builtin_nanf("")) : kept);
     }
 }
 
@@ -118,8 +118,59 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
     kv4_append<T, GL>(a, sq, blockIdx.y, 0, a.w.p.kv_heads, 0, sq.held, blockIdx.x * 256LL + threadIdx.x, gridDim.x * 256LL);
 }
 
-// What the cached keys and values that any query sees stand for, rounded to T, into pages of
-// their own, and the table of those: first the blocks of the sinks, then those of the window.
+// The keys that any of a sequence's queries sees, by their blocks of WIDE_PAGE: first those of
+// the sinks, then those of the window.
+struct WideBlocks {
+    int sinks, first, count;
+    __device__ int at(int i) const { return i < sinks ? i : first + i - sinks; }  // below count
+};
+__device__ __forceinline__ WideBlocks kv4_blocks(const osh_window_attn &p, const WinSeq &sq, const WinKeys &keys) {
+    const int sinks = cdiv(min(p.sinks, p.max_kv), WIDE_PAGE);
+    return {sinks, max(keys.lo / WIDE_PAGE, sinks), cdiv(sq.kl, WIDE_PAGE)};
+}
+
+// The power of two that keeps a head's largest visible key, and value, within 1.  f16's 11 bits
+// are then 8 times as close as bf16's rounding of the output down to 2^-14 of it (bf16 keys and
+// values add as much error as the output's own rounding twice over).  blockIdx: head, sequence.
+template <typename T>
+__global__ __launch_bounds__(1024) void kv4_range_kernel(Kv4Args a, int groups) {
+    const osh_window_attn &p = a.w.p;
+    const int b = blockIdx.y, h = blockIdx.x;
+    const WinSeq sq = win_seq(p, b);
+    if (!sq.ok || sq.ql == 0) return;
+    const WinKeys keys = win_keys(p, sq, 0, sq.ql - 1);
+    __shared__ float s_top[2][16];
+    float top[2] = {0.0f, 0.0f};
+    for (int v = threadIdx.x; v < keys.count; v += 1024) {
+        const int j = keys.at(v), slot = j % p.page, id = p.d_table[b * p.table_stride + j / p.page];
+        if ((unsigned)id >= (unsigned)p.pages) continue;
+#pragma unroll
+        for (int is_v = 0; is_v < 2; is_v++) {
+            const long long *st = is_v ? a.vs_stride : a.ks_stride;
+            const T *pair = static_cast<const T *>(is_v ? a.vs : a.ks) + id * st[0] + slot * st[1] + h * st[2];
+            for (int e = 0; e < groups; e++) {
+                const float s = (float)pair[2 * e], lo = (float)pair[2 * e + 1];
+                const float size = __builtin_fmaxf(__builtin_fabsf(lo), __builtin_fabsf(__builtin_fmaf(15.0f, s, lo)));
+                if (size < __builtin_inff()) top[is_v] = __builtin_fmaxf(top[is_v], size);
+            }
+        }
+    }
+#pragma unroll
+    for (int is_v = 0; is_v < 2; is_v++) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) top[is_v] = __builtin_fmaxf(top[is_v], __shfl_xor(top[is_v], o));
+        if ((threadIdx.x & 63) == 0) s_top[is_v][threadIdx.x >> 6] = top[is_v];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        float t = 0.0f;
+        for (int w = 0; w < 16; w++) t = __builtin_fmaxf(t, s_top[threadIdx.x][w]);
+        const int e = min(max(__builtin_amdgcn_frexp_expf(t), -120), 126);
+        a.wide_by[2 * ((long long)b * p.kv_heads + h) + threadIdx.x] = __builtin_amdgcn_ldexpf(1.0f, -e);
+    }
+}
+
+// The visible keys and values, the new ones too, into f16 pages, and the table of those.
 // blockIdx.y is the sequence, blockIdx.x deals out its pages.
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_expand_kernel(Kv4Args a, int group_log) {
@@ -129,21 +180,21 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(Kv4Args a, int group_lo
     if (blockIdx.x == 0 && threadIdx.x == 0) a.wide_kl[b] = sq.ok ? sq.kl : -1;
     if (!sq.ok || sq.ql == 0) return;
     const WinKeys keys = win_keys(p, sq, 0, sq.ql - 1);
-    const int sink_blocks = cdiv(min(p.sinks, p.max_kv), WIDE_PAGE);
-    const int first = max(keys.lo / WIDE_PAGE, sink_blocks), count = cdiv(sq.kl, WIDE_PAGE);
+    const WideBlocks blocks = kv4_blocks(p, sq, keys);
     for (int at = blockIdx.x; at < a.wide_blocks; at += gridDim.x) {
-        const int block = at < sink_blocks ? at : first + at - sink_blocks;
-        if (block >= count) return;
+        const int block = blocks.at(at);
+        if (block >= blocks.count) return;
         const long long page = (long long)b * a.wide_blocks + at;
         if (threadIdx.x == 0) a.wide_table[(long long)b * a.wide_width + block] = (int)page;
         for (int e = threadIdx.x; e < p.kv_heads * WIDE_PAGE * chunks; e += 256) {
             const int c = e % chunks, in = e / chunks % WIDE_PAGE, h = e / chunks / WIDE_PAGE;
             const int j = block * WIDE_PAGE + in;
-            if (j >= sq.past || (j < keys.lo && j >= p.sinks)) continue;
+            if (j >= sq.kl || (j < keys.lo && j >= p.sinks)) continue;
             const int slot = j % p.page, id = p.d_table[b * p.table_stride + j / p.page];
+            const float *by = a.wide_by + 2 * ((long long)b * p.kv_heads + h);
             f32x8 k = f32x8{} + __builtin_nanf(""), v = {};
             if ((unsigned)id < (unsigned)p.pages) {
-                auto load = [&](const void *codes, const int64_t *st, const void *pairs, const long long *pst) {
+                auto load = [&](const void *codes, const int64_t *st, const void *pairs, const long long *pst, float by) {
                     const unsigned w = *reinterpret_cast<const unsigned *>(static_cast<const char *>(codes) + id * st[0] +
                                                                            slot * st[1] + h * st[2] + 4 * c);
                     const T *pair = static_cast<const T *>(pairs) + id * pst[0] + slot * pst[1] + h * pst[2] +
@@ -151,14 +202,14 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(Kv4Args a, int group_lo
                     f32x8 f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) f[i] = __builtin_fmaf((float)pair[0], (float)(w >> (4 * i) & 15u), (float)pair[1]);
-                    return f;
+                    return f * by;
                 };
-                k = load(p.d_k_pages, p.k_stride, a.ks, a.ks_stride);
-                v = load(p.d_v_pages, p.v_stride, a.vs, a.vs_stride);
+                k = load(p.d_k_pages, p.k_stride, a.ks, a.ks_stride, by[0]);
+                v = load(p.d_v_pages, p.v_stride, a.vs, a.vs_stride, by[1]);
             }
             const long long to = ((page * p.kv_heads + h) * WIDE_PAGE + in) * d + 8 * c;
-            store8(static_cast<T *>(a.k_wide) + to, k);
-            store8(static_cast<T *>(a.v_wide) + to, v);
+            store8(a.k_wide + to, k);
+            store8(a.v_wide + to, v);
         }
     }
 }
@@ -691,21 +742,26 @@ static osh_status kv4_launch_g(const Kv4Args &a, unsigned units, hipStream_t st)
     return kv4_rows_launch<T, 8, GS>(a, units, st);
 }
 
-template <typename T>
 static osh_status kv4_wide(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
-    const osh_status s = group == 32   ? kv4_append_all<T, 4>(a, st)
-                         : group == 64 ? kv4_append_all<T, 8>(a, st)
-                                       : kv4_append_all<T, 16>(a, st);
+    const osh_status s = group == 32   ? kv4_append_all<__bf16, 4>(a, st)
+                         : group == 64 ? kv4_append_all<__bf16, 8>(a, st)
+                                       : kv4_append_all<__bf16, 16>(a, st);
     if (s) return s;
-    const int x = std::min(a.wide_blocks, std::max(1, 65536 / a.w.p.batch));
-    OSH_LAUNCH(kv4_expand_kernel<T>, dim3((unsigned)x, (unsigned)a.w.p.batch), dim3(256), 0, st, a, __builtin_ctz(group));
+    const osh_window_attn &p = a.w.p;
+    OSH_LAUNCH(kv4_range_kernel<__bf16>, dim3((unsigned)p.kv_heads, (unsigned)p.batch), dim3(1024), 0, st, a,
+               p.head_dim / group);
+    OSH_LAUNCH_CHECK("kv4_range_kernel");
+    const int x = std::min(a.wide_blocks, std::max(1, 65536 / p.batch));
+    OSH_LAUNCH(kv4_expand_kernel<__bf16>, dim3((unsigned)x, (unsigned)p.batch), dim3(256), 0, st, a, __builtin_ctz(group));
     OSH_LAUNCH_CHECK("kv4_expand_kernel");
-    return win_run(wide, units, st);
+    return win_run_expanded(wide, units, st);
 }
 
 template <typename T>
 static osh_status kv4_launch(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
-    if (a.wide_blocks) return kv4_wide<T>(a, wide, group, units, st);
+    if constexpr (__is_same(T, __bf16)) {
+        if (a.wide_blocks) return kv4_wide(a, wide, group, units, st);
+    }
     if (group == 32) return kv4_launch_g<T, 1>(a, units, st);
     if (group == 64) return kv4_launch_g<T, 2>(a, units, st);
     return kv4_launch_g<T, 4>(a, units, st);
@@ -714,11 +770,13 @@ static osh_status kv4_launch(const Kv4Args &a, const WinArgs &wide, int group, u
 // Where the parts of the scratch lie: a.w's own or, with many rows, `wide`, the 16-bit call.
 struct Kv4Room {
     bool wide;
-    size_t part, fresh, page, table, kl, total;  // bytes, of one tensor of K and V
+    size_t part, page, by, table, kl, total;  // bytes; page: of K or V
 };
 
-// Rows of a key head from which the visible cache is first expanded to 16 bits, and the room
-// that may take.
+// Rows of a key head from which a bf16 call first expands the visible cache to f16, and the room
+// that may take.  4096 tokens behind 12288, 32 heads of 128 on 8, window 8192: 1470 us in blocks
+// of 16 rows, 740 so; 4 x 64 tokens (256 rows) behind 8128 122 in blocks.  f16 calls have no
+// type with bits to spare for it.
 constexpr int WIDE_ROWS = 512;
 constexpr size_t WIDE_MAX = (size_t)16 << 30;
 
@@ -735,7 +793,7 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
     if (p->w.batch > 65535) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: %d sequences", p->w.batch);
     const int rows = p->w.max_q * a.group;
     auto align = [](size_t n) { return (n + 255) / 256 * 256; };
-    if (rows >= WIDE_ROWS && p->w.batch) {
+    if (rows >= WIDE_ROWS && p->w.batch && p->w.dtype == OSH_T_BF16) {
         const long long most = cdiv(p->w.max_kv, WIDE_PAGE), sinks = cdiv(std::min(p->w.sinks, p->w.max_kv), WIDE_PAGE);
         const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window - 1 + p->w.max_q);
         args.wide_blocks = (int)std::min(most, sinks + (span + WIDE_PAGE - 1) / WIDE_PAGE + 1);
@@ -749,17 +807,15 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
         w.k_stride[0] = w.v_stride[0] = w.kv_heads * WIDE_PAGE * head;
         w.k_stride[1] = w.v_stride[1] = head;
         w.k_stride[2] = w.v_stride[2] = WIDE_PAGE * head;
-        w.k_new_stride[0] = w.v_new_stride[0] = w.kv_heads * head;
-        w.k_new_stride[1] = w.v_new_stride[1] = head;
         if (const osh_status st = win_plan(&w, wide, room.part)) return st;
         room.part = align(room.part);
-        room.fresh = align((size_t)w.tokens * w.kv_heads * head * 2);
+        room.by = align((size_t)w.batch * w.kv_heads * 8);
         room.table = align((size_t)w.batch * args.wide_width * 4);
         room.kl = align((size_t)w.batch * 4);
         const double bytes = 4.0 * pages * w.kv_heads * WIDE_PAGE * head;
         room.wide = pages <= INT_MAX && w.k_stride[0] <= INT_MAX && bytes <= (double)WIDE_MAX;
         room.page = room.wide ? (size_t)bytes / 2 : 0;
-        room.total = room.part + 2 * room.fresh + 2 * room.page + room.table + room.kl;
+        room.total = room.part + room.by + 2 * room.page + room.table + room.kl;
         if (room.wide) return OSH_OK;
         args.wide_blocks = 0;
     }
@@ -864,10 +920,9 @@ OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *q, void *d_scratch, osh
     if (room.wide) {
         char *at = static_cast<char *>(d_scratch) + room.part;
         auto take = [&](size_t n) { return at += n, at - n; };
-        wide.p.d_k_new = a.k_fresh = take(room.fresh);
-        wide.p.d_v_new = a.v_fresh = take(room.fresh);
-        wide.p.d_k_pages = a.k_wide = take(room.page);
-        wide.p.d_v_pages = a.v_wide = take(room.page);
+        wide.expanded = a.wide_by = reinterpret_cast<float *>(take(room.by));
+        wide.p.d_k_pages = a.k_wide = reinterpret_cast<_Float16 *>(take(room.page));
+        wide.p.d_v_pages = a.v_wide = reinterpret_cast<_Float16 *>(take(room.page));
         wide.p.d_table = a.wide_table = reinterpret_cast<int32_t *>(take(room.table));
         wide.p.d_kl = a.wide_kl = reinterpret_cast<int32_t *>(take(room.kl));
     }

@@ -17,6 +17,7 @@ struct WinArgs {
     int page_shift;  // of a page that is a power of two, else -1
     float scale_log2;
     float *part_o, *part_ml;  // of a split: [unit][split][tile_rows][head_dim], [unit][split][tile_rows][2]
+    const float *expanded;    // [batch][kv_heads][2]: the powers of two that f16 pages of K and V were taken times
 };
 
 constexpr int WIN_MAX_SPLITS = 64;  // a lane a split in the join
@@ -197,6 +198,9 @@ static osh_status win_join(const WinArgs &a, unsigned units, hipStream_t st) {
 
 // The attention over 16-bit pages of a planned and checked call (osh_window_attn.hip).
 osh_status win_run(const WinArgs &a, unsigned units, hipStream_t st);
+// The same of bf16 queries over pages of f16 that hold the new tokens too, taken times
+// a.expanded; more than 16 rows a key head.
+osh_status win_run_expanded(const WinArgs &a, unsigned units, hipStream_t st);
 
 // Row blocks, splits and scratch of a call.
 static osh_status win_plan(const osh_window_attn *p, WinArgs &a, size_t &scratch) {

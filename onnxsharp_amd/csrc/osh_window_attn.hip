@@ -18,6 +18,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "osh_overlap.h"
 #include "osh_window.h"
@@ -272,9 +273,13 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void window_attn_rows
 //
 // The running maximum moves only when a row's scores pass it by 2^8: weights up to
 // 256 are as exact, and most tiles rescale nothing.
-template <typename T, int C, int KS, int OB, int NW>
+//
+// EXPANDED: queries and outputs are bf16, keys and values f16 pages that hold the new tokens
+// too, taken times a power of two that keeps the largest of a head within 1 (a.expanded); a
+// query is taken so as well, and its powers come back with the softmax's scale and at the end.
+template <typename T, int C, int KS, int OB, int NW, bool EXPANDED>
 __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kernel(WinArgs a) {
-    using H8 = typename Half8<T>::type;
+    using H8 = typename Half8<std::conditional_t<EXPANDED, _Float16, T>>::type;
     constexpr int BUF = 64 * C * 16, RPI = 64 / C, IT = 2 * C / NW;  // rows an instruction, instructions a wave
     static_assert(IT * NW == 2 * C, "loads are dealt evenly");
     extern __shared__ __align__(16) unsigned char lds[];  // two of [K tile][V tile]
@@ -299,10 +304,32 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
     if (r0 >= rows) return;
     T *o = static_cast<T *>(p.d_o);
     const int row = min(r0 + 32 * wave + ql32, rows - 1), tok = row / G, head = h * G + row % G;
-    if (split == 0) win_append<T>(p, sq, b, h, G, r0, 32 * NW, tid, 64 * NW);
+    if (!EXPANDED && split == 0) win_append<T>(p, sq, b, h, G, r0, 32 * NW, tid, 64 * NW);
+    WinSeq held = sq;  // for whom all keys lie in pages
+    if (EXPANDED) held.past = sq.kl;
 
     H8 q[KS];
-    {
+    float scale_log2 = a.scale_log2, back = 1.0f;
+    if constexpr (EXPANDED) {
+        const T *qr = static_cast<const T *>(p.d_q) + (long long)(sq.c0 + tok) * p.q_stride[0] + head * p.q_stride[1];
+        f32x8 f[KS];
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            f[s] = f32x8{};
+            if (16 * s + 8 * hl < d) f[s] = load8(qr + 16 * s + 8 * hl);
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = __builtin_fmaxf(top, __builtin_fabsf(f[s][i]));
+        }
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const int e = top < __builtin_inff() ? min(max(__builtin_amdgcn_frexp_expf(top), -120), 126) : 0;
+        const float by = __builtin_amdgcn_ldexpf(1.0f, -e);
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = __builtin_convertvector(f[s] * by, H8);
+        const float *x = a.expanded + 2 * ((long long)b * p.kv_heads + h);
+        scale_log2 = scale_log2 / by / x[0];
+        back = 1.0f / x[1];
+    } else {
         const T *qr = static_cast<const T *>(p.d_q) + (long long)(sq.c0 + tok) * p.q_stride[0] + head * p.q_stride[1];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
@@ -333,10 +360,10 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
     const int slot = lane % C;
     auto tile_row = [&](int e) { return (wave + NW * e) % C * RPI + lane / C; };
     const int my_tile_row = tile_row(lane % RW);
-    const int fresh0 = cdiv(max(sq.past + base, keys.sink_end), 64);  // first tile of new tokens alone
+    const int fresh0 = EXPANDED ? INT_MAX : cdiv(max(sq.past + base, keys.sink_end), 64);  // first tile of new tokens alone
     int page_id = 0;
     auto fetch_pages = [&](int t) {
-        if (t < fresh0) page_id = win_page(p, sq, keys, b, t * 64 + my_tile_row, a.page_shift);
+        if (t < fresh0) page_id = win_page(p, held, keys, b, t * 64 + my_tile_row, a.page_shift);
     };
     // Heads of 65 to 128 keep the byte offsets of a lane's chunks in a tile of new tokens
     // and sum their rounded weights two an instruction (4% of 8192 tokens without a window);
@@ -378,7 +405,7 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
             fk = static_cast<const T *>(p.d_k_new) + n * p.k_new_stride[0] + h * p.k_new_stride[1];
             fv = static_cast<const T *>(p.d_v_new) + n * p.v_new_stride[0] + h * p.v_new_stride[1];
         } else {
-            mine = win_rows<T>(p, sq, keys, t * 64 + my_tile_row, page_id, a.page_shift, h);
+            mine = win_rows<T>(p, held, keys, t * 64 + my_tile_row, page_id, a.page_shift, h);
         }
 #pragma unroll
         for (int e = 0; e < RW; e++) {
@@ -480,7 +507,7 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int r = 0; r < 16; r++) top = __builtin_fmaxf(top, s[kb][r]);
-        top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * scale_log2;
         if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
             const float old = m;
             m = __builtin_fmaxf(m, top);
@@ -496,7 +523,7 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
             f32x8 f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], a.scale_log2, -ref));
+                f[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], scale_log2, -ref));
                 if (!KEEP) l += f[i];
             }
             w[e] = __builtin_convertvector(f, H8);
@@ -517,7 +544,7 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
     // quads of values 8 e + 4 hl + 0..3: exchanging one quad between the halves of the
     // wave leaves a lane 8 neighbouring values
     const bool mine = wr + ql32 < rows;
-    const float inv = a.splits == 1 ? 1.0f / l : 1.0f;
+    const float inv = EXPANDED ? (a.splits == 1 ? back / l : back) : a.splits == 1 ? 1.0f / l : 1.0f;
     const long long u = (long long)unit * a.splits + split;
     const int tr = 32 * wave + ql32;
     if (a.splits > 1 && mine && hl == 0) {
@@ -545,9 +572,9 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
         }
 }
 
-template <typename T, int C, int KS, int OB, int NW>
+template <typename T, int C, int KS, int OB, int NW, bool EXPANDED = false>
 static osh_status win_tile_launch(const WinArgs &a, unsigned units, hipStream_t st) {
-    OSH_LAUNCH((window_attn_tile_kernel<T, C, KS, OB, NW>), dim3(units * a.splits), dim3(64 * NW), 4 * 64 * C * 16, st, a);
+    OSH_LAUNCH((window_attn_tile_kernel<T, C, KS, OB, NW, EXPANDED>), dim3(units * a.splits), dim3(64 * NW), 4 * 64 * C * 16, st, a);
     OSH_LAUNCH_CHECK("window_attn_tile_kernel");
     return win_join<T>(a, units, st);
 }
@@ -572,6 +599,15 @@ static osh_status win_launch_t(const WinArgs &a, unsigned units, hipStream_t st)
     if (a.p.head_dim <= 64) return a.wide ? win_launch<T, 64, 8>(a, units, st) : win_launch<T, 64, 4>(a, units, st);
     if (a.p.head_dim <= 128) return a.wide ? win_launch<T, 128, 8>(a, units, st) : win_launch<T, 128, 4>(a, units, st);
     return win_launch<T, 256, 4>(a, units, st);
+}
+
+osh_status win_run_expanded(const WinArgs &a, unsigned units, hipStream_t st) {
+    const int d = a.p.head_dim;
+    if (d <= 32) return win_tile_launch<__bf16, 4, 2, 1, 4, true>(a, units, st);
+    if (d <= 64) return win_tile_launch<__bf16, 8, 4, 2, 4, true>(a, units, st);
+    if (d <= 96) return win_tile_launch<__bf16, 16, 6, 3, 4, true>(a, units, st);
+    if (d <= 128) return win_tile_launch<__bf16, 16, 8, 4, 4, true>(a, units, st);
+    return win_tile_launch<__bf16, 32, 16, 8, 4, true>(a, units, st);
 }
 
 osh_status win_run(const WinArgs &a, unsigned units, hipStream_t st) {
