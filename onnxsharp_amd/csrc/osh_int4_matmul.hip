@@ -733,8 +733,11 @@ static Int4Room int4_room(int m, int n, int k, int group, int dtype) {
     if (!r.tile) {
         // Against a launch of int4_rows_kernel, two launches of the slim one cost 4 to 10 us more,
         // by the rows' blocks; it gains what the 16 outputs' own copies of the rows take (11
-        // TB/s) and 0.07 us a MB of weights.  FP32 rows gain where a wave has much to split.
-        const double copies = (double)cdiv(n, 16) * m * k * 2e-6 / 11, weights = (double)n * k * 0.5e-6 * 0.07;
+        // TB/s) and 0.03 us a MB of weights.  Rows against slim, bf16, k of 8192: 16 rows on 4096
+        // outputs 11.4 (11.6) us, 24 16.1 (13.7); 1, 8 and 32 on 16384 24.0 (21.4; 14 against 18
+        // where the weights lie in the last cache), 27.6 (21.9), 64 (31); 1 on 8192 12.0 (14.1).
+        // FP32 rows gain where a wave has much to split: 1 on 4096 23 (16), k of 768 on 768 4.8 (9).
+        const double copies = (double)cdiv(n, 16) * m * k * 2e-6 / 11, weights = (double)n * k * 0.5e-6 * 0.03;
         const double cost = m <= 16 ? 4.2 : m <= 32 ? 7.3 : 10.1;
         r.slim = f32 ? (long long)n * k >= 1 << 24 || m > 32 : copies + weights > cost || m > 64;
         if (!r.slim) return r;
