@@ -729,7 +729,7 @@ static Int4Room int4_room(int m, int n, int k, int group, int dtype) {
     // weights again for each 64 rows (32 in FP32).  Tile against slim: 128 rows of 4096 against
     // 4096 outputs 26.3 (22.2) us, 54.4 (39.7) in FP32; of 1024 against 4096 10.8 (16.0), 18.9
     // (16.9); 256 of 8192 against 8192 63.5 (93.7), 144 (286).
-    r.tile = m > 64 && ((long long)m * n > (f32 ? 1 << 19 : 1 << 20) || (!f32 && k < 2048));
+    r.tile = m > 64 && (nkb > 65535 || (long long)m * n > (f32 ? 1 << 19 : 1 << 20) || (!f32 && k < 2048));
     if (!r.tile) {
         // Against a launch of int4_rows_kernel, two launches of the slim one cost 4 to 10 us more,
         // by the rows' blocks; it gains what the 16 outputs' own copies of the rows take (11
@@ -746,6 +746,10 @@ static Int4Room int4_room(int m, int n, int k, int group, int dtype) {
         const long long tiles = (long long)cdiv(n, 128) * cdiv(m, 16 * mb);
         r.kr = (int)std::max(1LL, std::min<long long>(most, tiles * nkb / device_cus()));
         r.parts = cdiv(nkb, r.kr);
+        if (r.parts > 65535 && m <= 64) {  // more than a grid takes
+            r.slim = false;
+            return r;
+        }
         r.pitch = cdiv(n, 128) * 128;
         r.total = r.parts > 1 ? (size_t)r.parts * m * r.pitch * 4 : 0;
         return r;

@@ -29,11 +29,12 @@ struct Kv4Args {
     // many bf16 rows: the visible cache in f16, and what the 16-bit kernel is told about it
     _Float16 *k_wide, *v_wide;    // [batch * wide_blocks][kv_heads][WIDE_PAGE][head_dim]
     float *wide_by;               // [batch][kv_heads][2]: what K and V are taken times
+    float *wide_top;              // [batch][kv_heads][RANGE_PARTS][2]: the largest of each part of the keys
     int32_t *wide_table, *wide_kl;
     int wide_blocks, wide_width;  // pages of a sequence, entries of its table
 };
 
-constexpr int WIDE_PAGE = 64;
+constexpr int WIDE_PAGE = 64, RANGE_PARTS = 16;
 
 // -------------------------------------------------------------- quantization
 
@@ -49,11 +50,16 @@ __device__ __forceinline__ void kv4_append(const Kv4Args &a, const WinSeq &sq, i
     for (long long e0 = tid & ~63LL; e0 < total; e0 += threads) {
         const long long e = e0 + (tid & 63);
         const bool in = e < total;
-        const long long item = in ? e / chunks : 0;
-        const int c = in ? (int)(e - item * chunks) : 0;
+        long long item = 0, t = 0;
+        int c = 0, h = h0;
+        if (total <= INT_MAX) {  // divisions of 32 bits
+            const unsigned u = in ? (unsigned)e : 0u, i = u / (unsigned)chunks, at = i / 2 / (unsigned)heads;
+            c = (int)(u - i * chunks), h += (int)(i / 2 - at * heads), item = i, t = t0 + (int)at;
+        } else if (in) {
+            item = e / chunks, c = (int)(e - item * chunks), h += (int)(item / 2 % heads), t = t0 + item / 2 / heads;
+        }
         const bool is_v = item & 1;
-        const int h = h0 + (int)(item / 2 % heads);
-        const long long t = t0 + item / 2 / heads, row = sq.c0 + t;
+        const long long row = sq.c0 + t;
         const T *src = static_cast<const T *>(is_v ? p.d_v_new : p.d_k_new);
         const int64_t *st = is_v ? p.v_new_stride : p.k_new_stride;
         f32x8 f = {};
@@ -131,17 +137,18 @@ __device__ __forceinline__ WideBlocks kv4_blocks(const osh_window_attn &p, const
 
 // The power of two that keeps a head's largest visible key, and value, within 1.  f16's 11 bits
 // are then 8 times as close as bf16's rounding of the output down to 2^-14 of it (bf16 keys and
-// values add as much error as the output's own rounding twice over).  blockIdx: head, sequence.
+// values add as much error as the output's own rounding twice over).  First the largest of each
+// of RANGE_PARTS parts of the keys; kv4_expand_kernel joins them.  blockIdx: part and head, sequence.
 template <typename T>
-__global__ __launch_bounds__(1024) void kv4_range_kernel(Kv4Args a, int groups) {
+__global__ __launch_bounds__(256) void kv4_range_kernel(Kv4Args a, int groups) {
     const osh_window_attn &p = a.w.p;
-    const int b = blockIdx.y, h = blockIdx.x;
+    const int b = blockIdx.y, h = blockIdx.x / RANGE_PARTS, part = blockIdx.x % RANGE_PARTS;
     const WinSeq sq = win_seq(p, b);
     if (!sq.ok || sq.ql == 0) return;
     const WinKeys keys = win_keys(p, sq, 0, sq.ql - 1);
-    __shared__ float s_top[2][16];
+    __shared__ float s_top[2][4];
     float top[2] = {0.0f, 0.0f};
-    for (int v = threadIdx.x; v < keys.count; v += 1024) {
+    for (int v = part * 256 + threadIdx.x; v < keys.count; v += RANGE_PARTS * 256) {
         const int j = keys.at(v), slot = j % p.page, id = p.d_table[b * p.table_stride + j / p.page];
         if ((unsigned)id >= (unsigned)p.pages) continue;
 #pragma unroll
@@ -163,35 +170,45 @@ __global__ __launch_bounds__(1024) void kv4_range_kernel(Kv4Args a, int groups) 
     }
     __syncthreads();
     if (threadIdx.x < 2) {
-        float t = 0.0f;
-        for (int w = 0; w < 16; w++) t = __builtin_fmaxf(t, s_top[threadIdx.x][w]);
-        const int e = min(max(__builtin_amdgcn_frexp_expf(t), -120), 126);
-        a.wide_by[2 * ((long long)b * p.kv_heads + h) + threadIdx.x] = __builtin_amdgcn_ldexpf(1.0f, -e);
+        float t = s_top[threadIdx.x][0];
+        for (int w = 1; w < 4; w++) t = __builtin_fmaxf(t, s_top[threadIdx.x][w]);
+        a.wide_top[2 * (((long long)b * p.kv_heads + h) * RANGE_PARTS + part) + threadIdx.x] = t;
     }
 }
 
 // The visible keys and values, the new ones too, into f16 pages, and the table of those.
-// blockIdx.y is the sequence, blockIdx.x deals out its pages.
+// blockIdx.y is the sequence, blockIdx.x and .z deal out its pages and heads.
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_expand_kernel(Kv4Args a, int group_log) {
     const osh_window_attn &p = a.w.p;
     const int b = blockIdx.y, d = p.head_dim, chunks = d / 8;
     const WinSeq sq = win_seq(p, b);
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.wide_kl[b] = sq.ok ? sq.kl : -1;
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.wide_kl[b] = sq.ok ? sq.kl : -1;
     if (!sq.ok || sq.ql == 0) return;
     const WinKeys keys = win_keys(p, sq, 0, sq.ql - 1);
     const WideBlocks blocks = kv4_blocks(p, sq, keys);
+    for (int h = blockIdx.z; h < p.kv_heads; h += gridDim.z)
     for (int at = blockIdx.x; at < a.wide_blocks; at += gridDim.x) {
         const int block = blocks.at(at);
-        if (block >= blocks.count) return;
-        const long long page = (long long)b * a.wide_blocks + at;
-        if (threadIdx.x == 0) a.wide_table[(long long)b * a.wide_width + block] = (int)page;
-        for (int e = threadIdx.x; e < p.kv_heads * WIDE_PAGE * chunks; e += 256) {
-            const int c = e % chunks, in = e / chunks % WIDE_PAGE, h = e / chunks / WIDE_PAGE;
+        if (block >= blocks.count) break;
+        const long long head = (long long)b * p.kv_heads + h, page = (long long)b * a.wide_blocks + at;
+        float by[2];
+#pragma unroll
+        for (int is_v = 0; is_v < 2; is_v++) {
+            float top = a.wide_top[2 * (head * RANGE_PARTS + threadIdx.x % RANGE_PARTS) + is_v];
+#pragma unroll
+            for (int o = 1; o < RANGE_PARTS; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+            by[is_v] = __builtin_amdgcn_ldexpf(1.0f, -min(max(__builtin_amdgcn_frexp_expf(top), -120), 126));
+        }
+        if (threadIdx.x == 0) {
+            if (h == 0) a.wide_table[(long long)b * a.wide_width + block] = (int)page;
+            if (at == 0) a.wide_by[2 * head] = by[0], a.wide_by[2 * head + 1] = by[1];
+        }
+        for (int e = threadIdx.x; e < WIDE_PAGE * chunks; e += 256) {
+            const int in = e / chunks, c = e - in * chunks;
             const int j = block * WIDE_PAGE + in;
             if (j >= sq.kl || (j < keys.lo && j >= p.sinks)) continue;
             const int slot = j % p.page, id = p.d_table[b * p.table_stride + j / p.page];
-            const float *by = a.wide_by + 2 * ((long long)b * p.kv_heads + h);
             f32x8 k = f32x8{} + __builtin_nanf(""), v = {};
             if ((unsigned)id < (unsigned)p.pages) {
                 auto load = [&](const void *codes, const int64_t *st, const void *pairs, const long long *pst, float by) {
@@ -748,11 +765,11 @@ static osh_status kv4_wide(const Kv4Args &a, const WinArgs &wide, int group, uns
                                        : kv4_append_all<__bf16, 16>(a, st);
     if (s) return s;
     const osh_window_attn &p = a.w.p;
-    OSH_LAUNCH(kv4_range_kernel<__bf16>, dim3((unsigned)p.kv_heads, (unsigned)p.batch), dim3(1024), 0, st, a,
+    OSH_LAUNCH(kv4_range_kernel<__bf16>, dim3((unsigned)p.kv_heads * RANGE_PARTS, (unsigned)p.batch), dim3(256), 0, st, a,
                p.head_dim / group);
     OSH_LAUNCH_CHECK("kv4_range_kernel");
     const int x = std::min(a.wide_blocks, std::max(1, 65536 / p.batch));
-    OSH_LAUNCH(kv4_expand_kernel<__bf16>, dim3((unsigned)x, (unsigned)p.batch), dim3(256), 0, st, a, __builtin_ctz(group));
+    OSH_LAUNCH(kv4_expand_kernel<__bf16>, dim3((unsigned)x, (unsigned)p.batch, (unsigned)std::min(p.kv_heads, 256)), dim3(256), 0, st, a, __builtin_ctz(group));
     OSH_LAUNCH_CHECK("kv4_expand_kernel");
     return win_run_expanded(wide, units, st);
 }
@@ -775,7 +792,7 @@ struct Kv4Room {
 
 // Rows of a key head from which a bf16 call first expands the visible cache to f16, and the room
 // that may take.  4096 tokens behind 12288, 32 heads of 128 on 8, window 8192: 1470 us in blocks
-// of 16 rows, 740 so; 4 x 64 tokens (256 rows) behind 8128 122 in blocks.  f16 calls have no
+// of 16 rows, 690 so; 4 x 64 tokens (256 rows) behind 8128 122 in blocks.  f16 calls have no
 // type with bits to spare for it.
 constexpr int WIDE_ROWS = 512;
 constexpr size_t WIDE_MAX = (size_t)16 << 30;
@@ -809,7 +826,7 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
         w.k_stride[2] = w.v_stride[2] = WIDE_PAGE * head;
         if (const osh_status st = win_plan(&w, wide, room.part)) return st;
         room.part = align(room.part);
-        room.by = align((size_t)w.batch * w.kv_heads * 8);
+        room.by = align((size_t)w.batch * w.kv_heads * 8 * (1 + RANGE_PARTS));
         room.table = align((size_t)w.batch * args.wide_width * 4);
         room.kl = align((size_t)w.batch * 4);
         const double bytes = 4.0 * pages * w.kv_heads * WIDE_PAGE * head;
@@ -921,6 +938,7 @@ OSH_API osh_status osh_kv4_attention(const osh_kv4_attn *q, void *d_scratch, osh
         char *at = static_cast<char *>(d_scratch) + room.part;
         auto take = [&](size_t n) { return at += n, at - n; };
         wide.expanded = a.wide_by = reinterpret_cast<float *>(take(room.by));
+        a.wide_top = a.wide_by + 2LL * p->batch * p->kv_heads;
         wide.p.d_k_pages = a.k_wide = reinterpret_cast<_Float16 *>(take(room.page));
         wide.p.d_v_pages = a.v_wide = reinterpret_cast<_Float16 *>(take(room.page));
         wide.p.d_table = a.wide_table = reinterpret_cast<int32_t *>(take(room.table));
