@@ -145,6 +145,26 @@ def test_rows_of_float32_keep_their_24_bits(cuda, m):
     assert (Int4MatMulLayer().forward(t["x"], weight(t)) == 1 + 2.0 ** -23).all()
 
 
+@pytest.mark.parametrize("m", [3, 70, 300])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_of_any_size(cuda, m, group, dtype):
+    # zeros, the type's smallest numbers, signs, and neighbours many powers of two apart
+    dt = TYPES[dtype]
+    t = make(cuda, m, 200, 1280, group, True, dt)
+    torch.manual_seed(m + group)
+    lo, hi = (-24, 3) if dtype == "f16" else (-100, 30)
+    e = torch.randint(lo, hi, t["scales"].shape, device=cuda).float()
+    t["scales"] = (torch.exp2(e) * (1 + torch.rand_like(e)) * torch.where(torch.rand_like(e) < 0.3, -1.0, 1.0)).to(dt)
+    t["scales"][torch.rand_like(e) < 0.2] = 0
+    t["scales"][:20] = 0
+    t["scales"][20:40, 1:] = 0
+    t["x"] *= 0.01
+    y = Int4MatMulLayer().forward(t["x"], weight(t))
+    check(t, y)
+    assert (y[:, :20] == 0).all()
+
+
 @pytest.mark.parametrize("m", [3, 70])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_that_are_not_finite(cuda, m, dtype):
