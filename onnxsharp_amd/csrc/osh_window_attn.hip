@@ -327,7 +327,10 @@ __global__ __launch_bounds__(64 * NW, C > 16 ? 1 : 2) void window_attn_tile_kern
 #pragma unroll
         for (int s = 0; s < KS; s++) q[s] = __builtin_convertvector(f[s] * by, H8);
         const float *x = a.expanded + 2 * ((long long)b * p.kv_heads + h);
-        scale_log2 = scale_log2 / by / x[0];
+        // by the exponents' sum, kept among normal numbers: at 0 a hidden key's -infinity, and at
+        // infinity a score of 0, would make the row NaN
+        const int back2 = e + 1 - __builtin_amdgcn_frexp_expf(x[0]);
+        scale_log2 = __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_ldexpf(scale_log2, back2), 0x1p-126f), 0x1p127f);
         back = 1.0f / x[1];
     } else {
         const T *qr = static_cast<const T *>(p.d_q) + (long long)(sq.c0 + tok) * p.q_stride[0] + head * p.q_stride[1];
