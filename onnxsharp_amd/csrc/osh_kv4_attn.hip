@@ -26,6 +26,7 @@ struct Kv4Args {
     void *k_stored, *v_stored;
     long long ks_stride[3], vs_stride[3], k_stored_stride[2], v_stored_stride[2];
     unsigned page_mul, page_log;  // j / page = umulhi(4 j, page_mul) >> page_log for j < 2^30
+    bool append;                  // row blocks quantize the new tokens themselves, else a launch in front
     // many bf16 rows: the visible cache in f16, and what the 16-bit kernel is told about it
     _Float16 *k_wide, *v_wide;    // [batch * wide_blocks][kv_heads][WIDE_PAGE][head_dim]
     float *wide_by;               // [batch][kv_heads][2]: what K and V are taken times
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     if (!sq.ok) {
         if (tile == 0 && split == 0) {
             win_fill_nan<T>(p, sq, h, G, tid, 64 * WAVES);
-            kv4_append<T, 4 * GS>(args, sq, b, h, h + 1, 0, sq.held, tid, 64 * WAVES);  // NaN to the stored values
+            if (args.append) kv4_append<T, 4 * GS>(args, sq, b, h, h + 1, 0, sq.held, tid, 64 * WAVES);  // NaN to the stored values
         }
         return;
     }
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     const int s_end = min(steps, (split + 1) * per);
     // the new ones among this workgroup's keys go to the cache first, from where all keys are
     // read; another row block may write the same bytes there
-    {
+    if (args.append) {
         const int v0 = split * per * 64, v1 = min(nv, s_end * 64);
         const int t0 = max(0, (v0 < nv ? keys.at(v0) : sq.kl) - sq.past), t1 = v1 > v0 ? keys.at(v1 - 1) + 1 - sq.past : 0;
         if (t1 > t0) kv4_append<T, 4 * GS>(args, sq, b, h, h + 1, t0, t1, tid, 64 * WAVES);
@@ -760,10 +761,6 @@ static osh_status kv4_launch_g(const Kv4Args &a, unsigned units, hipStream_t st)
 }
 
 static osh_status kv4_wide(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
-    const osh_status s = group == 32   ? kv4_append_all<__bf16, 4>(a, st)
-                         : group == 64 ? kv4_append_all<__bf16, 8>(a, st)
-                                       : kv4_append_all<__bf16, 16>(a, st);
-    if (s) return s;
     const osh_window_attn &p = a.w.p;
     OSH_LAUNCH(kv4_range_kernel<__bf16>, dim3((unsigned)p.kv_heads * RANGE_PARTS, (unsigned)p.batch), dim3(256), 0, st, a,
                p.head_dim / group);
@@ -776,6 +773,12 @@ static osh_status kv4_wide(const Kv4Args &a, const WinArgs &wide, int group, uns
 
 template <typename T>
 static osh_status kv4_launch(const Kv4Args &a, const WinArgs &wide, int group, unsigned units, hipStream_t st) {
+    if (!a.append) {
+        const osh_status s = group == 32   ? kv4_append_all<T, 4>(a, st)
+                             : group == 64 ? kv4_append_all<T, 8>(a, st)
+                                           : kv4_append_all<T, 16>(a, st);
+        if (s) return s;
+    }
     if constexpr (__is_same(T, __bf16)) {
         if (a.wide_blocks) return kv4_wide(a, wide, group, units, st);
     }
@@ -844,6 +847,12 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
     a.tiles = cdiv(rows, a.tile_rows);
     const long long units = (long long)p->w.batch * p->w.kv_heads * a.tiles;
     if (units >= (1LL << 22)) return fail(OSH_E_UNSUPPORTED, "Kv4Attention: too many row blocks (%lld)", units);
+    // A sequence's few row blocks quantize the new tokens among their keys each for itself, which
+    // saves a launch: with 2, 4 and 8 of them, one sequence behind 2000 keys (32 heads of 128 on 8) in
+    // groups of 128, 15.4 (18.7 with one launch in front), 17.1 (19.2), 22.9 (22.2) us; 64 of them
+    // 70.6 (71.6), 135 (128), 279 (234).  With many it is the square of the new tokens: 4096 f16 ones
+    // behind 12288 10065 (1763).
+    args.append = a.tiles == 1 || (a.tiles <= 4 && units <= device_cus());
     const long long span = std::min<long long>(p->w.max_kv, (long long)p->w.window + p->w.sinks + 16 / a.group);
     const long long want = units ? std::max(1LL, 2LL * device_cus() / units) : 1;
     a.splits = (int)std::max(1LL, std::min({want, span / 256, (long long)WIN_MAX_SPLITS}));
