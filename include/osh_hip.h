@@ -720,8 +720,9 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
  * osh_window_attention does, with every key and value, the new ones too, as the cache
  * stands for it: o depends on the cache alone, not on how its tokens came in calls.  A query
  * that sees a key whose page id lies outside [0, pages) gets NaN, a new one too.
- * Scores are FP32 sums of the exact values.  What is rounded: a weight times a value's scale, to
- * dtype.  From 512 rows a key head on (max_q * (q_heads / kv_heads)) bf16 calls take queries,
+ * Scores are FP32 sums of the exact values; of a weight times a value's scale 16 bits are kept, in
+ * f16 as far as they lie above 2^-34 of the largest such scale of the group in the row block's keys.
+ * From 512 rows a key head on (max_q * (q_heads / kv_heads)) bf16 calls take queries,
  * keys, values and weights in f16, times a power of two that puts the largest of a query, and a
  * head's largest visible key and value, between 1/2 and 1: what lies below 2^-14 of it keeps fewer
  * than f16's 11 bits.  A value that is not finite may make other queries of its sequence NaN, as

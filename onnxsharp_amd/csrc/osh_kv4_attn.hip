@@ -4,11 +4,12 @@
 // Up to 512 rows of a key head, and f16 calls (kv4_rows_kernel): the products take the codes,
 // which are exact in 16 bits; scales and minima stay in FP32:
 //   q . k_j = sum over groups of scale_j (q . code_j) + lo_j (sum of q over the group),
-//   sum_j p_j v_j = sum_j (p_j scale_j) (code_j - 8) + sum_j p_j (lo_j + 8 scale_j).
-// Rounded are the weights p_j scale_j alone, half a step of dtype each as the weights are
-// over a 16-bit cache; codes less 8 have the size of the values about the group's middle, so
-// that the roundings weigh what they weigh there.  (8 is taken off the sums by a product
-// with the constant -8.)
+//   sum_j p_j v_j = sum_j (p_j scale_j) code_j + sum_j p_j lo_j.
+// The matrix instructions take p_j scale_j as two numbers of dtype, the second what rounding to
+// the first leaves: 16 bits of a bf16 weight, 22 of an f16 one.  The first alone leaves the output
+// a quarter more error than its own rounding (2.2e-3 of o for 1.7e-3 in bf16) and is 2 to 8% faster
+// (64 sequences of 5000 keys, 32 heads of 128 on 8: 70.2 us for 72.2 in groups of 128, 104.5 for
+// 108.5 of 32).
 // More rows in bf16: the visible cache is expanded to f16 pages once, and the kernel of
 // osh_window_attn.hip reads those.
 #include <limits.h>
@@ -379,18 +380,15 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     const int v_hi = my_pos + shift, v_lo = max(my_pos - p.window + 1, keys.lo) + shift;
 
     float m = -__builtin_inff(), l = 0.0f, zsum[NG];
-    f32x4 acc[OB], accz[NG];
+    f32x4 acc[OB];
 #pragma unroll
     for (int i = 0; i < OB; i++) acc[i] = f32x4{0, 0, 0, 0};
+    // f16 weights: p scale times a power of two of each group, since f16 has no room for the
+    // scales' own range: the scale that sets it becomes 2^9 to 2^10, and none passes 2^15
+    constexpr bool UNIT = __is_same(T, _Float16);
+    float by[NG];
 #pragma unroll
-    for (int e = 0; e < NG; e++) accz[e] = f32x4{0, 0, 0, 0}, zsum[e] = 0.0f;
-    // f16 weights: times 1 / unit, a power of two that keeps p scale / unit within 1, since
-    // f16 has no room for the scales' own range
-    constexpr bool UNIT = sizeof(H8) && __is_same(T, _Float16);
-    float unit_scale = 0x1p-100f;
-    H8 minus8;
-#pragma unroll
-    for (int i = 0; i < 8; i++) minus8[i] = -8.0f;
+    for (int e = 0; e < NG; e++) zsum[e] = 0.0f, by[e] = 0x1p127f;  // the first scale passes
 
     unsigned char *mine = lds + wave * WAVE_LDS;
     const float2 *kpair = reinterpret_cast<const float2 *>(mine + 4 * TILE + 256 + 2 * NG * 256), *vpair = kpair + NG * 64;
@@ -465,34 +463,29 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
         __builtin_memcpy(t, &u, 4);
         return float2{(float)t[0], (float)t[1]};
     };
-    // a step's pairs in FP32 to LDS: K's times the softmax's scale, V's scale and middle
+    // a step's pairs in FP32 to LDS: K's times the softmax's scale, V's scale as the weights take it
     auto convert = [&](bool in, bool bad) {
         float2 kp[NG], vp[NG];
-        float top = 0.0f;
 #pragma unroll
         for (int e = 0; e < NG; e++) {
             kp[e] = pair_of(raw_pair(0, e)), vp[e] = pair_of(raw_pair(1, e));
             kp[e].x *= a.scale_log2, kp[e].y *= a.scale_log2;
             if (bad) kp[e].x = __builtin_nanf("");
-            vp[e].y = __builtin_fmaf(8.0f, vp[e].x, vp[e].y);
             if (!in) vp[e] = float2{0.0f, 0.0f};
-            if (UNIT) top = __builtin_fmaxf(top, vp[e].x);
-        }
-        if (UNIT) {
+            if constexpr (UNIT) {
+                float top = vp[e].x;
+                vp[e].x *= by[e];
+                if (__builtin_amdgcn_ballot_w64(vp[e].x > 0x1p15f) != 0) {
+                    const float scale = top;
 #pragma unroll
-            for (int i = 32; i; i >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, i));
-            if (__builtin_amdgcn_readfirstlane(top > unit_scale)) {
-                const float next = __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
-                const float fade = unit_scale / next;
-                unit_scale = next;
+                    for (int i = 32; i; i >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, i));
+                    const float next = __uint_as_float((263u << 23) - (__float_as_uint(top) & 0x7f800000u));
+                    const float fade = next / by[e];
+                    by[e] = next, vp[e].x = scale * next;
 #pragma unroll
-                for (int i = 0; i < OB; i++) acc[i] *= fade;
-#pragma unroll
-                for (int e = 0; e < NG; e++) accz[e] *= fade;
+                    for (int i = 2 * GS * e; i < 2 * GS * (e + 1); i++) acc[i] *= fade;
+                }
             }
-            const float inv = 1.0f / unit_scale;
-#pragma unroll
-            for (int e = 0; e < NG; e++) vp[e].x *= inv;
         }
 #pragma unroll
         for (int e = 0; e < NG; e++) {
@@ -574,7 +567,7 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
 #pragma unroll
             for (int i = 0; i < OB; i++) acc[i] *= fade;
 #pragma unroll
-            for (int e = 0; e < NG; e++) accz[e] *= fade, zsum[e] *= fade;
+            for (int e = 0; e < NG; e++) zsum[e] *= fade;
         }
         // lane jl of 16 reads 16 codes of key 16 g + jl and gets 16 keys' codes of value jl
         unsigned vw[OB][2];
@@ -600,7 +593,8 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
 #pragma unroll
         for (int e = 0; e < NG; e++) {
             if (NG > 2 && SUB == 1) __builtin_amdgcn_sched_barrier(0);
-            // weights in the order of codes8: of 8 keys the even ones, then the odd ones
+            // weights in the order of codes8: of 8 keys the even ones, then the odd ones; what
+            // rounding to T leaves of them is a second operand
             float w[KPL];
 #pragma unroll
             for (int i = 0; i < KPL; i++) {
@@ -608,31 +602,42 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
                 w[i] = s[i] * vp.x;
                 zsum[e] = __builtin_fmaf(s[i], vp.y, zsum[e]);
             }
-            unsigned pw[8];
-            auto two = [&](int i, int j) {
-                typedef T T2 __attribute__((ext_vector_type(2)));
-                const T2 v = {(T)w[i], (T)w[j]};
-                return __builtin_bit_cast(unsigned, v);
-            };
+            H8 p[2][2];  // by part and 8 keys
 #pragma unroll
-            for (int i = 0; i < 8; i++) {  // registers 0..3 are of the first 8 keys
-                if constexpr (SUB == 1) pw[i] = two(8 * (i >> 2) + 4 * (i & 1) + (i >> 1 & 1), 8 * (i >> 2) + 4 * (i & 1) + (i >> 1 & 1) + 2);
-                if constexpr (SUB == 2) pw[i] = sub == i >> 2 ? two(4 * (i & 1) + (i >> 1 & 1), 4 * (i & 1) + (i >> 1 & 1) + 2) : 0u;
-                if constexpr (SUB == 4) pw[i] = sub == 2 * (i >> 2) + (i & 1) ? two(i >> 1 & 1, (i >> 1 & 1) + 2) : 0u;
-            }
-            H8 p0, p1;
-            __builtin_memcpy(&p0, pw, 16);
-            __builtin_memcpy(&p1, pw + 4, 16);
-            accz[e] = mma16(minus8, p0, accz[e]);
-            accz[e] = mma16(minus8, p1, accz[e]);
+            for (int part = 0; part < 2; part++) {
+                unsigned pw[8];
+                auto two = [&](int i, int j) {
+                    typedef T T2 __attribute__((ext_vector_type(2)));
+                    const T2 v = {(T)w[i], (T)w[j]};
+                    if (part == 0) w[i] = __builtin_fmaf((float)v[0], -1.0f, w[i]), w[j] = __builtin_fmaf((float)v[1], -1.0f, w[j]);
+                    return __builtin_bit_cast(unsigned, v);
+                };
 #pragma unroll
-            for (int i = 2 * GS * e; i < 2 * GS * (e + 1); i++) {
-                H8 v;
-                codes8(vw[i][0], v);
-                acc[i] = mma16(v, p0, acc[i]);
-                codes8(vw[i][1], v);
-                acc[i] = mma16(v, p1, acc[i]);
+                for (int i = 0; i < 8; i++) {  // registers 0..3 are of the first 8 keys
+                    if constexpr (SUB == 1) pw[i] = two(8 * (i >> 2) + 4 * (i & 1) + (i >> 1 & 1), 8 * (i >> 2) + 4 * (i & 1) + (i >> 1 & 1) + 2);
+                }
+                if constexpr (SUB > 1) {
+                    unsigned at[KPL / 2];
+#pragma unroll
+                    for (int i = 0; i < KPL / 2; i++) at[i] = two(4 * (i >> 1) + (i & 1), 4 * (i >> 1) + (i & 1) + 2);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int of = SUB == 2 ? i >> 2 : 2 * (i >> 2) + (i & 1);
+                        pw[i] = sub == of ? at[SUB == 2 ? 2 * (i & 1) + (i >> 1 & 1) : i >> 1 & 1] : 0u;
+                    }
+                }
+                __builtin_memcpy(&p[part][0], pw, 16);
+                __builtin_memcpy(&p[part][1], pw + 4, 16);
             }
+#pragma unroll
+            for (int i = 2 * GS * e; i < 2 * GS * (e + 1); i++)
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    H8 v;
+                    codes8(vw[i][half], v);
+                    acc[i] = mma16(v, p[0][half], acc[i]);
+                    acc[i] = mma16(v, p[1][half], acc[i]);
+                }
         }
     };
     int st = split * per + wave;
@@ -679,8 +684,8 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
     }
 #pragma unroll
     for (int i = 0; i < OB; i++) {
-        f32x4 f = acc[i] + accz[i / (2 * GS)];
-        if (UNIT) f *= unit_scale;
+        f32x4 f = acc[i];
+        if (UNIT) f *= 1.0f / by[i / (2 * GS)];
         f += zsum[i / (2 * GS)];
         *reinterpret_cast<f32x4 *>(os + (wave * 16 + jl) * OP + 16 * i + 4 * g) = f;
     }
