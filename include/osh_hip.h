@@ -643,8 +643,8 @@ OSH_API osh_status osh_block_norm(int64_t rows, int cols, int dtype, const void 
  * osh_int4_packed_bytes bytes at 16-byte alignment.
  * a [m][lda] and res [m][ldr] of type dtype at any pitch and alignment of whole elements;
  * bias FP32 and res may be NULL; act: none, relu, silu or gelu.  res may be y itself (same
- * pitch); no other overlap of y.  group is 32, 64 or a multiple of 128.  The sums are FP32 and
- * nothing is rounded before them.  Weights of one group with a scale of 0 are 0.  A row that
+ * pitch); no other overlap of y.  group is 32, 64 or a multiple of 128.  The sums are FP32, run
+ * from group to group (at most 128 of k at a time), and nothing is rounded before them.  Weights of one group with a scale of 0 are 0.  A row that
  * holds a NaN or an infinity gives outputs that are not finite; n, k <= 2^28, m <= 64 * 65535. */
 OSH_API osh_status osh_int4_packed_bytes(int n, int k, int group, int dtype, int has_zeros, size_t *bytes);
 OSH_API osh_status osh_int4_pack(int n, int k, int group, int dtype, const void *d_codes, int64_t ldc,
