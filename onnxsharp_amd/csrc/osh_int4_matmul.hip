@@ -730,12 +730,15 @@ static Int4Room int4_room(int m, int n, int k, int group, int dtype) {
     r.tile = m > 64 && (nkb > 65535 || (long long)m * n > (f32 ? 1 << 19 : 1 << 20) || (!f32 && k < 2048));
     if (!r.tile) {
         // Against a launch of int4_rows_kernel, two launches of the slim one cost 4 to 10 us more,
-        // by the rows' blocks; it gains what the 16 outputs' own copies of the rows take (11
-        // TB/s) and 0.03 us a MB of weights.  Rows against slim, bf16, k of 8192: 16 rows on 4096
-        // outputs 11.4 (11.6) us, 24 16.1 (13.7); 1, 8 and 32 on 16384 24.0 (21.4; 14 against 18
-        // where the weights lie in the last cache), 27.6 (21.9), 64 (31); 1 on 8192 12.0 (14.1).
+        // by the rows' blocks; it gains what the 16 outputs' own copies of the rows take (20 TB/s as
+        // one block of 16, 11 as more) and 0.055 us a MB of weights.  Rows against slim in bf16, every
+        // weight out of HBM (1.2 GB of them in turn): 1 row of 8192 on 8192 outputs 11.8 (14.4) us, on
+        // 16384 22.9 (22.3), on 32768 43.0 (36.3); of 4096 on 28672 19.3 (19.7); 8 rows of 4096 on
+        // 12288 11.4 (13.6), of 8192 on 16384 26.7 (21.0); 16 of 4096 on 4096 6.9 (9.5), on 12288 15.2
+        // (14.4); 32 on 4096 10.6 (12.3), on 12288 25.6 (18.1).  Weights that the last cache still
+        // holds change it: 1 row on 16384 takes 14 (18).
         // FP32 rows gain where a wave has much to split: 1 on 4096 23 (16), k of 768 on 768 4.8 (9).
-        const double copies = (double)cdiv(n, 16) * m * k * 2e-6 / 11, weights = (double)n * k * 0.5e-6 * 0.03;
+        const double copies = (double)cdiv(n, 16) * m * k * 2e-6 / (m <= 16 ? 20 : 11), weights = (double)n * k * 0.5e-6 * 0.055;
         const double cost = m <= 16 ? 4.2 : m <= 32 ? 7.3 : 10.1;
         r.slim = f32 ? (long long)n * k >= 1 << 24 || m > 32 : copies + weights > cost || m > 64;
         if (!r.slim) return r;
