@@ -53,11 +53,10 @@ def _check_tensor(layer, what: str, t: torch.Tensor, dtype: torch.dtype, shape: 
         raise _invalid(layer, f"{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _check_sizes(layer, **sizes: int) -> None:
+def _check_sizes(layer, *sizes: int) -> None:
     """The C ABI takes 32-bit sizes, and ctypes would cut longer ones down to those."""
-    for what, n in sizes.items():
-        if n > _MAX_INT:
-            raise N.OshUnsupported(N.OSH_E_UNSUPPORTED, f"{type(layer).__name__} '{layer.name}': {what} {n}")
+    if max(sizes) > _MAX_INT:
+        raise N.OshUnsupported(N.OSH_E_UNSUPPORTED, f"{type(layer).__name__} '{layer.name}': a size of {max(sizes)}")
 
 
 def _check_device(layer, *tensors) -> torch.device:
@@ -120,7 +119,7 @@ class RmsNormQuantLayer:
         if x.dim() != 2:
             raise _invalid(self, f"x must be [rows, cols], got {tuple(x.shape)}")
         rows, cols = x.shape
-        _check_sizes(self, cols=cols)
+        _check_sizes(self, cols)
         _check_tensor(self, "gamma", gamma, x.dtype, (cols,))
         if residual is not None:
             _check_tensor(self, "residual", residual, x.dtype, x.shape)
@@ -176,7 +175,7 @@ class QuantMatMulLayer:
             raise _invalid(self, f"a {tuple(a.shape)} and w {tuple(w.shape)} must be [m, k] and [n, k]")
         m, k = a.shape
         n = w.shape[0]
-        _check_sizes(self, m=m, n=n, k=k)
+        _check_sizes(self, m, n, k)
         _check_tensor(self, "a_scale", a_scale, torch.float32, (m,))
         _check_tensor(self, "w_scale", w_scale, torch.float32, (n,))
         if bias is not None:
@@ -232,7 +231,7 @@ class BlockNormLayer:
         if x.dim() != 2:
             raise _invalid(self, f"x must be [rows, cols], got {tuple(x.shape)}")
         rows, cols = x.shape
-        _check_sizes(self, cols=cols)
+        _check_sizes(self, cols)
         if branch is None and gamma is None:
             raise _invalid(self, "neither a branch nor gamma")
         if branch is None and not (post_gamma is None and gate is None and out_h is None):
@@ -283,7 +282,7 @@ class Int4Weight:
         if codes.dim() != 2 or k < 1 or group < 1:
             raise _invalid(self, f"codes must be [n, ceil(k / 2)], got {tuple(codes.shape)} for k {k} in groups of {group}")
         n, groups = codes.shape[0], -(-k // group)
-        _check_sizes(self, n=n, k=k, group=group)
+        _check_sizes(self, n, k, group)
         _check_tensor(self, "codes", codes, torch.uint8, (n, -(-k // 2)))
         if scales.dtype not in _ROW_TYPES:
             raise TypeError(f"Int4Weight '{name}': scales must be float32, float16 or bfloat16, got {scales.dtype}")
@@ -349,7 +348,7 @@ class Int4MatMulLayer:
         if a.dim() != 2 or a.shape[1] != w.k:
             raise _invalid(self, f"a must be [m, {w.k}], got {tuple(a.shape)}")
         m, n, k = a.shape[0], w.n, w.k
-        _check_sizes(self, m=m)
+        _check_sizes(self, m)
         if bias is not None:
             _check_tensor(self, "bias", bias, torch.float32, (n,))
             bias = bias.contiguous()
