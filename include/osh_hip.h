@@ -714,8 +714,8 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
  * (scale, lo) of type dtype:
  *   lo = min, scale = round((max - lo) / 15), code = rint((v - lo) / scale) within 0..15
  *   (0 where scale is 0), in FP32; the cache stands for lo + scale * code.
- * A group that holds a NaN or an infinity is kept as NaN.  Codes lie two a byte, the even
- * value in the low half.
+ * A group that holds a NaN or an infinity, or whose max - lo FP32 cannot hold, is kept as NaN.
+ * Codes lie two a byte, the even value in the low half.
  * The call quantizes the new keys and values into their pages and computes o as
  * osh_window_attention does, with every key and value, the new ones too, as the cache
  * stands for it: o depends on the cache alone, not on how its tokens came in calls.  A query
@@ -725,8 +725,9 @@ OSH_API osh_status osh_window_attention(const osh_window_attn *p, void *d_scratc
  * From 512 rows a key head on (max_q * (q_heads / kv_heads)) bf16 calls take queries,
  * keys, values and weights in f16, times a power of two that puts the largest of a query, and a
  * head's largest visible key and value, between 1/2 and 1: what lies below 2^-14 of it keeps fewer
- * than f16's 11 bits.  A value that is not finite may make other queries of its sequence NaN, as
- * above.
+ * than f16's 11 bits; the scratch then holds what any sequence's queries see in f16, up to 16 GiB
+ * (where that would be more, the call goes as one of fewer rows).  A value that is not finite may
+ * make other queries of its sequence NaN, as above.
  * d_k_stored and d_v_stored (both or neither NULL) receive what the cache stands for at
  * the new tokens, rounded to dtype; rows that are not kept get NaN.
  * `w` holds sizes, pointers and strides as above, with codes for k_pages and v_pages and

@@ -826,8 +826,8 @@ static osh_status int4_launch(const Int4Args &p, const Int4Room &room, void *scr
                    (long long)room.pitch, (long long)room.plane);
     }
     OSH_LAUNCH_CHECK("int4_prep_kernel");
-    // 64 x 256 tiles where they fill the card, else 32 x 128 ones: 512 x 4096 x 4096 in bf16 takes
-    // 56 us as 128 large tiles, 35 as 512 small ones
+    // 64 x 256 tiles where they fill the card, else 32 x 128 ones: 512 x 4096 x 4096 in bf16 took
+    // 56 us as 128 large tiles, 35 as 512 small ones (now 32)
     if ((long long)cdiv(p.m, 64) * cdiv(p.n, 256) >= device_cus()) int4_tile<T, 2, 2, 1, 4, GS>(p, q, st);
     else int4_tile<T, 1, 1, 1, 4, GS>(p, q, st);
     OSH_LAUNCH_CHECK("int4_tile_kernel");

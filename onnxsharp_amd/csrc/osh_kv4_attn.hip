@@ -799,9 +799,9 @@ struct Kv4Room {
 };
 
 // Rows of a key head from which a bf16 call first expands the visible cache to f16, and the room
-// that may take.  4096 tokens behind 12288, 32 heads of 128 on 8, window 8192: 1470 us in blocks
-// of 16 rows, 690 so; 4 x 64 tokens (256 rows) behind 8128 122 in blocks.  f16 calls have no
-// type with bits to spare for it.
+// that may take.  4096 tokens behind 12288, 32 heads of 128 on 8, window 8192: 690 us so, 1726 as
+// f16 blocks of 16 rows (f16 has no type with bits to spare for it); behind 8128, 4 x 64 tokens
+// (256 rows) 125 in blocks, 4 x 127 224, 4 x 128 153 so.
 constexpr int WIDE_ROWS = 512;
 constexpr size_t WIDE_MAX = (size_t)16 << 30;
 
@@ -845,7 +845,7 @@ static osh_status kv4_plan(const osh_kv4_attn *p, Kv4Args &args, WinArgs &wide, 
         args.wide_blocks = 0;
     }
     // four or eight groups a head leave no registers for 16 rows' scores: 16 rows of 64 sequences
-    // of 5000 keys, 8 heads of 128 in groups of 32, take 465 us in one block (spilled), 250 in two
+    // of 5000 keys, 8 heads of 128 in groups of 32, took 465 us in one block (spilled) and take 242 in two
     const int groups = cdiv(p->w.head_dim, 128) * (p->w.head_dim <= 64 ? 64 : 128) / p->group;
     const int most = groups >= 8 ? 4 : groups >= 4 ? 8 : 16;
     a.tile_rows = std::min(most, rows <= 4 ? 4 : rows <= 8 ? 8 : 16);
