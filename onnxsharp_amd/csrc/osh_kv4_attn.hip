@@ -473,10 +473,10 @@ __global__ __launch_bounds__(64 * WAVES, CP > 4 ? 1 : 2) void kv4_rows_kernel(Kv
             if (bad) kp[e].x = __builtin_nanf("");
             if (!in) vp[e] = float2{0.0f, 0.0f};
             if constexpr (UNIT) {
-                float top = vp[e].x;
+                const float scale = vp[e].x;
                 vp[e].x *= by[e];
-                if (__builtin_amdgcn_ballot_w64(vp[e].x > 0x1p15f) != 0) {
-                    const float scale = top;
+                if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(vp[e].x) > 0x1p15f) != 0) {
+                    float top = __builtin_fabsf(scale);
 #pragma unroll
                     for (int i = 32; i; i >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, i));
                     const float next = __uint_as_float((263u << 23) - (__float_as_uint(top) & 0x7f800000u));

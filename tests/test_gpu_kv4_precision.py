@@ -9,7 +9,7 @@ little.  Both together stay below a tenth of r for keys and values of one size: 
 import pytest
 import torch
 
-from test_gpu_kv4_attention import make, ref, run
+from test_gpu_kv4_attention import check, make, ref, run
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,15 @@ def test_a_large_key_that_other_queries_see(cuda, where, dtype, power):
         r = float((out[i] - o[i]).norm() / (rounded[i] - o[i]).norm())
         print(where, dtype, power, i, r, flush=True)
         assert r <= 1.1
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,new,group", [(4, 1, 64), (8, 3, 32), (4, 60, 128), (8, 130, 64)])
+def test_scales_below_zero(cuda, hq, new, group, dtype):
+    # pages that another program filled from the largest value down: lo + scale code all the same
+    s = make(cuda, hq, 2, 128, group, 16, [(new, 700)], dtype, 9)
+    for codes, pairs in ((s["cache"].k_codes, s["cache"].k_scales), (s["cache"].v_codes, s["cache"].v_scales)):
+        codes.copy_(255 - codes)
+        pairs[..., 1] += 15 * pairs[..., 0]
+        pairs[..., 0].neg_()
+    check(s, None, 0)
